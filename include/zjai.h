@@ -559,6 +559,90 @@ int zjai_transformer_block_backward(zjai_ctx *ctx, const float *dout, int dim, i
                                     int heads, int h, int w, const zjai_tb_tape *tape,
                                     const zjai_tb_weights *wts, float *din, int mem);
 
+/* ---------------------------------------------------------------------------------------- */
+/* Training operators: 8-bit activation tapes and what reads them                             */
+/* ---------------------------------------------------------------------------------------- */
+
+/* Operators for training and refinement around the transformer blocks, next to the VJPs above.
+ * The reference has none of them (its tapes are f32 tensors, its refinement needs input gradients
+ * only). Maps are planar [n][c][h][w] of one element type, f32, f16 or bf16, contiguous and
+ * aligned to their element size; parameters and their gradients are f32. n, c, h, w >= 1,
+ * n * c < 2^31, h * w < 2^31 - 64. No output may overlap an input. Sums, statistics and products
+ * are held in f32 and reduced in a fixed order: the same call gives the same bits. Work and errors
+ * as for the other layer entries: ZJAI_MEM_DEVICE calls return once enqueued on the context's
+ * stream, their scratch comes from the context's arena (ZJAI_LIMIT_EXCEEDED when it is too small). */
+enum { ZJAI_F32 = 0, ZJAI_F16 = 1, ZJAI_BF16 = 2 };
+
+/* A map held in 8 bits: codes [n][c][h * w], and one exponent byte e per group of 32 consecutive
+ * positions of a channel row, exps [n][c][ceil(h * w / 32)]. A position's value is code * 2^e;
+ * e = clamp(floor(log2 max|x|) - 6, -126, 121) over the group, code = clamp(rint(x * 2^-e),
+ * -127, 127), so the error is at most 2^(e - 1) (2^e where |x| > 127 * 2^e); a group with an
+ * infinity or a NaN has e = 127 and codes 0, and stands for NaN. */
+typedef struct {
+  int8_t *codes;
+  int8_t *exps;
+} zjai_tape;
+
+/* x -> tape, and back (a tape's values are exact in bf16, and in f16 above its subnormals). */
+int zjai_tape_pack(zjai_ctx *ctx, const void *x, int dtype, int n, int c, int h, int w,
+                   const zjai_tape *tape, int mem);
+int zjai_tape_unpack(zjai_ctx *ctx, const zjai_tape *tape, int n, int c, int h, int w, void *x,
+                     int dtype, int mem);
+
+/* The residual step of a block whose branch gave f, with the norm after the block, its gate and
+ * residual scale, and the norm before the next block:
+ *   u = LN(f) * post_weight + post_bias (post_weight NULL: u = f)
+ *   y = x + scale * sigmoid(gate) * u (scale NULL: 1; gate_channels 0: no gate)
+ *   z = LN(y) * pre_weight + pre_bias (pre_weight NULL: no z)
+ * LN normalises over the channels of a position (zjai_layer_norm's, eps 1e-5). Parameters [c].
+ * gate holds gate_channels maps: c, or 1 (one logit per position for all channels). With
+ * everything NULL it is the block's plain residual; with pre alone it is the step between the
+ * halves of TransformerBlock::forward (attention.rs:328-372). c <= 8192. */
+typedef struct {
+  const float *post_weight, *post_bias;
+  const float *scale;
+  const float *pre_weight, *pre_bias;
+} zjai_residual_params;
+/* tapes: where to hold f, gate, y and z in 8 bits on the way (NULL codes: not held). Statistics
+ * and y's tape come from the f32 y, which is rounded to dtype only as it is stored. */
+typedef struct {
+  zjai_tape f, gate, y, z;
+} zjai_residual_tapes;
+int zjai_gated_residual_norm(zjai_ctx *ctx, const void *x, const void *f, const void *gate,
+                             int gate_channels, int dtype, int n, int c, int h, int w,
+                             const zjai_residual_params *prm, void *y, void *z,
+                             const zjai_residual_tapes *tapes, int mem);
+
+/* Its backward pass: dy and dz (NULL without pre) and the step's f, gate and y -> the gradients of
+ * its inputs (d_x, d_f, d_gate, in dtype) and parameters (f32), all on the values that are given:
+ * either maps of dtype, or 8-bit tapes (tapes not NULL; f, gate and y are then NULL). f is needed
+ * with post, scale or a gate, y with pre. d_x, and d_f (where f feeds the step through post, scale
+ * or a gate; else it equals d_x and may be NULL), and the gradients of what is present are
+ * required; the gradient of a one-channel gate is summed over the channels. */
+typedef struct {
+  void *x, *f, *gate;
+  float *post_weight, *post_bias, *scale, *pre_weight, *pre_bias;
+} zjai_residual_grads;
+int zjai_gated_residual_norm_backward(zjai_ctx *ctx, const void *dy, const void *dz, const void *f,
+                                      const void *gate, int gate_channels, const void *y,
+                                      const zjai_residual_tapes *tapes, int dtype, int n, int c,
+                                      int h, int w, const zjai_residual_params *prm,
+                                      const zjai_residual_grads *grads, int mem);
+
+/* The parameter gradients of a 1x1 convolution (`prep_conv1`, `ffn_in`, ... of the transformer
+ * block) from d_out [n][oc][h][w] and the 8-bit tape of its input [n][c][h][w]:
+ * dw[o][i] = sum over pictures and positions of d_out[o] * x[i] ([oc][c]), db[o] = sum of d_out[o]
+ * (db NULL: not wanted). */
+int zjai_conv1x1_weight_grad(zjai_ctx *ctx, const void *dout, int dtype, int n, int oc, int c,
+                             int h, int w, const zjai_tape *tape, float *dw, float *db, int mem);
+
+/* Ordering with a caller's stream, for callers whose buffers are in use on a stream other than the
+ * context's: after zjai_ctx_wait_stream the context's stream runs nothing more until the work
+ * enqueued on cuda_stream so far is done; after zjai_ctx_release_stream cuda_stream waits for the
+ * context's work so far. cuda_stream: a cudaStream_t (NULL: the legacy default stream). */
+int zjai_ctx_wait_stream(zjai_ctx *ctx, void *cuda_stream);
+int zjai_ctx_release_stream(zjai_ctx *ctx, void *cuda_stream);
+
 /* `math::layer_norm_channels` (math.rs:423-448), out of place. */
 int zjai_layer_norm(zjai_ctx *ctx, const float *x, int c, int h, int w, const float *weight,
                     const float *bias, float *out, int mem);

@@ -25,13 +25,15 @@ import ctypes
 
 import numpy as np
 
-from . import _lib
+from . import _lib, tape as _tape
+from .tape import STREAM_LEGACY, Tape
 from ._lib import (ACT_LEAKY, ACT_NONE, ACT_RELU, ACT_RELU6, ACT_SIGMOID, ANA_UV, ANA_Y, BOP,
                    HOP, ICCI, LATENT, SOP, SYN_UV, SYN_Y, ZjaiError, check)
 
 __all__ = ["Engine", "ZjaiError", "SOP", "BOP", "HOP", "SYN_Y", "SYN_UV", "ANA_Y", "ANA_UV",
            "ACT_NONE", "ACT_RELU", "ACT_LEAKY", "ACT_SIGMOID", "ACT_RELU6", "Network", "Stage",
            "LatentModel", "LATENT", "ICCI",
+           "Tape", "STREAM_LEGACY",
            "synthesis_tiles", "synth_out_size", "version"]
 
 _lib.lib()  # load now: importing the package without its CUDA library is an error
@@ -80,6 +82,7 @@ class Engine:
         check(_lib.lib().zjai_ctx_create(int(device), int(arena_bytes), ctypes.byref(h)))
         self.handle = h
         self.device = device
+        self.stream = None  # the caller's stream of set_stream, None: the context's own
 
     def close(self):
         if self.handle:
@@ -93,7 +96,10 @@ class Engine:
             pass
 
     def set_stream(self, cuda_stream_ptr):
+        """Work on the caller's CUDA stream (its handle as an int; STREAM_LEGACY for torch's default
+        stream); 0 or None restores the context's own."""
         check(_lib.lib().zjai_ctx_set_stream(self.handle, ctypes.c_void_p(cuda_stream_ptr)))
+        self.stream = cuda_stream_ptr or None
 
     def sync(self):
         check(_lib.lib().zjai_ctx_sync(self.handle))
@@ -322,6 +328,37 @@ class Engine:
         check(_lib.lib().zjai_cab_backward(self.handle, pd, c, h, w, ctypes.byref(t),
                                            ctypes.byref(wts), po, mem))
         return out
+
+    # ---- training operators: 8-bit tapes and what reads them (tape.py) --------------------
+    def tape_pack(self, x):
+        """Hold a map in 8 bits: x [(n,) c, h, w] -> Tape, one power-of-two scale per group of 32
+        positions of a channel row (error at most half a step; a step is 2^-6 of the group's
+        largest magnitude rounded down to a power of two)."""
+        return _tape.tape_pack(self, x)
+
+    def tape_unpack(self, tape, dtype=None):
+        """The map that a tape stands for, float32 or of `dtype` (bfloat16 holds it exactly)."""
+        return _tape.tape_unpack(self, tape, dtype)
+
+    def gated_residual_norm(self, x, f, post=None, gate=None, scale=None, pre=None, tape=()):
+        """The residual step of a block with branch output f, its norms, gate and scale fused:
+        y = x + scale . sigmoid(gate) . LN_post(f), z = LN_pre(y). x, f [(n,) c, h, w]; post and pre
+        (weight [c], bias [c]); gate like f or one channel; scale [c]; each may be None. `tape`
+        names what to hold in 8 bits on the way ("f", "gate", "y", "z"; parts the step lacks are
+        skipped). Returns (y, z or None, {name: Tape})."""
+        return _tape.gated_residual_norm(self, x, f, post, gate, scale, pre, tape)
+
+    def gated_residual_norm_backward(self, dy, dz=None, f=None, y=None, post=None, gate=None,
+                                     scale=None, pre=None):
+        """Its backward pass from dy, dz (with pre) and the step's f, gate and y, all as Tapes or
+        all as maps -> {"x", "f", "gate", "post_weight", "post_bias", "scale", "pre_weight",
+        "pre_bias"}: the gradients of what is present, on the values that are given."""
+        return _tape.gated_residual_norm_backward(self, dy, dz, f, y, post, gate, scale, pre)
+
+    def conv1x1_weight_grad(self, dout, tape):
+        """Parameter gradients of a 1x1 convolution from dout [(n,) oc, h, w] and the Tape of its
+        input [(n,) c, h, w]: (dw [oc, c], db [oc]), float32."""
+        return _tape.conv1x1_weight_grad(self, dout, tape)
 
     def layer_norm(self, x, weight, bias, out=None):
         c, h, w = x.shape

@@ -84,6 +84,23 @@ class TbWeights(ctypes.Structure):
                                    "attn_out", "ffn_norm", "ffn_in", "ffn_dw", "ffn_out")]
 
 
+class TapeC(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("exps", _vp)]
+
+
+class ResidualParams(ctypes.Structure):
+    _fields_ = [(k, _vp) for k in ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")]
+
+
+class ResidualTapes(ctypes.Structure):
+    _fields_ = [(k, TapeC) for k in ("f", "gate", "y", "z")]
+
+
+class ResidualGrads(ctypes.Structure):
+    _fields_ = [(k, _vp) for k in ("x", "f", "gate", "post_weight", "post_bias", "scale",
+                                   "pre_weight", "pre_bias")]
+
+
 _lib = None
 
 
@@ -199,6 +216,17 @@ def lib():
     L.zjai_depthwise3x3.argtypes = [_vp, _vp, _i, _i, _i, _vp, _vp, _i]
     L.zjai_depthwise3x3_elu_gate.argtypes = [_vp, _vp, _i, _i, _i, _vp, _vp, _i]
     L.zjai_transformer_ffn.argtypes = [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i]
+    _tp = ctypes.POINTER(TapeC)
+    L.zjai_tape_pack.argtypes = [_vp, _vp, _i, _i, _i, _i, _i, _tp, _i]
+    L.zjai_tape_unpack.argtypes = [_vp, _tp, _i, _i, _i, _i, _vp, _i, _i]
+    L.zjai_gated_residual_norm.argtypes = [_vp, _vp, _vp, _vp] + [_i] * 6 + [
+        ctypes.POINTER(ResidualParams), _vp, _vp, ctypes.POINTER(ResidualTapes), _i]
+    L.zjai_gated_residual_norm_backward.argtypes = [_vp, _vp, _vp, _vp, _vp, _i, _vp,
+                                                    ctypes.POINTER(ResidualTapes)] + [_i] * 5 + [
+        ctypes.POINTER(ResidualParams), ctypes.POINTER(ResidualGrads), _i]
+    L.zjai_conv1x1_weight_grad.argtypes = [_vp, _vp] + [_i] * 6 + [_tp, _vp, _vp, _i]
+    L.zjai_ctx_wait_stream.argtypes = [_vp, _vp]
+    L.zjai_ctx_release_stream.argtypes = [_vp, _vp]
     _dp = ctypes.POINTER(ctypes.c_double)
     L.zjai_conv_bench.argtypes = [_vp] + [_i] * 11 + [_dp, _dp]
     L.zjai_kernel_bench.argtypes = [_vp] + [_i] * 6 + [_dp, _dp]

@@ -146,6 +146,7 @@ int zjai_ctx_create(int device, size_t arena_bytes, zjai_ctx** out) {
       (st = cuda_check(cudaStreamCreateWithFlags(&c->stream2, cudaStreamNonBlocking), "stream")) ||
       (st = cuda_check(cudaEventCreateWithFlags(&c->ev_fork, cudaEventDisableTiming), "event")) ||
       (st = cuda_check(cudaEventCreateWithFlags(&c->ev_join, cudaEventDisableTiming), "event")) ||
+      (st = cuda_check(cudaEventCreateWithFlags(&c->ev_caller, cudaEventDisableTiming), "event")) ||
       (st = cuda_check(cudaMalloc(&c->arena.base, arena_bytes), "arena cudaMalloc")) ||
       (st = cuda_check(cudaMalloc(&c->d_err, 2 * sizeof(int)), "status cudaMalloc")) ||
       (st = cuda_check(cudaMemset(c->d_err, 0, 2 * sizeof(int)), "status memset")) ||
@@ -179,6 +180,7 @@ int zjai_ctx_destroy(zjai_ctx* ctx) {
   if (ctx->d_err) cudaFree(ctx->d_err);
   if (ctx->ev_fork) cudaEventDestroy(ctx->ev_fork);
   if (ctx->ev_join) cudaEventDestroy(ctx->ev_join);
+  if (ctx->ev_caller) cudaEventDestroy(ctx->ev_caller);
   for (cudaStream_t gs : ctx->group_streams) {
     cudaStreamSynchronize(gs);
     cudaStreamDestroy(gs);

@@ -76,6 +76,7 @@ struct Ctx {
   int sms = 148;
   cudaStream_t own = nullptr, stream = nullptr, stream2 = nullptr;
   cudaEvent_t ev_fork = nullptr, ev_join = nullptr;
+  cudaEvent_t ev_caller = nullptr;  // ordering with a caller's stream
   Arena arena;   // work of `stream`
   Arena arena2;  // work of `stream2` (chroma synthesis runs beside luma)
   Arena* cur_arena = nullptr;  // arena of the network runner currently launching (or null)
