@@ -109,7 +109,8 @@ static CUtensorMapSwizzle swizzle_for(int kc) {
 
 static int encode(Ctx* ctx, CUtensorMap* m, int rank, void* addr, const cuuint64_t* dims,
                   const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw,
-                  size_t span_bytes) {
+                  size_t span_bytes,
+                  CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16) {
   cuuint32_t es[5] = {1, 1, 1, 1, 1};
   if ((reinterpret_cast<uintptr_t>(addr) & 15) != 0)
     return fail(ZJAI_INVALID_ARGUMENT, "TMA base address not 16-byte aligned");
@@ -117,7 +118,7 @@ static int encode(Ctx* ctx, CUtensorMap* m, int rank, void* addr, const cuuint64
     if (strides[i] % 16 != 0)
       return fail(ZJAI_INVALID_ARGUMENT, "TMA stride not a multiple of 16 bytes");
   auto fn = reinterpret_cast<EncodeTiledFn>(ctx->encode_fn);
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, addr, dims, strides, box, es,
+  CUresult r = fn(m, type, rank, addr, dims, strides, box, es,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -158,6 +159,19 @@ int make_tile_map(Ctx* ctx, CUtensorMap* m, const TView& v, int bc, int bx, int 
   cuuint32_t box[4] = {(cuuint32_t)bc, (cuuint32_t)bx, (cuuint32_t)by, 1};
   return encode(ctx, m, 4, v.p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
                 (size_t)v.img * v.n * 2);
+}
+
+int make_planar_map(Ctx* ctx, CUtensorMap* m, const void* p, int elem, int npos, int rows, int n,
+                    int bp, int br, bool swizzle) {
+  cuuint64_t dims[3] = {(cuuint64_t)npos, (cuuint64_t)rows, (cuuint64_t)n};
+  cuuint64_t strides[2] = {(cuuint64_t)npos * elem, (cuuint64_t)npos * elem * rows};
+  cuuint32_t box[3] = {(cuuint32_t)bp, (cuuint32_t)br, 1};
+  return encode(ctx, m, 3, const_cast<void*>(p), dims, strides, box,
+                swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                (size_t)npos * elem * rows * n,
+                elem == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                            : CU_TENSOR_MAP_DATA_TYPE_UINT8);
 }
 
 int make_store_map(Ctx* ctx, CUtensorMap* m, const TView& v, int bx, int by) {

@@ -163,6 +163,10 @@ int make_act_map_s2(Ctx* ctx, CUtensorMap* m, const TView& v, int img, int kc, i
 // box [bc channels, bx, by] over an NHWC f16 view, no swizzle (shared-memory image
 // [by][bx][bc])
 int make_tile_map(Ctx* ctx, CUtensorMap* m, const TView& v, int bc, int bx, int by);
+// box [bp positions, br rows, 1 picture] over planar maps [n][rows][npos] of `elem`-byte elements
+// (rows a multiple of 16 bytes), rows of 128 bytes swizzled when `swizzle`
+int make_planar_map(Ctx* ctx, CUtensorMap* m, const void* p, int elem, int npos, int rows, int n,
+                    int bp, int br, bool swizzle);
 // output map of the TMA-store epilogue: box [16 channels, bx, by] over an NHWC f16 view
 int make_store_map(Ctx* ctx, CUtensorMap* m, const TView& v, int bx, int by);
 

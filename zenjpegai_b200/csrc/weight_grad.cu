@@ -15,15 +15,21 @@
 // accumulator of their own, and both are drained every kWindow positions and added, rounding to
 // nearest, to f32 sums in registers.
 //
-// One CTA per SM takes a 128 x N tile of dw over a range of positions:
-//  - 8 loader warps read both operands into registers a chunk ahead, convert, and store them in the
-//    128-byte-swizzled K-major layout the tensor core reads (16-byte piece j of row r at j ^ (r & 7));
-//    no TMA: its boxes cannot start at the odd row strides of planar maps, and all but bf16 d_out
-//    passes through registers anyway. They also sum d_out's rows for db;
+// One CTA per SM takes a 128 x N tile of dw over a range of positions, in chunks of 64:
+//  - the operands come to shared memory some chunks ahead: by TMA where all rows start on 16 bytes
+//    (kVec; bf16 d_out, which needs no conversion, straight into the operand), else by cp.async,
+//    each thread copying what it will itself convert (rows of odd length start anywhere, which a
+//    TMA box cannot);
+//  - 16 converter warps turn a chunk into bf16 in the 128-byte-swizzled K-major layout that the
+//    tensor core reads (16-byte piece j of row r at j ^ (r & 7)), and drain the accumulators, half
+//    a window after they are complete. They are what bounds the kernel below HBM's rate (issue
+//    slots), so a chunk is read, converted and stored in three strokes, with packed arithmetic;
 //  - one thread issues the MMAs of a chunk, alternating between two accumulator sets in TMEM;
-//  - 8 warps drain a finished set while the next one fills.
+//  - db comes from the converters' registers, or, where d_out does not pass through them, from a
+//    row of ones below the input's rows in the operand: one more column of the product.
 // Ranges of one tile are summed in order by a second kernel (no atomics). Every wait is bounded.
 #include <algorithm>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "train.h"
@@ -33,25 +39,52 @@ namespace {
 
 constexpr int kM = 128, kN = 128;       // tile of dw
 constexpr int kWindow = 256;            // positions between drains
-constexpr int kLoaderWarp = 8, kMmaWarp = 16;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
-constexpr int kBlock = kM * 64 * 2;     // 64 positions of 128 rows in bf16
+constexpr int kWorkers = 16, kMmaWarp = kWorkers, kTmaWarp = kWorkers + 1;
+constexpr int kWorkThreads = 32 * kWorkers;
+constexpr int kThreads = 32 * (kTmaWarp + 1);
+constexpr int kChunk = 64;                 // positions of a pipeline stage
+constexpr int kPerWindow = kWindow / kChunk;
+constexpr int kBlock = kM * kChunk * 2;    // a chunk of 128 rows in bf16
+constexpr int kOnes = 16 * kChunk * 2;     // and of the 16 rows with the ones
+constexpr int kBufCols = 256;              // TMEM columns of an accumulator set
 
-// bf16 terms of a d_out element, positions per pipeline stage, stages
-template <class T>
+// Per element type and alignment: bf16 terms of a d_out element; stages of converted operands,
+// chunks copied ahead of them (kAhead); 32-bit words a thread copies (cp.async) of 8 positions of
+// d_out (the words that hold them: one more where they start anywhere) and of 16 codes.
+template <bool kVec, class T>
 struct Form;
 template <>
-struct Form<float> {
-  static constexpr int kTerms = 3, kChunk = 64, kStages = 3;
+struct Form<true, float> {
+  static constexpr int kTerms = 3, kStages = 2, kAhead = 2, kRaw = 2 * kBlock + kBlock / 2;
 };
 template <>
-struct Form<__half> {
-  static constexpr int kTerms = 2, kChunk = 128, kStages = 2;
+struct Form<true, __half> {
+  static constexpr int kTerms = 2, kStages = 2, kAhead = 4, kRaw = kBlock + kBlock / 2;
 };
 template <>
-struct Form<__nv_bfloat16> {
-  static constexpr int kTerms = 1, kChunk = 128, kStages = 3;
+struct Form<true, __nv_bfloat16> {  // kRaw: the codes alone
+  static constexpr int kTerms = 1, kStages = 5, kAhead = 4, kRaw = kBlock / 2;
 };
+template <class T>
+struct Form<false, T> {
+  static constexpr int kTerms = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;
+  static constexpr int kStages = kTerms == 1 ? 3 : 2, kAhead = kTerms == 3 ? 2 : 3;
+  static constexpr int kWordsD = sizeof(T) == 4 ? 8 : 5, kWordsX = 5;
+  static constexpr int kRaw = (2 * kWordsD + kWordsX) * 4 * kWorkThreads;
+};
+template <bool kVec, class T>
+constexpr bool direct() {  // d_out is copied into the operand, the ones row gives db
+  return kVec && std::is_same<T, __nv_bfloat16>::value;
+}
+template <bool kVec, class T>
+constexpr int stage_bytes() {
+  return (Form<kVec, T>::kTerms + 1) * kBlock + (direct<kVec, T>() ? kOnes : 0);
+}
+template <bool kVec, class T>
+constexpr int smem_bytes() {
+  return 1024 + Form<kVec, T>::kStages * stage_bytes<kVec, T>() +
+         Form<kVec, T>::kAhead * Form<kVec, T>::kRaw;
+}
 
 struct WgArgs {
   const void* dout;
@@ -59,10 +92,10 @@ struct WgArgs {
   int oc, c, p, groups;
   int nb;          // N of the MMA: rows of the input tile, a multiple of 16
   int m_tiles;
+  long long d_elems, x_elems;  // of d_out and the codes
   int chunks_img;  // chunks per picture
   long long chunks;
   int splits;
-  int vec_d, vec_x;  // rows start on 16-byte boundaries
   float *dw, *db;    // [split][oc][c], [split][oc] (db null: not wanted)
   int* err;
   long long limit;
@@ -75,9 +108,8 @@ __device__ __forceinline__ float trunc_bf(float v) {
   return __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 // what truncation to bf16 left of v (none of an infinity; NaN stays NaN)
-__device__ __forceinline__ float rest_bf(float v) {
-  const float r = v - trunc_bf(v);
-  return fabsf(v) == __uint_as_float(0x7f800000u) ? 0.f : r;
+__device__ __forceinline__ float rest_bf_any(float v) {
+  return fabsf(v) == __uint_as_float(0x7f800000u) ? 0.f : v - trunc_bf(v);
 }
 
 __device__ __forceinline__ void st_shared16(uint32_t at, uint4 v) {
@@ -86,64 +118,95 @@ __device__ __forceinline__ void st_shared16(uint32_t at, uint4 v) {
                : "memory");
 }
 
-// 8 positions of a d_out row, raw
-template <class T>
-struct Raw {
-  uint4 v[sizeof(T) == 4 ? 2 : 1];
-};
-template <class T>
-__device__ __forceinline__ Raw<T> load_d(const T* row, int at, int p, bool ok, bool vec) {
-  Raw<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.v[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (!ok || at >= p) return r;
-  if (vec) {  // p is a multiple of 8 elements here: all eight are in
-    const uint4* q = reinterpret_cast<const uint4*>(row + at);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.v[i] = __ldg(q + i);
-    return r;
-  }
-  uint32_t e[8];
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = at + i < p ? __ldg(q + at + i) : 0u;
-    r.v[0] = make_uint4(e[0], e[1], e[2], e[3]);
-    r.v[sizeof(T) / 2 - 1] = make_uint4(e[4], e[5], e[6], e[7]);
-  } else {
-    const unsigned short* q = reinterpret_cast<const unsigned short*>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = at + i < p ? __ldg(q + at + i) : 0u;
-    r.v[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-  }
-  return r;
+__device__ __forceinline__ void ld_shared16(uint32_t at, uint32_t* w) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared4(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+// asynchronous copy to shared memory: the first `bytes` from src, zeros after them
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kNewer>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kNewer) : "memory");
 }
 
-// 16 codes of an input row and their exponent
-struct RawX {
-  uint4 v;
-  int e;
-};
-__device__ __forceinline__ RawX load_x(const int8_t* row, const int8_t* exps, int at, int p, bool ok,
-                                       bool vec) {
-  RawX r = {make_uint4(0u, 0u, 0u, 0u), 0};
-  if (!ok || at >= p) return r;
-  r.e = __ldg(exps + at / kTapeGroup);
-  if (vec) {
-    r.v = __ldg(reinterpret_cast<const uint4*>(row + at));
-    return r;
-  }
-  const uint8_t* q = reinterpret_cast<const uint8_t*>(row);
-  uint32_t w[4];
+// The five aligned words that hold the `valid` (0 to 16) bytes at q, word j to dst + j kWorkThreads
+// words; q may start anywhere. Words without a valid byte are zero. Nothing outside the tensor
+// [lo, hi) is read: a word that sticks out behind is copied as far as it goes, and the one that may
+// stick out before (the tensor's first) is put together from its bytes.
+__device__ __forceinline__ void copy_words5(uint32_t dst, const uint8_t* q, int valid,
+                                            const uint8_t* lo, const uint8_t* hi) {
+  const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3);
+  const uint8_t* a = q - off;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (at + 4 * i + j < p) w[i] |= (uint32_t)__ldg(q + at + 4 * i + j) << (8 * j);
+  for (int j = 0; j < 5; ++j) {
+    const uint8_t* at = a + 4 * j;
+    const uint32_t to = dst + j * 4 * kWorkThreads;
+    const bool want = 4 * j - off < valid;
+    if (j == 0 && want && at < lo) {
+      uint32_t w = 0u;
+      for (int i = 0; i < 4; ++i)
+        if (at + i >= lo && at + i < hi) w |= (uint32_t)__ldg(at + i) << (8 * i);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(w) : "memory");
+    } else {
+      const long long left = hi - at;
+      copy4(to, want ? at : lo + ((4 - (reinterpret_cast<uintptr_t>(lo) & 3)) & 3),
+            want ? (left < 4 ? (int)left : 4) : 0);
+    }
   }
-  r.v = make_uint4(w[0], w[1], w[2], w[3]);
-  return r;
+}
+// the 16 bytes in place, those from `valid` on zero
+__device__ __forceinline__ void place_words5(uint32_t src, const uint8_t* q, int valid,
+                                             uint32_t* v) {
+  const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(q) & 3) * 8;
+  uint32_t w[5];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) w[j] = ld_shared4(src + j * 4 * kWorkThreads);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = __funnelshift_r(w[j], w[j + 1], sh);
+    const int left = valid - 4 * j;
+    if (left < 4) v[j] = left <= 0 ? 0u : v[j] & (0xffffffffu >> (32 - 8 * left));
+  }
+}
+
+// One thread's piece of a chunk of d_out whose rows start anywhere, 8 positions of a row: the copy
+// to `raw` (the thread's place in a slot), and the words from there (8 f32, or 8 halves in 4).
+template <class T>
+__device__ __forceinline__ void copy_piece(uint32_t raw, const T* row, int at, int p, bool ok,
+                                           const T* lo, const T* hi) {
+  const int valid = ok ? max(0, min(8, p - at)) : 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      copy4(raw + i * 4 * kWorkThreads, i < valid ? row + at + i : lo, i < valid ? 4 : 0);
+  } else {
+    copy_words5(raw, reinterpret_cast<const uint8_t*>(row + at), 2 * valid,
+                reinterpret_cast<const uint8_t*>(lo), reinterpret_cast<const uint8_t*>(hi));
+  }
+}
+template <class T>
+__device__ __forceinline__ void get_piece(uint32_t raw, const T* row, int at, int p, bool ok,
+                                          uint32_t* w) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = ld_shared4(raw + i * 4 * kWorkThreads);
+  } else {
+    place_words5(raw, reinterpret_cast<const uint8_t*>(row + at),
+                 ok ? 2 * max(0, min(8, p - at)) : 0, w);
+  }
 }
 
 // 4 codes -> 4 bf16 values code 2^e: the low 7 bits and the sign bit of a code, each as the low
@@ -163,15 +226,18 @@ __device__ __forceinline__ uint2 taped_bf16(uint32_t w, __nv_bfloat162 scale) {
   return out;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const WgArgs a) {
-  using F = Form<T>;
-  constexpr int kTerms = F::kTerms, kSub = F::kChunk / 64, kStages = F::kStages;
-  constexpr int kStageBytes = (kTerms + 1) * kSub * kBlock;
-  constexpr int kPerWindow = kWindow / F::kChunk;
+template <bool kVec, class T>
+__global__ void __launch_bounds__(kThreads, 1)
+    weight_grad_kernel(const __grid_constant__ CUtensorMap map_d,
+                       const __grid_constant__ CUtensorMap map_x, const WgArgs a) {
+  using F = Form<kVec, T>;
+  constexpr int kTerms = F::kTerms, kStages = F::kStages, kAhead = F::kAhead, kRaw = F::kRaw;
+  constexpr int kStageBytes = stage_bytes<kVec, T>();
+  constexpr bool kDirect = direct<kVec, T>();
   constexpr int kSets = kTerms > 1 ? 2 : 1;  // accumulators of a set: first terms, the others
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 4 + 1];
+  // full / empty: operand stages; d_full: a stage's directly copied d_out; raw_*: copied chunks
+  __shared__ __align__(8) uint64_t bars[3 * kStages + 2 * kAhead + 4 + 1];
   __shared__ uint32_t tmem_at;
   __shared__ int abort_flag;
 
@@ -180,23 +246,43 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const WgArgs a
   const int o0 = (tile % a.m_tiles) * kM, i0 = (tile / a.m_tiles) * kN;
   const long long q0 = a.chunks * split / a.splits, q1 = a.chunks * (split + 1) / a.splits;
   const int count = (int)(q1 - q0), windows = (count + kPerWindow - 1) / kPerWindow;
+  const int img0 = (int)(q0 / a.chunks_img), in_img0 = (int)(q0 - (long long)img0 * a.chunks_img);
+  const bool want_db = a.db && i0 == 0;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages,
-                 acc_empty = acc_full + 16, drain = acc_empty + 16;
+  const uint32_t raw_base = smem + kStages * kStageBytes;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, d_full = empty + 8 * kStages,
+                 raw_full = d_full + 8 * kStages, raw_empty = raw_full + 8 * kAhead,
+                 acc_full = raw_empty + 8 * kAhead, acc_empty = acc_full + 16,
+                 drain = acc_empty + 16;
   volatile int* abort = &abort_flag;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + 8 * i, 8);
+      mbar_init(full + 8 * i, kWorkers);
       mbar_init(empty + 8 * i, 1);
+      mbar_init(d_full + 8 * i, 1);
+    }
+    for (int i = 0; i < kAhead; ++i) {
+      mbar_init(raw_full + 8 * i, 1);
+      mbar_init(raw_empty + 8 * i, kWorkers);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, 8);
+      mbar_init(acc_empty + 8 * i, kWorkers);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
+  }
+  if (kDirect && want_db) {
+    // the ones: row nb of each stage's input rows, the 15 rows behind it zero
+    for (int i = threadIdx.x; i < kStages * kOnes / 16; i += kThreads) {
+      const int st = i / (kOnes / 16), e = i % (kOnes / 16);
+      const uint32_t v = e < 8 ? 0x3f803f80u : 0u;
+      st_shared16(smem + st * kStageBytes + kTerms * kBlock + a.nb * 128 + e * 16,
+                  make_uint4(v, v, v, v));
+    }
+    fence_proxy_async_smem();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_at), 512);
@@ -209,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const WgArgs a
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
-      const uint32_t idesc = idesc_f16((uint32_t)a.nb) | (1u << 7) | (1u << 10);  // bf16 operands
+      const int n = kDirect && want_db ? a.nb + 16 : a.nb;
+      const uint32_t idesc = idesc_f16((uint32_t)n) | (1u << 7) | (1u << 10);  // bf16 operands
       bool ok = true;
       for (int k = 0; k < count && ok; ++k) {
         const int st = k % kStages, win = k / kPerWindow, buf = win & 1;
@@ -219,22 +306,22 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const WgArgs a
                          DEV_TIMEOUT_ACC_EMPTY, a.limit);
           if (!ok) break;
         }
+        if (kDirect) {
+          ok = mbar_wait(d_full + 8 * st, (k / kStages) & 1, abort, a.err, DEV_TIMEOUT_FULL, a.limit);
+          if (!ok) break;
+        }
         ok = mbar_wait(full + 8 * st, (k / kStages) & 1, abort, a.err, DEV_TIMEOUT_FULL, a.limit);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem + buf * kSets * kN;
+        const uint32_t d = tmem + buf * kBufCols, at = smem + st * kStageBytes;
+        const uint64_t db = smem_desc(at + kTerms * kBlock, 128u);
 #pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          const uint32_t at = smem + st * kStageBytes + s * (kTerms + 1) * kBlock;
-          const uint64_t db = smem_desc(at + kTerms * kBlock, 128u);
+        for (int t = 0; t < kTerms; ++t) {
+          const uint64_t da = smem_desc(at + t * kBlock, 128u);
 #pragma unroll
-          for (int t = 0; t < kTerms; ++t) {
-            const uint64_t da = smem_desc(at + t * kBlock, 128u);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 16 positions: 32 bytes along the row
-              umma_f16(d + (t ? kN : 0), da + 2 * kk, db + 2 * kk, idesc,
-                       first && s == 0 && t < 2 && kk == 0 ? 0u : 1u);
-          }
+          for (int kk = 0; kk < 4; ++kk)  // 16 positions: 32 bytes along the row
+            umma_f16(d + (t ? kN : 0), da + 2 * kk, db + 2 * kk, idesc,
+                     first && t < 2 && kk == 0 ? 0u : 1u);
         }
         umma_commit(empty + 8 * st);
         if (k % kPerWindow == kPerWindow - 1 || k == count - 1) umma_commit(acc_full + 8 * buf);
@@ -244,166 +331,302 @@ __global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const WgArgs a
       mbar_wait_drain(drain, 0, a.err);
     }
     __syncwarp();
-  } else if (warp >= kLoaderWarp) {
-    const int tid = threadIdx.x - kLoaderWarp * 32;
-    constexpr int kUd = 4 * kSub, kUx = 2 * kSub;
-    const T* dout = static_cast<const T*>(a.dout);
-    const int dr = tid >> 3, dj = tid & 7;  // d_out: row (of 32), 8 positions
-    const int xr = tid >> 2, xj = tid & 3;  // input: row (of 64), 16 positions
-    Raw<T> rd[kUd];
-    RawX rx[kUx];
-    float bsum[4] = {}, btot[4] = {};
-    const bool want_db = a.db && i0 == 0;
-    // the chunk being loaded: its picture and first position
-    long long img = q0 / a.chunks_img;
-    int at0 = (int)(q0 - img * a.chunks_img) * F::kChunk;
-    const T* pd = dout + (img * a.oc + o0 + dr) * (long long)a.p;
-    const int8_t* px = a.codes + (img * a.c + i0 + xr) * (long long)a.p;
-    const int8_t* pe = a.exps + (img * a.c + i0 + xr) * (long long)a.groups;
-    const long long d32 = 32LL * a.p, x64 = 64LL * a.p, e64 = 64LL * a.groups;
-    const int x_rows = min(a.nb, a.c - i0);
-    auto load_du = [&](int u) {
-      return load_d(pd + (u & 3) * d32, at0 + (u >> 2) * 64 + dj * 8, a.p,
-                    o0 + (u & 3) * 32 + dr < a.oc, a.vec_d);
+  } else if (warp == kTmaWarp) {
+    if (kVec && lane == 0) {
+      tma_prefetch_desc(&map_d);
+      tma_prefetch_desc(&map_x);
+      int img = img0, at = in_img0 * kChunk, k = 0;
+      for (; k < count; ++k) {
+        const int sl = k % kAhead, st = k % kStages;
+        if (k >= kAhead &&
+            !mbar_wait(raw_empty + 8 * sl, (k / kAhead - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
+                       a.limit))
+          break;
+        if (kDirect && k >= kStages &&
+            !mbar_wait(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
+                       a.limit))
+          break;
+        const uint32_t raw = raw_base + sl * kRaw, bar = raw_full + 8 * sl;
+        mbar_arrive_expect_tx(bar, kRaw);
+        if constexpr (kDirect) {
+          mbar_arrive_expect_tx(d_full + 8 * st, kBlock);
+          tma_load_3d(smem + st * kStageBytes, &map_d, d_full + 8 * st, at, o0, img);
+        } else {
+          tma_load_3d(raw, &map_d, bar, at, o0, img);
+          if constexpr (sizeof(T) == 4) tma_load_3d(raw + kBlock, &map_d, bar, at + 32, o0, img);
+        }
+        tma_load_3d(raw + kRaw - kBlock / 2, &map_x, bar, at, i0, img);
+        at += kChunk;
+        if (at >= a.p) {
+          at = 0;
+          ++img;
+        }
+      }
+      // all copies landed before the CTA goes, also after a wait that gave up
+      for (int j = max(0, k - kAhead); j < k; ++j)
+        mbar_wait_drain(raw_full + 8 * (j % kAhead), (j / kAhead) & 1, a.err);
+      if (kDirect)
+        for (int j = max(0, k - kStages); j < k; ++j)
+          mbar_wait_drain(d_full + 8 * (j % kStages), (j / kStages) & 1, a.err);
+    }
+    __syncwarp();
+  } else {
+    const int tid = threadIdx.x;
+    // d_out: rows dr and dr + 64, positions 8 dj ..; f32 from TMA: row dr, positions 8 dj .. of
+    // each half of the chunk, rows spread over a warp's lanes such that eight lanes' 16 bytes lie
+    // in different banks both as read (two pieces of four of a half row) and as stored
+    constexpr bool kHalves = kVec && sizeof(T) == 4;
+    const int l8 = lane >> 2;
+    const int dr = kHalves ? warp * 8 + ((l8 >> 1) ^ (l8 & 1 ? 5 : 0)) : tid >> 3;
+    const int dj = kHalves ? lane & 3 : tid & 7;
+    const int xr = tid >> 2, xj = tid & 3;  // input: row xr, positions 16 xj ..
+    const bool d_ok[2] = {o0 + dr < a.oc, o0 + 64 + dr < a.oc};
+    const bool x_ok = xr < min(a.nb, a.c - i0), x_in = xr < a.nb;
+    auto swizzled = [](uint32_t base, int r, int j) { return base + r * 128 + ((j ^ (r & 7)) << 4); };
+
+    // cp.async: the chunk being copied, and the one being converted
+    struct Place {
+      const T* d;
+      const uint8_t* x;
+      int at;
     };
-    auto load_xu = [&](int u) {
-      return load_x(px + (u & 1) * x64, pe + (u & 1) * e64, at0 + (u >> 1) * 64 + xj * 16, a.p,
-                    (u & 1) * 64 + xr < x_rows, a.vec_x);
+    const T* d_lo = static_cast<const T*>(a.dout);
+    const T* d_hi = d_lo + a.d_elems;
+    const uint8_t* x_lo = reinterpret_cast<const uint8_t*>(a.codes);
+    const uint8_t* x_hi = x_lo + a.x_elems;
+    const long long d64 = 64LL * a.p;
+    Place next = {d_lo + ((long long)img0 * a.oc + o0 + dr) * a.p,
+                  x_lo + ((long long)img0 * a.c + i0 + xr) * a.p, in_img0 * kChunk};
+    Place cur = next;
+    int copied = 0;
+    auto advance = [&](Place& pl) {
+      pl.at += kChunk;
+      if (pl.at >= a.p) {
+        pl.at = 0;
+        pl.d += (long long)a.oc * a.p;
+        pl.x += (long long)a.c * a.p;
+      }
     };
-    auto advance = [&]() {
-      at0 += F::kChunk;
-      if (at0 >= a.p) {
-        at0 = 0;
-        pd += (long long)a.oc * a.p;
-        px += (long long)a.c * a.p;
+    auto copy_chunk = [&]() {
+      if constexpr (!kVec) {
+        if (copied < count) {
+          const uint32_t raw = raw_base + copied % kAhead * kRaw + tid * 4;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            copy_piece<T>(raw + u * F::kWordsD * 4 * kWorkThreads, next.d + u * d64,
+                          next.at + dj * 8, a.p, d_ok[u], d_lo, d_hi);
+          const int at = next.at + xj * 16;
+          copy_words5(raw + 2 * F::kWordsD * 4 * kWorkThreads, next.x + at,
+                      x_ok ? max(0, min(16, a.p - at)) : 0, x_lo, x_hi);
+          ++copied;
+          advance(next);
+        }
+        copy_commit();
+      }
+    };
+    // what a chunk's exponents are taken from: a quad of lanes shares a row, and holds the row's 16
+    // exponent bytes of 8 chunks, 4 a lane, loaded 8 chunks ahead
+    const int8_t* pe = a.exps + ((long long)img0 * a.c + i0 + xr) * a.groups;
+    int exp_at = in_img0 & ~7;             // chunk in the picture of the window to load next
+    int exp_left = count + (in_img0 & 7);  // chunks from there on
+    uint32_t eb[4], ew = 0u;
+    auto load_exps = [&]() {
+      if (exp_left <= 0) return;
+      const int g0 = exp_at * 2 + xj * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        eb[i] = x_ok && g0 + i < a.groups ? (uint32_t)(uint8_t)__ldg(pe + g0 + i) : 0u;
+      exp_left -= min(8, a.chunks_img - exp_at);
+      exp_at += 8;
+      if (exp_at >= a.chunks_img) {
+        exp_at = 0;
         pe += (long long)a.c * a.groups;
       }
     };
+
+    // accumulator rows 32 (warp % 4) + lane, columns 32 (warp / 4) ..
+    float acc[32], acc_db = 0.f;
 #pragma unroll
-    for (int u = 0; u < kUd; ++u) rd[u] = load_du(u);
-#pragma unroll
-    for (int u = 0; u < kUx; ++u) rx[u] = load_xu(u);
-    for (int k = 0; k < count; ++k) {
-      const int st = k % kStages;
-      if (k >= kStages &&
-          !mbar_wait(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY, a.limit))
-        break;
-      const uint32_t stage = smem + st * kStageBytes;
-      const bool more = k + 1 < count;
-      advance();
-#pragma unroll
-      for (int u = 0; u < kUd; ++u) {
-        const int r = (u & 3) * 32 + dr;
-        const uint32_t at = stage + (u >> 2) * (kTerms + 1) * kBlock + r * 128 + ((dj ^ (r & 7)) << 4);
-        float s = 0.f;
-        if constexpr (kTerms == 1) {
-          st_shared16(at, rd[u].v[0]);
-          const uint32_t w[4] = {rd[u].v[0].x, rd[u].v[0].y, rd[u].v[0].z, rd[u].v[0].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s += __uint_as_float(w[i] << 16) + __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          float f[8];
-          if constexpr (kTerms == 2) {
-            const uint32_t w[4] = {rd[u].v[0].x, rd[u].v[0].y, rd[u].v[0].z, rd[u].v[0].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 t = __half22float2(reinterpret_cast<const __half2&>(w[i]));
-              f[2 * i] = t.x;
-              f[2 * i + 1] = t.y;
-            }
-          } else {
-            const uint4 v0 = rd[u].v[0], v1 = rd[u].v[sizeof(T) / 2 - 1];
-            const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) s += f[i] + f[i + 1];
-#pragma unroll
-          for (int t = 0; t < kTerms; ++t) {
-            st_shared16(at + t * kBlock, make_uint4(bf2(f[0], f[1]), bf2(f[2], f[3]), bf2(f[4], f[5]),
-                                                    bf2(f[6], f[7])));
-            if (t + 1 < kTerms)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = rest_bf(f[i]);
-          }
-        }
-        bsum[u & 3] += s;
-        if (more) rd[u] = load_du(u);
-      }
-#pragma unroll
-      for (int u = 0; u < kUx; ++u) {
-        const int r = (u & 1) * 64 + xr;
-        const uint32_t row = stage + ((u >> 1) * (kTerms + 1) + kTerms) * kBlock + r * 128;
-        const uint32_t sb = rx[u].e == kTapeNan ? 0x7fc0u : (uint32_t)(max(rx[u].e, -126) + 127) << 7;
-        const uint32_t s2 = sb | sb << 16;
-        const __nv_bfloat162 sc = reinterpret_cast<const __nv_bfloat162&>(s2);
-        const uint2 v0 = taped_bf16(rx[u].v.x, sc), v1 = taped_bf16(rx[u].v.y, sc);
-        const uint2 v2 = taped_bf16(rx[u].v.z, sc), v3 = taped_bf16(rx[u].v.w, sc);
-        if (r < a.nb) {
-          st_shared16(row + (((2 * xj) ^ (r & 7)) << 4), make_uint4(v0.x, v0.y, v1.x, v1.y));
-          st_shared16(row + (((2 * xj + 1) ^ (r & 7)) << 4), make_uint4(v2.x, v2.y, v3.x, v3.y));
-        }
-        if (more) rx[u] = load_xu(u);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * st);
-      if ((k & 31) == 31)  // two levels: chains of 32 chunks, and of the chains
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          btot[i] += bsum[i];
-          bsum[i] = 0.f;
-        }
-    }
-    if (want_db) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float s = btot[i] + bsum[i];
-#pragma unroll
-        for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const int row = o0 + i * 32 + dr;
-        if (dj == 0 && row < a.oc) a.db[(long long)split * a.oc + row] = s;
-      }
-    }
-  } else {
-    // warp w: rows 32 (w % 4) + lane of the tile, columns 64 (w / 4) ..
-    float acc[64];
-#pragma unroll
-    for (int j = 0; j < 64; ++j) acc[j] = 0.f;
-    const int c0 = (warp >> 2) * 64;
-    const uint32_t base = tmem + ((uint32_t)(warp & 3) * 32u << 16) + c0;
-    bool ok = true;
-    for (int w = 0; w < windows && ok; ++w) {
-      const int buf = w & 1;
-      ok = mbar_wait_sleep(acc_full + 8 * buf, (w >> 1) & 1, abort, a.err, DEV_TIMEOUT_ACC_FULL,
-                           a.limit);
-      if (!ok) break;
+    for (int j = 0; j < 32; ++j) acc[j] = 0.f;
+    const int c0 = (warp >> 2) * 32;
+    int drained = 0;
+    auto drain_window = [&]() {
+      const int buf = drained & 1;
+      if (!mbar_wait_sleep(acc_full + 8 * buf, (drained >> 1) & 1, abort, a.err,
+                           DEV_TIMEOUT_ACC_FULL, a.limit))
+        return false;
       tc_fence_after();
       __syncwarp();
+      const uint32_t base = tmem + ((uint32_t)(warp & 3) * 32u << 16) + buf * kBufCols;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         if (c0 + j * 16 < a.nb) {
-          const uint32_t at = base + buf * kSets * kN + j * 16;
 #pragma unroll
           for (int set = kSets - 1; set >= 0; --set) {
             float v[16];
-            tmem_ld16(at + set * kN, v);
+            tmem_ld16(base + set * kN + c0 + j * 16, v);
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[j * 16 + i] += v[i];
           }
         }
       }
+      if (kDirect && want_db && c0 == 0) {
+        float v[16];
+        tmem_ld16(base + a.nb, v);
+        acc_db += v[0];
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+      ++drained;
+      return true;
+    };
+    constexpr int kRows = kHalves ? 1 : 2;
+    float2 bsum[kRows] = {};
+    float btot[kRows] = {};
+
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) copy_chunk();
+    load_exps();
+    int in = in_img0;  // the chunk's place in its picture
+    bool fresh = true, ok = true;
+    for (int k = 0; k < count && ok; ++k) {
+      const int st = k % kStages, sl = k % kAhead;
+      const uint32_t stage = smem + st * kStageBytes;
+      const uint32_t raw = raw_base + sl * kRaw;
+      // read
+      uint32_t wd[2][2 * sizeof(T)], wx[4];
+      if constexpr (kVec) {
+        ok = mbar_wait_sleep(raw_full + 8 * sl, (k / kAhead) & 1, abort, a.err, DEV_TIMEOUT_FULL,
+                             a.limit);
+        if (!ok) break;
+        ld_shared16(raw + kRaw - kBlock / 2 + xr * 64 + xj * 16, wx);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if constexpr (kHalves) {
+            ld_shared16(swizzled(raw + u * kBlock, dr, 2 * dj), wd[u]);
+            ld_shared16(swizzled(raw + u * kBlock, dr, 2 * dj + 1), wd[u] + 4);
+          } else if constexpr (!kDirect) {
+            ld_shared16(swizzled(raw, u * 64 + dr, dj), wd[u]);
+          }
+        }
+      } else {
+        copy_wait<kAhead - 1>();
+        const uint32_t mine = raw + tid * 4;
+        const int at = cur.at + xj * 16;
+        place_words5(mine + 2 * F::kWordsD * 4 * kWorkThreads, cur.x + at,
+                     x_ok ? max(0, min(16, a.p - at)) : 0, wx);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          get_piece<T>(mine + u * F::kWordsD * 4 * kWorkThreads, cur.d + u * d64, cur.at + dj * 8,
+                       a.p, d_ok[u], wd[u]);
+        advance(cur);
+      }
+      if (fresh || (in & 7) == 0) {
+        ew = eb[0] | eb[1] << 8 | eb[2] << 16 | eb[3] << 24;
+        load_exps();
+        fresh = false;
+      }
+      const int g = 2 * (in & 7) + (xj >> 1);
+      const int e = (int)(int8_t)(__shfl_sync(0xffffffffu, ew, (lane & ~3) + (g >> 2)) >> (8 * (g & 3)));
+      if (++in == a.chunks_img) in = 0;
+      // convert
+      const uint32_t sb = e == kTapeNan ? 0x7fc0u : (uint32_t)(max(e, -126) + 127) << 7;
+      const uint32_t s2 = sb | sb << 16;
+      const __nv_bfloat162 sc = reinterpret_cast<const __nv_bfloat162&>(s2);
+      const uint2 v0 = taped_bf16(wx[0], sc), v1 = taped_bf16(wx[1], sc);
+      const uint2 v2 = taped_bf16(wx[2], sc), v3 = taped_bf16(wx[3], sc);
+      if constexpr (kVec) {  // the slot is read out once its words are used
+        __syncwarp();
+        if (kDirect && lane == 0) mbar_arrive(raw_empty + 8 * sl);
+      }
+      if (k >= kStages) {
+        ok = mbar_wait_sleep(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
+                             a.limit);
+        if (!ok) break;
+      }
+      if (x_in) {
+        const uint32_t to = stage + kTerms * kBlock;
+        st_shared16(swizzled(to, xr, 2 * xj), make_uint4(v0.x, v0.y, v1.x, v1.y));
+        st_shared16(swizzled(to, xr, 2 * xj + 1), make_uint4(v2.x, v2.y, v3.x, v3.y));
+      }
+      if constexpr (!kDirect) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t at = kHalves ? swizzled(stage, dr, 4 * u + dj)
+                                      : swizzled(stage, u * 64 + dr, dj);
+          const uint32_t* w = wd[u];
+          float2 f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4)
+              f[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            else if constexpr (kTerms == 2)
+              f[i] = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+            else
+              f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+          }
+          const float2 s = __fadd2_rn(__fadd2_rn(f[0], f[1]), __fadd2_rn(f[2], f[3]));
+          bsum[u % kRows] = __fadd2_rn(bsum[u % kRows], s);
+          if constexpr (kTerms == 1) {
+            st_shared16(at, make_uint4(w[0], w[1], w[2], w[3]));
+          } else {
+            const bool finite = fabsf(s.x + s.y) < __uint_as_float(0x7f800000u);
+#pragma unroll
+            for (int t = 0; t < kTerms; ++t) {
+              st_shared16(at + t * kBlock, make_uint4(bf2(f[0].x, f[0].y), bf2(f[1].x, f[1].y),
+                                                      bf2(f[2].x, f[2].y), bf2(f[3].x, f[3].y)));
+              if (t + 1 == kTerms) continue;
+              if (finite) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  f[i] = __fadd2_rn(f[i], make_float2(-trunc_bf(f[i].x), -trunc_bf(f[i].y)));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  f[i] = make_float2(rest_bf_any(f[i].x), rest_bf_any(f[i].y));
+              }
+            }
+          }
+        }
+      }
+      copy_chunk();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full + 8 * st);
+        if (kVec && !kDirect) mbar_arrive(raw_empty + 8 * sl);
+      }
+      if (!kDirect && (k & 31) == 31) {  // two levels: chains of 32 chunks, and of the chains
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          btot[i] += bsum[i].x + bsum[i].y;
+          bsum[i] = make_float2(0.f, 0.f);
+        }
+      }
+      if (k % kPerWindow == kPerWindow / 2 && k >= kPerWindow) ok = drain_window();
     }
+    if (!kVec) copy_wait<0>();
+    while (ok && drained < windows) ok = drain_window();
     const int o = o0 + (warp & 3) * 32 + lane;
+    if (want_db) {
+      float* db = a.db + (long long)split * a.oc;
+      if constexpr (kDirect) {
+        if (c0 == 0 && o < a.oc) db[o] = acc_db;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          float s = btot[i] + (bsum[i].x + bsum[i].y);
+#pragma unroll
+          for (int x = kHalves ? 2 : 4; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+          if (dj == 0 && d_ok[i]) db[o0 + i * 64 + dr] = s;
+        }
+      }
+    }
     if (o < a.oc) {
       float* out = a.dw + ((long long)split * a.oc + o) * a.c + i0 + c0;
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < 32; ++j)
         if (i0 + c0 + j < a.c) out[j] = acc[j];
     }
   }
@@ -483,9 +706,10 @@ extern "C" int zjai_conv1x1_weight_grad(zjai_ctx* ctx, const void* dout, int dty
     auto aligned = [&](const void* q, size_t row) {
       return reinterpret_cast<uintptr_t>(q) % 16 == 0 && row % 16 == 0;
     };
+    // rows on 16-byte boundaries, and 16 positions of the codes all in a row or past it
+    const bool vec = aligned(dd, (size_t)p * es) && aligned(dc, (size_t)p);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      using F = Form<T>;
       WgArgs a = {};
       a.dout = dd;
       a.codes = dc;
@@ -496,12 +720,11 @@ extern "C" int zjai_conv1x1_weight_grad(zjai_ctx* ctx, const void* dout, int dty
       a.groups = (int)groups;
       a.nb = c >= kN ? kN : (c + 15) / 16 * 16;
       a.m_tiles = (int)m_tiles;
-      a.chunks_img = (p + F::kChunk - 1) / F::kChunk;
+      a.d_elems = (long long)n * oc * p;
+      a.x_elems = (long long)n * c * p;
+      a.chunks_img = (p + kChunk - 1) / kChunk;
       a.chunks = (long long)n * a.chunks_img;
       a.splits = choose_splits(tiles, a.chunks, ctx->sms);
-      // eight elements at a time: rows of 16 bytes and of eight elements
-      a.vec_d = aligned(dd, (size_t)p * es) && p % 8 == 0;
-      a.vec_x = aligned(dc, (size_t)p);
       a.dw = ow;
       a.db = ob;
       a.err = ctx->d_err;
@@ -512,11 +735,18 @@ extern "C" int zjai_conv1x1_weight_grad(zjai_ctx* ctx, const void* dout, int dty
         if (!a.dw || (ob && !a.db))
           return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (weight gradient)");
       }
-      const int smem = 1024 + F::kStages * (F::kTerms + 1) * (F::kChunk / 64) * kBlock;
-      ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)weight_grad_kernel<T>,
+      CUtensorMap md = {}, mx = {};
+      if (vec) {
+        // d_out in boxes of 128 rows of 128 bytes, swizzled; the codes in boxes of 128 rows of 64
+        ZJAI_TRY(make_planar_map(ctx, &md, dd, (int)es, p, oc, n, 128 / (int)es, kM, true));
+        ZJAI_TRY(make_planar_map(ctx, &mx, dc, 1, p, c, n, kChunk, kN, false));
+      }
+      auto k = vec ? weight_grad_kernel<true, T> : weight_grad_kernel<false, T>;
+      const int smem = vec ? smem_bytes<true, T>() : smem_bytes<false, T>();
+      ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                           me));
-      weight_grad_kernel<T><<<dim3((unsigned)tiles, a.splits), kThreads, smem, ctx->stream>>>(a);
+      k<<<dim3((unsigned)tiles, a.splits), kThreads, smem, ctx->stream>>>(md, mx, a);
       ctx->launches++;
       if (a.splits > 1) {
         auto sum = [&](const float* part, long long e, float* out) {
