@@ -8,14 +8,19 @@
 //   du = D q, dg = D s u sigma(g) (1 - sigma(g)), ds = sum D sigma(g) u
 //   b = du w1, df = (b - mean b - fn mean(b fn)) r1
 //   dw1 = sum du fn, db1 = sum du, dw2 = sum dz yn, db2 = sum dz             (sums over positions)
-// Maps are planar: a channel row holds a picture's positions. A block takes a tile of 32
-// consecutive positions of one picture, which are one group of each row's 8-bit tape: lane =
-// position, the channels spread over the warps, a position's sums gathered over the warps in
-// shared memory. Variances are two-pass (the mean first; one pass would cancel), and the second pass
-// also sums the deviations, which corrects the mean's own rounding: a normalised value near zero
-// keeps its relative precision. The products in a - mean a and b - mean b are the ones that were
-// summed (no fused multiply-add): with one channel they cancel to zero.
+// Maps are planar: a channel row holds a picture's positions. A block takes tiles of 32 consecutive
+// positions of one picture, which are one group of each row's 8-bit tape. A lane has four
+// neighbouring positions, eight lanes a row, a warp four rows at a time: vector loads and stores,
+// packed f32x2 arithmetic, and a group's maximum within eight lanes (one position a lane needed
+// three times the instructions, and issue slots bounded the kernels, not HBM). Up to 256 channels
+// a block holds its tile in registers (kRows rows a thread) and reads everything once; above, rows
+// are read again for each pass, mostly from the caches. A position's sums go over the warps'
+// shared-memory partials, gathered by one warp. Statistics: a mean and sum of squared deviations
+// per warp, joined by their exact update formula (sums of squares would cancel).
+// The products in a - mean a and b - mean b are the ones that were summed (not fused): with one
+// channel they cancel to zero. Both kernels are bound by HBM at large sizes.
 #include <algorithm>
+#include <type_traits>
 
 #include "train.h"
 
@@ -24,7 +29,8 @@ namespace {
 
 constexpr float kEps = 1e-5f;
 constexpr int kMaxC = 8192;  // the parameter sums of a block sit in shared memory, 20 B a channel
-constexpr int kWarps = 8;
+constexpr int kMaxWarps = 16;
+constexpr int kVecs = 4;  // positions of a lane
 
 template <class T>
 struct FwdArgs {
@@ -47,247 +53,569 @@ struct BwdArgs {
   float* sums;  // [blocks][5][c]: scale, post_weight, post_bias, pre_weight, pre_bias
 };
 
+// Four neighbouring positions, as two packed pairs.
+struct F4 {
+  float2 a, b;
+};
+__device__ __forceinline__ F4 operator+(F4 x, F4 y) {
+  return {__fadd2_rn(x.a, y.a), __fadd2_rn(x.b, y.b)};
+}
+__device__ __forceinline__ F4 operator*(F4 x, F4 y) {
+  return {__fmul2_rn(x.a, y.a), __fmul2_rn(x.b, y.b)};
+}
+__device__ __forceinline__ F4 fma4(F4 x, F4 y, F4 z) {
+  return {__ffma2_rn(x.a, y.a, z.a), __ffma2_rn(x.b, y.b, z.b)};
+}
+__device__ __forceinline__ F4 all(float v) {
+  return {make_float2(v, v), make_float2(v, v)};
+}
+__device__ __forceinline__ F4 operator-(F4 x) {
+  return {make_float2(-x.a.x, -x.a.y), make_float2(-x.b.x, -x.b.y)};
+}
+__device__ __forceinline__ F4 operator-(F4 x, F4 y) { return x + (-y); }
+__device__ __forceinline__ F4 make4(float4 v) {
+  return {make_float2(v.x, v.y), make_float2(v.z, v.w)};
+}
+__device__ __forceinline__ float4 flat(F4 v) { return make_float4(v.a.x, v.a.y, v.b.x, v.b.y); }
+
+// four positions from row pointer + at, zeros behind the row's end; kVec: all in or out, aligned
+template <bool kVec, class T>
+__device__ __forceinline__ F4 load4(const T* row, int at, int p) {
+  if constexpr (kVec) {
+    if (at >= p) return all(0.f);
+    if constexpr (sizeof(T) == 4) {
+      return make4(__ldg(reinterpret_cast<const float4*>(row + at)));
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + at));
+      if constexpr (std::is_same<T, __half>::value)
+        return {__half22float2(reinterpret_cast<const __half2&>(w.x)),
+                __half22float2(reinterpret_cast<const __half2&>(w.y))};
+      else
+        return {make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u)),
+                make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u))};
+    }
+  } else {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = at + i < p ? to_f32(row[at + i]) : 0.f;
+    return {make_float2(v[0], v[1]), make_float2(v[2], v[3])};
+  }
+}
+template <bool kVec, class T>
+__device__ __forceinline__ void store4(T* row, int at, int p, F4 v) {
+  if constexpr (kVec) {
+    if (at >= p) return;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + at) = flat(v);
+    } else {
+      uint2 w;
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 x = __float22half2_rn(v.a), y = __float22half2_rn(v.b);
+        w = make_uint2(reinterpret_cast<const uint32_t&>(x), reinterpret_cast<const uint32_t&>(y));
+      } else {
+        const __nv_bfloat162 x = __float22bfloat162_rn(v.a), y = __float22bfloat162_rn(v.b);
+        w = make_uint2(reinterpret_cast<const uint32_t&>(x), reinterpret_cast<const uint32_t&>(y));
+      }
+      *reinterpret_cast<uint2*>(row + at) = w;
+    }
+  } else {
+    const float f[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i < p) row[at + i] = from_f32<T>(f[i]);
+  }
+}
+// codes of four positions as a word, and back to values
+template <bool kVec>
+__device__ __forceinline__ uint32_t load_codes(const int8_t* row, int at, int p) {
+  if constexpr (kVec) return at < p ? __ldg(reinterpret_cast<const uint32_t*>(row + at)) : 0u;
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < p) w |= (uint32_t)(uint8_t)__ldg(row + at + i) << (8 * i);
+  return w;
+}
+__device__ __forceinline__ F4 taped4(uint32_t codes, int e) {
+  const uint32_t w = codes ^ 0x80808080u;
+  const F4 off = all(-8388736.f);  // see tape_value
+  const F4 v = {make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)),
+                            __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441))),
+                make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)),
+                            __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)))};
+  return (v + off) * all(tape_scale(e));
+}
+
 // sigmoid(g) and 1 - sigmoid(g), neither by cancellation and both finite for every g but NaN
 __device__ __forceinline__ void sigmoid2(float g, float* s, float* one_minus) {
-  const float a = expf(-fabsf(g)), r = 1.f / (1.f + a), ar = a * r;
-  *s = g >= 0.f ? r : (g < 0.f ? ar : g);
-  *one_minus = g >= 0.f ? ar : (g < 0.f ? r : g);
+  const float a = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + a), ar = a * r;
+  *s = g >= 0.f ? r : ar;
+  *one_minus = g >= 0.f ? ar : r;
+}
+__device__ __forceinline__ void sigmoid4(F4 g, F4* s, F4* one_minus) {
+  sigmoid2(g.a.x, &s->a.x, &one_minus->a.x);
+  sigmoid2(g.a.y, &s->a.y, &one_minus->a.y);
+  sigmoid2(g.b.x, &s->b.x, &one_minus->b.x);
+  sigmoid2(g.b.y, &s->b.y, &one_minus->b.y);
 }
 
-// A position's mean over the channels (m, and what its rounding left, dm) and 1 / sigma.
-struct Stats {
-  float m = 0.f, dm = 0.f, r = 1.f;
-  // from the means of v - m and (v - m)^2
-  __device__ __forceinline__ void finish(float d, float sq) {
-    dm = d;
-    r = 1.f / sqrtf(fmaxf(sq - d * d, 0.f) + kEps);
+// over the four rows of a warp: lanes with the same positions
+__device__ __forceinline__ F4 over_rows(F4 v) {
+  float f[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] += __shfl_xor_sync(0xffffffffu, f[i], 8);
+    f[i] += __shfl_xor_sync(0xffffffffu, f[i], 16);
   }
-  __device__ __forceinline__ float norm(float v) const { return ((v - m) - dm) * r; }
+  return {make_float2(f[0], f[1]), make_float2(f[2], f[3])};
+}
+
+// Hold four positions of a row (zeros behind its end) as part of a tape's group; the row's eight
+// lanes call together (`on`: the row exists).
+template <bool kVec>
+__device__ __forceinline__ void tape_store4(const zjai_tape& t, long long row, int groups, int g,
+                                            int at, int p, F4 v, bool on) {
+  const uint32_t b[4] = {__float_as_uint(v.a.x), __float_as_uint(v.a.y), __float_as_uint(v.b.x),
+                         __float_as_uint(v.b.y)};
+  uint32_t m = max(max(b[0] & 0x7fffffffu, b[1] & 0x7fffffffu),
+                   max(b[2] & 0x7fffffffu, b[3] & 0x7fffffffu));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (!on) return;
+  const int e = tape_exp(m);
+  uint32_t w;
+  // only the largest 1 / 128 of magnitudes can round to 128, and only a marked group has no codes
+  if ((m & 0x7fffffu) < 0x7f0000u && m < 0x7f800000u) {
+    const F4 c = fma4(v, all(tape_inv_scale(e)), all(12582912.f));
+    w = __byte_perm(__byte_perm(__float_as_uint(c.a.x), __float_as_uint(c.a.y), 0x0040),
+                    __byte_perm(__float_as_uint(c.b.x), __float_as_uint(c.b.y), 0x0040), 0x5410);
+  } else {
+    w = 0u;
+    if (e != kTapeNan) {
+      const float inv = tape_inv_scale(e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w |= (tape_code_bits(__uint_as_float(b[i]), inv) & 0xffu) << (8 * i);
+    }
+  }
+  int8_t* codes = t.codes + row * p;
+  if constexpr (kVec) {
+    if (at < p) *reinterpret_cast<uint32_t*>(codes + at) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i < p) codes[at + i] = (int8_t)(w >> (8 * i) & 0xffu);
+  }
+  if ((threadIdx.x & 7) == 0) t.exps[row * groups + g] = (int8_t)e;
+}
+
+// The block's partial sums per warp and position, and their totals.
+template <int kVals>
+struct Exchange {
+  float part[kMaxWarps][kVals][32], total[kVals][32];
 };
 
-// Sum of v over the block's warps, per lane, in warp order.
-__device__ __forceinline__ float over_warps(float v, float (*red)[32]) {
-  const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
-  __syncthreads();
-  red[wp][lane] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) s += red[k][lane];
-  return s;
-}
+// Rows of the calling thread: row(j) for j < rows(). kRows > 0: held in registers, consecutive
+// groups of four per warp; 0: any number, strided over the block.
+template <int kRows>
+struct Rows {
+  int c, first, step, n, warp_rows;
+  __device__ __forceinline__ Rows(int c_, int warps) : c(c_) {
+    const int wp = threadIdx.x >> 5, rg = (threadIdx.x & 31) >> 3;
+    if (kRows) {
+      first = wp * 4 * kRows + rg;
+      step = 4;
+      n = kRows;
+      warp_rows = max(0, min(c - wp * 4 * kRows, 4 * kRows));
+    } else {
+      first = wp * 4 + rg;
+      step = 4 * warps;
+      n = (c + step - 1) / step;
+      const int whole = c / step, rest = c - whole * step - wp * 4;
+      warp_rows = whole * 4 + max(0, min(4, rest));
+    }
+  }
+  __device__ __forceinline__ int row(int j) const { return first + j * step; }
+  __device__ __forceinline__ bool on(int j) const { return row(j) < c; }
+  // a row that exists, to read for one that does not
+  __device__ __forceinline__ int param(int j) const { return min(row(j), c - 1); }
+};
+#define FOR_ROWS(j) _Pragma("unroll") for (int j = 0; j < (kRows ? kRows : rows.n); ++j)
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Per warp the sum and the squared deviations from the warp's own mean of v(j), to ex.part at val,
+// val + 1.
+template <int kRows, int kVals, class V>
+__device__ __forceinline__ void stats_part(const Rows<kRows>& rows, V&& v, Exchange<kVals>& ex,
+                                           int val) {
+  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  F4 s = all(0.f), q = all(0.f);
+  FOR_ROWS(j) if (rows.on(j)) s = s + v(j);
+  s = over_rows(s);
+  const F4 m = s * all(rows.warp_rows ? 1.f / (float)rows.warp_rows : 0.f);
+  FOR_ROWS(j) if (rows.on(j)) {
+    const F4 d = v(j) - m;
+    q = fma4(d, d, q);
+  }
+  q = over_rows(q);
+  if (lane < 8) {
+    *reinterpret_cast<float4*>(&ex.part[wp][val][lane * 4]) = flat(s);
+    *reinterpret_cast<float4*>(&ex.part[wp][val + 1][lane * 4]) = flat(q);
+  }
 }
-
-// Hold a value per lane (0 beyond the row's end) as the group of a tape: row, group index.
-__device__ __forceinline__ void tape_group_store(const zjai_tape& t, long long row, int groups,
-                                                 int g, int p, float v, bool in) {
+// Joined by one warp: ex.total at val, val + 1 the mean and 1 / sigma.
+template <int kRows, int kVals>
+__device__ __forceinline__ void stats_join(Exchange<kVals>& ex, int val, int c, int warps) {
   const int lane = threadIdx.x & 31;
-  const int e = tape_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-  const uint32_t code = e == kTapeNan ? 0u : tape_code_bits(v, tape_inv_scale(e));
-  if (in) t.codes[row * p + g * kTapeGroup + lane] = (int8_t)(code & 0xffu);
-  if (lane == 0) t.exps[row * groups + g] = (int8_t)e;
+  float s = 0.f, q = 0.f;
+  for (int w = 0; w < warps; ++w) s += ex.part[w][val][lane];
+  const float m = s / (float)c;
+  for (int w = 0; w < warps; ++w) {
+    // rows of warp w, as in Rows
+    int n;
+    if (kRows) {
+      n = max(0, min(c - w * 4 * kRows, 4 * kRows));
+    } else {
+      const int whole = c / (4 * warps);
+      n = whole * 4 + max(0, min(4, c - whole * 4 * warps - w * 4));
+    }
+    if (!n) continue;
+    const float d = ex.part[w][val][lane] / (float)n - m;
+    q += ex.part[w][val + 1][lane] + (float)n * d * d;
+  }
+  ex.total[val][lane] = m;
+  ex.total[val + 1][lane] = rsqrtf(q / (float)c + kEps);
+}
+template <int kVals>
+__device__ __forceinline__ F4 total4(const Exchange<kVals>& ex, int val) {
+  return make4(*reinterpret_cast<const float4*>(&ex.total[val][(threadIdx.x & 7) * 4]));
+}
+// Sums s (already over the thread's rows) to ex.part, and their joining.
+template <int kVals>
+__device__ __forceinline__ void sum_part(F4 s, Exchange<kVals>& ex, int val) {
+  s = over_rows(s);
+  if ((threadIdx.x & 31) < 8)
+    *reinterpret_cast<float4*>(&ex.part[threadIdx.x >> 5][val][(threadIdx.x & 7) * 4]) = flat(s);
+}
+template <int kVals>
+__device__ __forceinline__ void sum_join(Exchange<kVals>& ex, int val, int warps) {
+  const int lane = threadIdx.x & 31;
+  float s = 0.f;
+  for (int w = 0; w < warps; ++w) s += ex.part[w][val][lane];
+  ex.total[val][lane] = s;
 }
 
-template <bool kTaped, class T>
-__device__ __forceinline__ float load_kept(const T* v, const zjai_tape& t, long long row,
-                                           int groups, int g, int p, bool in) {
-  const long long at = row * p + g * kTapeGroup + (threadIdx.x & 31);
-  if (!in) return 0.f;
-  if (kTaped) return (float)t.codes[at] * tape_scale(t.exps[row * groups + g]);
-  return to_f32(v[at]);
+// threads a block may have, and blocks an SM holds of the largest
+constexpr int kThreadsMost = 32 * kMaxWarps;
+template <int kRows>
+constexpr int blocks_least() {
+  return kRows == 4 ? 1 : 2;
 }
 
-// Any channel count: a tile's channels are read again for each of the step's sums.
-template <class T>
-__global__ void __launch_bounds__(kWarps * 32) residual_norm_kernel(FwdArgs<T> a) {
-  __shared__ float red[kWarps][32];
-  const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
+// value of positions behind the row's end set to zero
+template <bool kVec>
+__device__ __forceinline__ F4 clip4(F4 v, int at, int p) {
+  if (kVec) return at < p ? v : all(0.f);
+  return {make_float2(at < p ? v.a.x : 0.f, at + 1 < p ? v.a.y : 0.f),
+          make_float2(at + 2 < p ? v.b.x : 0.f, at + 3 < p ? v.b.y : 0.f)};
+}
+__device__ __forceinline__ float sum4(F4 v) {
+  const float2 t = __fadd2_rn(v.a, v.b);
+  return t.x + t.y;
+}
+
+template <int kRows, bool kVec, class T>
+__global__ void __launch_bounds__(kThreadsMost, blocks_least<kRows>())
+    residual_norm_kernel(const FwdArgs<T> a) {
+  __shared__ Exchange<2> ex;
+  const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Rows<kRows> rows(a.c, warps);
+  constexpr int kHeld = kRows ? kRows : 1;
   const int groups = (int)tape_groups(a.p);
-  const float inv_c = 1.f / (float)a.c;
+  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const long long img = tile / groups;
-    const int g = (int)(tile - img * groups), at = g * kTapeGroup + lane;
-    const bool in = at < a.p;
-    const long long base = img * a.c;
-    const T* gate = a.gate ? a.gate + img * a.gate_c * a.p + at : nullptr;
-    auto value = [&](const T* v, int ch) { return in ? to_f32(v[(base + ch) * a.p + at]) : 0.f; };
-    // mean, its correction and 1 / sigma of v(ch) over the channels
-    auto stats = [&](auto v) {
-      float s = 0.f, t = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) s += v(ch);
-      Stats st;
-      st.m = over_warps(s, red) * inv_c;
-      s = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) {
-        const float d = v(ch) - st.m;
-        s += d * d;
-        t += d;
-      }
-      st.finish(over_warps(t, red) * inv_c, over_warps(s, red) * inv_c);
-      return st;
+    const long long img = tile / groups, base = img * a.c;
+    const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * kVecs;
+    F4 f[kHeld], x[kHeld], q[kHeld];  // branch, input (then y), gate logits
+    auto load = [&](const T* v, int j) {
+      return rows.on(j) ? load4<kVec>(v + (base + rows.row(j)) * a.p, at, a.p) : all(0.f);
     };
-    Stats s1, s2;
-    if (a.prm.post_weight) s1 = stats([&](int ch) { return value(a.f, ch); });
-    float sg1 = 1.f, unused;
-    if (a.gate && a.gate_c == 1) sigmoid2(in ? to_f32(gate[0]) : 0.f, &sg1, &unused);
-    auto y_of = [&](int ch) {
-      float u = value(a.f, ch), q = sg1;
-      if (a.prm.post_weight)
-        u = s1.norm(u) * __ldg(a.prm.post_weight + ch) + __ldg(a.prm.post_bias + ch);
-      if (a.gate && a.gate_c != 1)
-        sigmoid2(in ? to_f32(gate[(long long)ch * a.p]) : 0.f, &q, &unused);
-      if (a.prm.scale) q *= __ldg(a.prm.scale + ch);
-      return value(a.x, ch) + q * u;
+    if (kRows) {
+      FOR_ROWS(j) f[j % kHeld] = load(a.f, j);
+      FOR_ROWS(j) x[j % kHeld] = load(a.x, j);
+      if (per_row) FOR_ROWS(j) q[j % kHeld] = load(a.gate, j);
+    }
+    auto f_of = [&](int j) { return kRows ? f[j % kHeld] : load(a.f, j); };
+    auto gate_of = [&](int j) { return kRows ? q[j % kHeld] : load(a.gate, j); };
+    F4 gate1 = all(0.f), sg1 = all(1.f), unused;
+    if (a.gate_c == 1) {
+      gate1 = load4<kVec>(a.gate + img * a.p, at, a.p);
+      sigmoid4(gate1, &sg1, &unused);
+    }
+    F4 m = all(0.f), r = all(1.f);
+    auto exchange = [&](auto v) {
+      stats_part(rows, v, ex, 0);
+      __syncthreads();
+      if (wp == 0) stats_join<kRows>(ex, 0, a.c, warps);
+      __syncthreads();
+      m = total4(ex, 0);
+      r = total4(ex, 1);
     };
-    if (a.prm.pre_weight) s2 = stats(y_of);
-    for (int ch = wp; ch < a.c; ch += kWarps) {
-      const long long row = base + ch;
-      const float y = y_of(ch);
-      if (in) a.y[row * a.p + at] = from_f32<T>(y);
-      if (a.tp.f.codes) tape_group_store(a.tp.f, row, groups, g, a.p, value(a.f, ch), in);
-      if (a.tp.gate.codes && (a.gate_c != 1 || ch == 0))
-        tape_group_store(a.tp.gate, img * a.gate_c + (a.gate_c == 1 ? 0 : ch), groups, g, a.p,
-                         in ? to_f32(gate[a.gate_c == 1 ? 0 : (long long)ch * a.p]) : 0.f, in);
-      if (a.tp.y.codes) tape_group_store(a.tp.y, row, groups, g, a.p, in ? y : 0.f, in);
-      if (a.prm.pre_weight) {
-        const float z = s2.norm(y) * __ldg(a.prm.pre_weight + ch) + __ldg(a.prm.pre_bias + ch);
-        if (in) a.z[row * a.p + at] = from_f32<T>(z);
-        if (a.tp.z.codes) tape_group_store(a.tp.z, row, groups, g, a.p, in ? z : 0.f, in);
+    if (post) exchange(f_of);
+    const F4 m1 = m, r1 = r;
+    auto y_of = [&](int j) {
+      const int ch = rows.param(j);
+      F4 u = f_of(j), s = sg1;
+      if (post)
+        u = fma4((u - m1) * r1, all(__ldg(a.prm.post_weight + ch)), all(__ldg(a.prm.post_bias + ch)));
+      if (per_row) sigmoid4(gate_of(j), &s, &unused);
+      if (a.prm.scale) s = s * all(__ldg(a.prm.scale + ch));
+      return fma4(s, u, kRows ? x[j % kHeld] : load(a.x, j));
+    };
+    // y and the tapes of f, gate and y (whole warps call)
+    auto emit = [&](int j, F4 y) {
+      const bool on = rows.on(j);
+      const long long row = base + rows.row(j);
+      if (on) store4<kVec>(a.y + row * a.p, at, a.p, y);
+      if (a.tp.f.codes) tape_store4<kVec>(a.tp.f, row, groups, g, at, a.p, f_of(j), on);
+      if (per_row && a.tp.gate.codes)
+        tape_store4<kVec>(a.tp.gate, row, groups, g, at, a.p, gate_of(j), on);
+      if (a.tp.y.codes)
+        tape_store4<kVec>(a.tp.y, row, groups, g, at, a.p, clip4<kVec>(y, at, a.p), on);
+    };
+    if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
+      tape_store4<kVec>(a.tp.gate, img, groups, g, at, a.p, gate1, lane < 8);
+    if (kRows) {
+      FOR_ROWS(j) {
+        const F4 y = y_of(j);
+        emit(j, y);
+        x[j % kHeld] = y;
       }
+    }
+    auto done_y = [&](int j) { return kRows ? x[j % kHeld] : y_of(j); };
+    if (pre) exchange(done_y);
+    if (kRows && !pre) continue;
+    FOR_ROWS(j) {
+      const F4 y = done_y(j);
+      if (!kRows) emit(j, y);
+      if (!pre) continue;
+      const int ch = rows.param(j);
+      const F4 z = fma4((y - m) * r, all(__ldg(a.prm.pre_weight + ch)), all(__ldg(a.prm.pre_bias + ch)));
+      const long long row = base + rows.row(j);
+      if (rows.on(j)) store4<kVec>(a.z + row * a.p, at, a.p, z);
+      if (a.tp.z.codes)
+        tape_store4<kVec>(a.tp.z, row, groups, g, at, a.p, clip4<kVec>(z, at, a.p), rows.on(j));
     }
   }
 }
 
-// Backward, any channel count: as the forward kernel, and a block's parameter sums in shared
-// memory, a channel's by the warp that owns it, written out per block when the block ends.
-template <bool kTaped, class T>
-__global__ void __launch_bounds__(kWarps * 32) residual_norm_bwd_kernel(BwdArgs<T> a) {
-  __shared__ float red[kWarps][32];
-  extern __shared__ float acc[];  // [5][c]
-  const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
+// A row's four positions of a kept map: codes and exponent of a tape, or values.
+template <bool kTaped, bool kVec, class T>
+struct Kept {
+  F4 v;
+  __device__ __forceinline__ void load(const T* map, const zjai_tape&, long long row, int, int,
+                                       int at, int p) {
+    v = load4<kVec>(map + row * p, at, p);
+  }
+  __device__ __forceinline__ F4 get() const { return v; }
+};
+template <bool kVec, class T>
+struct Kept<true, kVec, T> {
+  uint32_t w;
+  int e;
+  __device__ __forceinline__ void load(const T*, const zjai_tape& t, long long row, int groups,
+                                       int g, int at, int p) {
+    w = load_codes<kVec>(t.codes + row * p, at, p);
+    e = __ldg(t.exps + row * groups + g);
+  }
+  __device__ __forceinline__ F4 get() const { return taped4(w, e); }
+};
+
+// The parameter gradients are summed over a block's tiles (in registers, or per channel in shared
+// memory where rows are not held) and written out per block.
+template <int kRows, bool kTaped, bool kVec, class T>
+__global__ void __launch_bounds__(kThreadsMost, 1)
+    residual_norm_bwd_kernel(const BwdArgs<T> a) {
+  __shared__ Exchange<4> ex;
+  extern __shared__ float acc_c[];  // [5][c] where rows are not held
+  const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Rows<kRows> rows(a.c, warps);
+  constexpr int kHeld = kRows ? kRows : 1;
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
-  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, gated = a.gate_c != 0;
-  const bool need_f = post || gated || a.prm.scale;
-  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc[i] = 0.f;
-  __syncthreads();
+  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
+  const bool need_f = post || a.gate_c || a.prm.scale;
+  const int second = warps > 1 ? 1 : 0;  // warp that joins the second of two sums
+  float acc[kHeld][5];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
+  if (!kRows) {
+    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
+    __syncthreads();
+  }
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const long long img = tile / groups;
-    const int g = (int)(tile - img * groups), at = g * kTapeGroup + lane;
-    const bool in = at < a.p;
-    const long long base = img * a.c;
-    auto grad = [&](const T* v, int ch) { return in ? to_f32(v[(base + ch) * a.p + at]) : 0.f; };
-    auto f_of = [&](int ch) {
-      return load_kept<kTaped>(a.f, a.tp.f, base + ch, groups, g, a.p, in);
+    const long long img = tile / groups, base = img * a.c;
+    const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * kVecs;
+    using K = Kept<kTaped, kVec, T>;
+    F4 dy[kHeld], dz[kHeld];
+    K f[kHeld], y[kHeld], q[kHeld];
+    auto grad = [&](const T* v, int j) {
+      return rows.on(j) ? load4<kVec>(v + (base + rows.row(j)) * a.p, at, a.p) : all(0.f);
     };
-    auto y_of = [&](int ch) {
-      return load_kept<kTaped>(a.y, a.tp.y, base + ch, groups, g, a.p, in);
+    auto kept = [&](const T* v, const zjai_tape& t, int j) {
+      K k;
+      k.load(v, t, base + rows.param(j), groups, g, at, a.p);
+      return k;
     };
-    auto gate_of = [&](int ch) {
-      return load_kept<kTaped>(a.gate, a.tp.gate, img * a.gate_c + ch, groups, g, a.p, in);
-    };
-    auto stats = [&](auto v) {
-      float s = 0.f, t = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) s += v(ch);
-      Stats st;
-      st.m = over_warps(s, red) * inv_c;
-      s = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) {
-        const float d = v(ch) - st.m;
-        s += d * d;
-        t += d;
-      }
-      st.finish(over_warps(t, red) * inv_c, over_warps(s, red) * inv_c);
-      return st;
-    };
-    Stats s1, s2;
-    float am = 0.f, ay = 0.f;
-    if (post) s1 = stats(f_of);
-    if (pre) {
-      s2 = stats(y_of);
-      float t0 = 0.f, t1 = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) {
-        const float t = __fmul_rn(grad(a.dz, ch), __ldg(a.prm.pre_weight + ch));
-        t0 += t;
-        t1 += t * s2.norm(y_of(ch));
-      }
-      am = over_warps(t0, red) * inv_c;
-      ay = over_warps(t1, red) * inv_c;
+    if (kRows) {
+      if (pre) FOR_ROWS(j) y[j % kHeld] = kept(a.y, a.tp.y, j);
+      if (need_f) FOR_ROWS(j) f[j % kHeld] = kept(a.f, a.tp.f, j);
+      if (pre) FOR_ROWS(j) dz[j % kHeld] = grad(a.dz, j);
+      FOR_ROWS(j) dy[j % kHeld] = grad(a.dy, j);
+      if (per_row) FOR_ROWS(j) q[j % kHeld] = kept(a.gate, a.tp.gate, j);
     }
-    float sg1 = 1.f, os1 = 0.f;
-    if (a.gate_c == 1) sigmoid2(gate_of(0), &sg1, &os1);
-    // D, fn, u, sigma(g), 1 - sigma(g), s of one channel
-    struct Chan {
-      float d, fn, u, sg, os, sc, yn, dz;
+    auto f_of = [&](int j) { return kRows ? f[j % kHeld].get() : kept(a.f, a.tp.f, j).get(); };
+    auto y_of = [&](int j) { return kRows ? y[j % kHeld].get() : kept(a.y, a.tp.y, j).get(); };
+    auto gate_of = [&](int j) {
+      return kRows ? q[j % kHeld].get() : kept(a.gate, a.tp.gate, j).get();
     };
-    auto chan = [&](int ch) {
-      Chan k;
-      k.d = grad(a.dy, ch);
-      k.yn = k.dz = 0.f;
-      if (pre) {
-        k.dz = grad(a.dz, ch);
-        k.yn = s2.norm(y_of(ch));
-        k.d += (__fmul_rn(k.dz, __ldg(a.prm.pre_weight + ch)) - am - k.yn * ay) * s2.r;
+    auto dz_of = [&](int j) { return kRows ? dz[j % kHeld] : grad(a.dz, j); };
+    F4 sg1 = all(1.f), os1 = all(0.f);
+    if (a.gate_c == 1) {
+      K k;
+      k.load(a.gate, a.tp.gate, img, groups, g, at, a.p);
+      sigmoid4(k.get(), &sg1, &os1);
+    }
+    F4 m1 = all(0.f), r1 = all(1.f), m2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
+    if (post) stats_part(rows, f_of, ex, 0);
+    if (pre) stats_part(rows, y_of, ex, 2);
+    if (post || pre) {
+      __syncthreads();
+      if (post && wp == 0) stats_join<kRows>(ex, 0, a.c, warps);
+      if (pre && wp == second) stats_join<kRows>(ex, 2, a.c, warps);
+      __syncthreads();
+      if (post) m1 = total4(ex, 0), r1 = total4(ex, 1);
+      if (pre) m2 = total4(ex, 2), r2 = total4(ex, 3);
+    }
+    if (pre) {
+      F4 s0 = all(0.f), s1 = all(0.f);
+      FOR_ROWS(j) if (rows.on(j)) {
+        const F4 t = dz_of(j) * all(__ldg(a.prm.pre_weight + rows.param(j)));
+        s0 = s0 + t;
+        s1 = fma4(t, (y_of(j) - m2) * r2, s1);
       }
-      k.fn = k.u = 0.f;
+      sum_part(s0, ex, 0);
+      sum_part(s1, ex, 1);
+      __syncthreads();
+      if (wp == 0) sum_join(ex, 0, warps);
+      if (wp == second) sum_join(ex, 1, warps);
+      __syncthreads();
+      am = total4(ex, 0) * all(inv_c);
+      ay = total4(ex, 1) * all(inv_c);
+    }
+    // everything of a row but d_f's projection
+    struct Row {
+      F4 d, du, fn, u, sg, os, sc, yn, dz;
+    };
+    auto row_of = [&](int j) {
+      const int ch = rows.param(j);
+      Row k;
+      k.d = kRows ? dy[j % kHeld] : grad(a.dy, j);
+      k.yn = k.dz = all(0.f);
+      if (pre) {
+        k.dz = dz_of(j);
+        k.yn = (y_of(j) - m2) * r2;
+        const F4 t = k.dz * all(__ldg(a.prm.pre_weight + ch));
+        k.d = fma4(fma4(-k.yn, ay, t - am), r2, k.d);
+      }
+      k.fn = k.u = all(0.f);
       if (need_f) {
-        const float f = f_of(ch);
-        k.fn = s1.norm(f);
-        k.u = post ? k.fn * __ldg(a.prm.post_weight + ch) + __ldg(a.prm.post_bias + ch) : f;
+        k.u = f_of(j);
+        k.fn = (k.u - m1) * r1;
+        if (post)
+          k.u = fma4(k.fn, all(__ldg(a.prm.post_weight + ch)), all(__ldg(a.prm.post_bias + ch)));
       }
       k.sg = sg1;
       k.os = os1;
-      if (gated && a.gate_c != 1) sigmoid2(gate_of(ch), &k.sg, &k.os);
-      k.sc = a.prm.scale ? __ldg(a.prm.scale + ch) : 1.f;
+      if (per_row) sigmoid4(gate_of(j), &k.sg, &k.os);
+      k.sc = all(a.prm.scale ? __ldg(a.prm.scale + ch) : 1.f);
+      k.du = k.d * k.sc * k.sg;
       return k;
     };
-    float bm = 0.f, bf = 0.f;
-    if (post || a.gate_c == 1) {
-      float t0 = 0.f, t1 = 0.f, t2 = 0.f;
-      for (int ch = wp; ch < a.c; ch += kWarps) {
-        const Chan k = chan(ch);
-        if (post) {
-          const float t = __fmul_rn(k.d * k.sc * k.sg, __ldg(a.prm.post_weight + ch));
-          t0 += t;
-          t1 += t * k.fn;
-        }
-        t2 += k.d * k.sc * k.u;
+    F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
+    FOR_ROWS(j) {
+      const Row k = row_of(j);
+      const int ch = rows.param(j);
+      const long long e = (base + ch) * a.p;
+      F4 b = k.du;
+      if (post) b = b * all(__ldg(a.prm.post_weight + ch));
+      if (rows.on(j)) {
+        store4<kVec>(a.dx + e, at, a.p, k.d);
+        if (!post && a.df) store4<kVec>(a.df + e, at, a.p, k.du);
+        if (per_row) store4<kVec>(a.dgate + e, at, a.p, k.du * k.u * k.os);
+        t0 = t0 + b;
+        t1 = fma4(b, k.fn, t1);
+        t2 = fma4(k.d * k.sc, k.u, t2);
       }
-      bm = over_warps(t0, red) * inv_c;
-      bf = over_warps(t1, red) * inv_c;
-      if (a.gate_c == 1) {
-        t2 = over_warps(t2, red);
-        if (wp == 0 && in) a.dgate[img * a.p + at] = from_f32<T>(t2 * sg1 * os1);
-      }
-    }
-    for (int ch = wp; ch < a.c; ch += kWarps) {
-      const Chan k = chan(ch);
-      const long long e = (base + ch) * a.p + at;
-      const float du = k.d * k.sc * k.sg;
-      if (in) {
-        a.dx[e] = from_f32<T>(k.d);
-        if (a.df)
-          a.df[e] = from_f32<T>(
-              post ? (__fmul_rn(du, __ldg(a.prm.post_weight + ch)) - bm - k.fn * bf) * s1.r : du);
-        if (a.gate_c > 1)
-          a.dgate[e] = from_f32<T>(k.d * k.sc * k.u * k.sg * k.os);
-      }
-      float v[5] = {k.d * k.sg * k.u, du * k.fn, du, k.dz * k.yn, k.dz};
+      const float v[5] = {sum4(k.d * k.sg * k.u), sum4(k.du * k.fn), sum4(k.du), sum4(k.dz * k.yn),
+                          sum4(k.dz)};
 #pragma unroll
       for (int i = 0; i < 5; ++i) {
-        const float s = warp_sum(in ? v[i] : 0.f);
-        if (lane == 0) acc[i * a.c + ch] += s;
+        if (kRows) {
+          acc[j % kHeld][i] += v[i];
+        } else {
+          float s = v[i];
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if ((lane & 7) == 0 && rows.on(j)) acc_c[i * a.c + ch] += s;
+        }
+      }
+      if (kRows) {
+        dy[j % kHeld] = b;  // from here on b
+      }
+    }
+    if (post || a.gate_c == 1) {
+      if (post) sum_part(t0, ex, 0), sum_part(t1, ex, 1);
+      if (a.gate_c == 1) sum_part(t2, ex, 2);
+      __syncthreads();
+      if (post && wp == 0) sum_join(ex, 0, warps);
+      if (post && wp == second) sum_join(ex, 1, warps);
+      if (a.gate_c == 1 && wp == warps - 1) sum_join(ex, 2, warps);
+      __syncthreads();
+      if (a.gate_c == 1 && threadIdx.x < 8)
+        store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * sg1 * os1);
+      if (post) {
+        const F4 bm = total4(ex, 0) * all(inv_c), bf = total4(ex, 1) * all(inv_c);
+        FOR_ROWS(j) if (rows.on(j)) {
+          const int ch = rows.param(j);
+          F4 b = dy[j % kHeld], fn;
+          if (kRows) {
+            fn = (f_of(j) - m1) * r1;
+          } else {
+            const Row k = row_of(j);
+            fn = k.fn;
+            b = k.du * all(__ldg(a.prm.post_weight + ch));
+          }
+          store4<kVec>(a.df + (base + ch) * a.p, at, a.p, fma4(-fn, bf, b - bm) * r1);
+        }
       }
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x)
-    a.sums[(long long)blockIdx.x * 5 * a.c + i] = acc[i];
+  float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
+  if (kRows) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        float s = acc[j][i];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if ((lane & 7) == 0 && rows.on(j)) out[i * a.c + rows.row(j)] = s;
+      }
+  } else {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) out[i] = acc_c[i];
+  }
 }
 
 struct SumOut {
@@ -324,6 +652,36 @@ int stage_params(Ctx* ctx, const zjai_residual_params& in, int c, int mem,
   ZJAI_TRY(stage_param(ctx, in.pre_weight, c, mem, "pre_weight", &out->pre_weight));
   return stage_param(ctx, in.pre_bias, c, mem, "pre_bias", &out->pre_bias);
 }
+
+// Rows a thread holds for c channels (0: not held) and the block's warps.
+struct Shape {
+  int rows, warps, per_sm;
+};
+Shape shape_of(int c) {
+  const int rows = c <= 64 ? 1 : c <= 128 ? 2 : c <= 256 ? 4 : 0;
+  const int warps = rows ? (c + 4 * rows - 1) / (4 * rows) : kMaxWarps;
+  // blocks that are resident at the register limits of __launch_bounds__
+  const int least = rows == 4 ? 1 : 2;
+  return {rows, warps, std::max(1, std::min(16, least * kMaxWarps / warps))};
+}
+// f(std::integral_constant) with the rows held
+template <class F>
+int by_rows(int rows, F&& f) {
+  if (rows == 1) return f(std::integral_constant<int, 1>());
+  if (rows == 2) return f(std::integral_constant<int, 2>());
+  if (rows == 4) return f(std::integral_constant<int, 4>());
+  return f(std::integral_constant<int, 0>());
+}
+// Four neighbouring positions can be loaded and stored at once: rows of a multiple of four
+// positions, maps aligned to four elements and codes to four bytes.
+struct VecCheck {
+  bool ok;
+  explicit VecCheck(int p) : ok(p % 4 == 0) {}
+  VecCheck& map(const void* q, size_t es) {
+    ok = ok && reinterpret_cast<uintptr_t>(q) % (4 * es) == 0;
+    return *this;
+  }
+};
 
 int check_step(const char* what, int c, int gate_channels, const zjai_residual_params* prm) {
   if (c > kMaxC)
@@ -385,13 +743,21 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->codes, tr[i] * p, 1, mem, "codes", &tt[i]->codes));
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->exps, tr[i] * groups, 1, mem, "exps", &tt[i]->exps));
     }
+    const Shape sh = shape_of(c);
+    VecCheck vec(p);
+    vec.map(dx, es).map(df, es).map(dg, es).map(dyo, es).map(dzo, es);
+    for (zjai_tape* t : tt) vec.map(t->codes, 1);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
-                      (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
-      const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * 8);
-      residual_norm_kernel<T><<<blocks, kWarps * 32, 0, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), "gated_residual_norm");
+      return by_rows(sh.rows, [&](auto r) -> int {
+        constexpr int kRows = decltype(r)::value;
+        FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
+                        (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
+        const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
+        auto k = vec.ok ? residual_norm_kernel<kRows, true, T> : residual_norm_kernel<kRows, false, T>;
+        k<<<blocks, sh.warps * 32, 0, ctx->stream>>>(a);
+        return cuda_check(cudaGetLastError(), "gated_residual_norm");
+      });
     }));
     ctx->launches++;
     ZJAI_TRY(finish_bytes_out(ctx, y, dyo, bytes, mem));
@@ -473,21 +839,33 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     for (int i = 0; i < 5; ++i)
       ZJAI_TRY(stage_bytes_out(ctx, host[i], (size_t)c * 4, 4, mem, "parameter gradient", &so.p[i]));
     const long long tiles = (long long)n * (long long)groups;
-    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * 4);
+    const Shape sh = shape_of(c);
+    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
     float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
     if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
+    VecCheck vec(p);
+    vec.map(ddy, es).map(ddz, es).map(df, es).map(dg, es).map(dyy, es);
+    vec.map(gx, es).map(gf, es).map(gg, es);
+    vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
-                      gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
-      const size_t smem = (size_t)5 * c * sizeof(float);
-      auto k = taped ? residual_norm_bwd_kernel<true, T> : residual_norm_bwd_kernel<false, T>;
-      ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               5 * kMaxC * (int)sizeof(float)),
-                          "gated_residual_norm_backward"));
-      k<<<blocks, kWarps * 32, smem, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
+      return by_rows(sh.rows, [&](auto r) -> int {
+        constexpr int kRows = decltype(r)::value;
+        BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
+                        gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
+        auto k = taped ? (vec.ok ? residual_norm_bwd_kernel<kRows, true, true, T>
+                                 : residual_norm_bwd_kernel<kRows, true, false, T>)
+                       : (vec.ok ? residual_norm_bwd_kernel<kRows, false, true, T>
+                                 : residual_norm_bwd_kernel<kRows, false, false, T>);
+        const size_t smem = kRows ? 0 : (size_t)5 * c * sizeof(float);
+        if (!kRows)
+          ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   5 * kMaxC * (int)sizeof(float)),
+                              "gated_residual_norm_backward"));
+        k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
+        return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
+      });
     }));
     residual_sums_kernel<<<dim3((c + 31) / 32, 5), 256, 0, ctx->stream>>>(sums, blocks, c, so);
     ctx->launches += 2;
