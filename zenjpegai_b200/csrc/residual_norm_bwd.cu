@@ -1,0 +1,367 @@
+// Backward pass of the residual step with its norms, gate and scale
+// (zjai_gated_residual_norm_backward): the mathematics and the layout are in residual_norm.cuh.
+#include "residual_norm.cuh"
+
+namespace zjai {
+namespace {
+
+template <class T>
+struct BwdArgs {
+  const T *dy, *dz, *f, *gate, *y;
+  zjai_residual_tapes tp;  // taped f, gate, y
+  int gate_c, c, p;
+  long long tiles;
+  zjai_residual_params prm;
+  T *dx, *df, *dgate;
+  float* sums;  // [blocks][5][c]: scale, post_weight, post_bias, pre_weight, pre_bias
+};
+
+// A row's four positions of a kept map: codes and exponent of a tape, or values.
+template <bool kTaped, bool kVec, class T>
+struct Kept {
+  F4 v;
+  __device__ __forceinline__ void load(const T* map, const zjai_tape&, long long row, int, int,
+                                       int at, int p) {
+    v = load4<kVec>(map + row * p, at, p);
+  }
+  __device__ __forceinline__ F4 get() const { return v; }
+};
+template <bool kVec, class T>
+struct Kept<true, kVec, T> {
+  uint32_t w;
+  int e;
+  __device__ __forceinline__ void load(const T*, const zjai_tape& t, long long row, int groups,
+                                       int g, int at, int p) {
+    w = load_codes<kVec>(t.codes + row * p, at, p);
+    e = __ldg(t.exps + row * groups + g);
+  }
+  __device__ __forceinline__ F4 get() const { return taped4(w, e); }
+};
+
+// The parameter gradients are summed over a block's tiles (in registers, or per channel in shared
+// memory where rows are not held) and written out per block.
+template <int kRows, bool kTaped, bool kVec, class T>
+__global__ void __launch_bounds__(kThreadsMost, 1)
+    residual_norm_bwd_kernel(const BwdArgs<T> a) {
+  __shared__ Exchange<4> ex;
+  extern __shared__ float acc_c[];  // [5][c] where rows are not held
+  const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Rows<kRows> rows(a.c, warps);
+  constexpr int kHeld = kRows ? kRows : 1;
+  const int groups = (int)tape_groups(a.p);
+  const float inv_c = 1.f / (float)a.c;
+  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
+  const bool need_f = post || a.gate_c || a.prm.scale;
+  const int second = warps > 1 ? 1 : 0;  // warp that joins the second of two sums
+  float acc[kHeld][5];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
+  if (!kRows) {
+    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
+    __syncthreads();
+  }
+  for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const long long img = tile / groups, base = img * a.c;
+    const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
+    using K = Kept<kTaped, kVec, T>;
+    F4 dy[kHeld], dz[kHeld];
+    K f[kHeld], y[kHeld], q[kHeld];
+    auto grad = [&](const T* v, int j) {
+      return rows.on(j) ? load4<kVec>(v + (base + rows.row(j)) * a.p, at, a.p) : all(0.f);
+    };
+    auto kept = [&](const T* v, const zjai_tape& t, int j) {
+      K k;
+      k.load(v, t, base + rows.param(j), groups, g, at, a.p);
+      return k;
+    };
+    if (kRows) {
+      if (pre) FOR_ROWS(j) y[j % kHeld] = kept(a.y, a.tp.y, j);
+      if (need_f) FOR_ROWS(j) f[j % kHeld] = kept(a.f, a.tp.f, j);
+      if (pre) FOR_ROWS(j) dz[j % kHeld] = grad(a.dz, j);
+      FOR_ROWS(j) dy[j % kHeld] = grad(a.dy, j);
+      if (per_row) FOR_ROWS(j) q[j % kHeld] = kept(a.gate, a.tp.gate, j);
+    }
+    auto f_of = [&](int j) { return kRows ? f[j % kHeld].get() : kept(a.f, a.tp.f, j).get(); };
+    auto y_of = [&](int j) { return kRows ? y[j % kHeld].get() : kept(a.y, a.tp.y, j).get(); };
+    auto gate_of = [&](int j) {
+      return kRows ? q[j % kHeld].get() : kept(a.gate, a.tp.gate, j).get();
+    };
+    auto dz_of = [&](int j) { return kRows ? dz[j % kHeld] : grad(a.dz, j); };
+    F4 sg1 = all(1.f), os1 = all(0.f);
+    if (a.gate_c == 1) {
+      K k;
+      k.load(a.gate, a.tp.gate, img, groups, g, at, a.p);
+      sigmoid4(k.get(), &sg1, &os1);
+    }
+    F4 m1 = all(0.f), r1 = all(1.f), m2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
+    if (post) stats_part(rows, f_of, ex, 0);
+    if (pre) stats_part(rows, y_of, ex, 2);
+    if (post || pre) {
+      __syncthreads();
+      if (post && wp == 0) stats_join<kRows>(ex, 0, a.c, warps);
+      if (pre && wp == second) stats_join<kRows>(ex, 2, a.c, warps);
+      __syncthreads();
+      if (post) m1 = total4(ex, 0), r1 = total4(ex, 1);
+      if (pre) m2 = total4(ex, 2), r2 = total4(ex, 3);
+    }
+    if (pre) {
+      F4 s0 = all(0.f), s1 = all(0.f);
+      FOR_ROWS(j) if (rows.on(j)) {
+        const F4 t = dz_of(j) * all(__ldg(a.prm.pre_weight + rows.param(j)));
+        s0 = s0 + t;
+        s1 = fma4(t, (y_of(j) - m2) * r2, s1);
+      }
+      sum_part(s0, ex, 0);
+      sum_part(s1, ex, 1);
+      __syncthreads();
+      if (wp == 0) sum_join(ex, 0, warps);
+      if (wp == second) sum_join(ex, 1, warps);
+      __syncthreads();
+      am = total4(ex, 0) * all(inv_c);
+      ay = total4(ex, 1) * all(inv_c);
+    }
+    // everything of a row but d_f's projection
+    struct Row {
+      F4 d, du, fn, u, sg, os, sc, yn, dz;
+    };
+    auto row_of = [&](int j) {
+      const int ch = rows.param(j);
+      Row k;
+      k.d = kRows ? dy[j % kHeld] : grad(a.dy, j);
+      k.yn = k.dz = all(0.f);
+      if (pre) {
+        k.dz = dz_of(j);
+        k.yn = (y_of(j) - m2) * r2;
+        const F4 t = k.dz * all(__ldg(a.prm.pre_weight + ch));
+        k.d = fma4(fma4(-k.yn, ay, t - am), r2, k.d);
+      }
+      k.fn = k.u = all(0.f);
+      if (need_f) {
+        k.u = f_of(j);
+        k.fn = (k.u - m1) * r1;
+        if (post)
+          k.u = fma4(k.fn, all(__ldg(a.prm.post_weight + ch)), all(__ldg(a.prm.post_bias + ch)));
+      }
+      k.sg = sg1;
+      k.os = os1;
+      if (per_row) sigmoid4(gate_of(j), &k.sg, &k.os);
+      k.sc = all(a.prm.scale ? __ldg(a.prm.scale + ch) : 1.f);
+      k.du = k.d * k.sc * k.sg;
+      return k;
+    };
+    F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
+    FOR_ROWS(j) {
+      const Row k = row_of(j);
+      const int ch = rows.param(j);
+      const long long e = (base + ch) * a.p;
+      F4 b = k.du;
+      if (post) b = b * all(__ldg(a.prm.post_weight + ch));
+      if (rows.on(j)) {
+        store4<kVec>(a.dx + e, at, a.p, k.d);
+        if (!post && a.df) store4<kVec>(a.df + e, at, a.p, k.du);
+        if (per_row) store4<kVec>(a.dgate + e, at, a.p, k.du * k.u * k.os);
+        t0 = t0 + b;
+        t1 = fma4(b, k.fn, t1);
+        t2 = fma4(k.d * k.sc, k.u, t2);
+      }
+      const float v[5] = {sum4(k.d * k.sg * k.u), sum4(k.du * k.fn), sum4(k.du), sum4(k.dz * k.yn),
+                          sum4(k.dz)};
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        if (kRows) {
+          acc[j % kHeld][i] += v[i];
+        } else {
+          float s = v[i];
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if ((lane & 7) == 0 && rows.on(j)) acc_c[i * a.c + ch] += s;
+        }
+      }
+      if (kRows) {
+        dy[j % kHeld] = b;  // from here on b
+      }
+    }
+    if (post || a.gate_c == 1) {
+      if (post) sum_part(t0, ex, 0), sum_part(t1, ex, 1);
+      if (a.gate_c == 1) sum_part(t2, ex, 2);
+      __syncthreads();
+      if (post && wp == 0) sum_join(ex, 0, warps);
+      if (post && wp == second) sum_join(ex, 1, warps);
+      if (a.gate_c == 1 && wp == warps - 1) sum_join(ex, 2, warps);
+      __syncthreads();
+      if (a.gate_c == 1 && threadIdx.x < 8)
+        store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * sg1 * os1);
+      if (post) {
+        const F4 bm = total4(ex, 0) * all(inv_c), bf = total4(ex, 1) * all(inv_c);
+        FOR_ROWS(j) if (rows.on(j)) {
+          const int ch = rows.param(j);
+          F4 b = dy[j % kHeld], fn;
+          if (kRows) {
+            fn = (f_of(j) - m1) * r1;
+          } else {
+            const Row k = row_of(j);
+            fn = k.fn;
+            b = k.du * all(__ldg(a.prm.post_weight + ch));
+          }
+          store4<kVec>(a.df + (base + ch) * a.p, at, a.p, fma4(-fn, bf, b - bm) * r1);
+        }
+      }
+    }
+  }
+  float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
+  if (kRows) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        float s = acc[j][i];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if ((lane & 7) == 0 && rows.on(j)) out[i * a.c + rows.row(j)] = s;
+      }
+  } else {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) out[i] = acc_c[i];
+  }
+}
+
+struct SumOut {
+  float* p[5];
+};
+
+// out[k][ch] = sum over the blocks of sums[block][k][ch], in a fixed order
+__global__ void __launch_bounds__(256) residual_sums_kernel(const float* __restrict__ sums,
+                                                            int blocks, int c, SumOut out) {
+  __shared__ float red[8][33];
+  const int k = blockIdx.y, ch = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  float s = 0.f;
+  if (ch < c)
+    for (int b = r; b < blocks; b += 8) s += sums[((long long)b * 5 + k) * c + ch];
+  red[r][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (r == 0 && ch < c && out.p[k]) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x & 31];
+    out.p[k][ch] = s;
+  }
+}
+
+}  // namespace
+}  // namespace zjai
+
+using namespace zjai;
+
+extern "C" {
+
+int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void* dz, const void* f,
+                                      const void* gate, int gate_channels, const void* y,
+                                      const zjai_residual_tapes* tapes, int dtype, int n, int c,
+                                      int h, int w, const zjai_residual_params* prm,
+                                      const zjai_residual_grads* grads, int mem) {
+  return guarded([&]() -> int {
+    const char* me = "gated_residual_norm_backward";
+    ZJAI_TRY(ctx_enter(ctx));
+    ZJAI_TRY(check_map(me, dtype, n, c, h, w));
+    ZJAI_TRY(check_mem(mem));
+    ZJAI_TRY(check_step(me, c, gate_channels, prm));
+    const bool post = prm->post_weight, pre = prm->pre_weight, taped = tapes != nullptr;
+    const bool need_f = post || prm->scale || gate_channels;
+    if (!dy || !grads || !grads->x || (pre && !dz) || (need_f && !grads->f) ||
+        (gate_channels && !grads->gate) || (post && (!grads->post_weight || !grads->post_bias)) ||
+        (prm->scale && !grads->scale) || (pre && (!grads->pre_weight || !grads->pre_bias)))
+      return fail(ZJAI_INVALID_ARGUMENT, std::string(me) + ": null buffer");
+    if (taped && (f || gate || y))
+      return fail(ZJAI_INVALID_ARGUMENT, std::string(me) + ": either tapes or maps");
+    auto have = [&](const void* map, const zjai_tape* t) {
+      return taped ? t->codes && t->exps : map != nullptr;
+    };
+    const zjai_residual_tapes none = {};
+    const zjai_residual_tapes& kept = taped ? *tapes : none;
+    if ((need_f && !have(f, &kept.f)) || (gate_channels && !have(gate, &kept.gate)) ||
+        (pre && !have(y, &kept.y)))
+      return fail(ZJAI_INVALID_ARGUMENT, std::string(me) + ": f, gate or y missing");
+    ArenaScope scope(ctx);
+    const int p = h * w;
+    const size_t es = dtype_size(dtype), rows = (size_t)n * c, groups = tape_groups(p);
+    const size_t bytes = rows * p * es, grows = (size_t)n * gate_channels;
+    const char *ddy, *ddz, *df = nullptr, *dg = nullptr, *dyy = nullptr;
+    zjai_residual_tapes dt = {};
+    zjai_residual_params dp = {};
+    ZJAI_TRY(stage_bytes_in(ctx, (const char*)dy, bytes, es, mem, "dy", &ddy));
+    ZJAI_TRY(stage_bytes_in(ctx, pre ? (const char*)dz : nullptr, bytes, es, mem, "dz", &ddz));
+    if (!taped) {
+      ZJAI_TRY(stage_bytes_in(ctx, need_f ? (const char*)f : nullptr, bytes, es, mem, "f", &df));
+      ZJAI_TRY(stage_bytes_in(ctx, gate_channels ? (const char*)gate : nullptr, grows * p * es, es,
+                              mem, "gate", &dg));
+      ZJAI_TRY(stage_bytes_in(ctx, pre ? (const char*)y : nullptr, bytes, es, mem, "y", &dyy));
+    } else {
+      const zjai_tape* in[3] = {need_f ? &kept.f : nullptr, gate_channels ? &kept.gate : nullptr,
+                                pre ? &kept.y : nullptr};
+      zjai_tape* out[3] = {&dt.f, &dt.gate, &dt.y};
+      const size_t tr[3] = {rows, grows, rows};
+      for (int i = 0; i < 3; ++i) {
+        if (!in[i]) continue;
+        const int8_t *cd, *ex;
+        ZJAI_TRY(stage_bytes_in(ctx, (const int8_t*)in[i]->codes, tr[i] * p, 1, mem, "codes", &cd));
+        ZJAI_TRY(
+            stage_bytes_in(ctx, (const int8_t*)in[i]->exps, tr[i] * groups, 1, mem, "exps", &ex));
+        *out[i] = {const_cast<int8_t*>(cd), const_cast<int8_t*>(ex)};
+      }
+    }
+    ZJAI_TRY(stage_params(ctx, *prm, c, mem, &dp));
+    char *gx, *gf, *gg;
+    ZJAI_TRY(stage_bytes_out(ctx, (char*)grads->x, bytes, es, mem, "d_x", &gx));
+    ZJAI_TRY(stage_bytes_out(ctx, (char*)grads->f, bytes, es, mem, "d_f", &gf));
+    ZJAI_TRY(stage_bytes_out(ctx, gate_channels ? (char*)grads->gate : nullptr, grows * p * es, es,
+                             mem, "d_gate", &gg));
+    float* host[5] = {prm->scale ? grads->scale : nullptr, post ? grads->post_weight : nullptr,
+                      post ? grads->post_bias : nullptr, pre ? grads->pre_weight : nullptr,
+                      pre ? grads->pre_bias : nullptr};
+    SumOut so;
+    for (int i = 0; i < 5; ++i)
+      ZJAI_TRY(stage_bytes_out(ctx, host[i], (size_t)c * 4, 4, mem, "parameter gradient", &so.p[i]));
+    const long long tiles = (long long)n * (long long)groups;
+    const Shape sh = shape_of(c);
+    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
+    float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
+    if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
+    VecCheck vec(p);
+    vec.map(ddy, es).map(ddz, es).map(df, es).map(dg, es).map(dyy, es);
+    vec.map(gx, es).map(gf, es).map(gg, es);
+    vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
+    ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      return by_rows(sh.rows, [&](auto r) -> int {
+        constexpr int kRows = decltype(r)::value;
+        BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
+                        gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
+        auto k = taped ? (vec.ok ? residual_norm_bwd_kernel<kRows, true, true, T>
+                                 : residual_norm_bwd_kernel<kRows, true, false, T>)
+                       : (vec.ok ? residual_norm_bwd_kernel<kRows, false, true, T>
+                                 : residual_norm_bwd_kernel<kRows, false, false, T>);
+        const size_t smem = kRows ? 0 : (size_t)5 * c * sizeof(float);
+        if (!kRows)
+          ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   5 * kMaxC * (int)sizeof(float)),
+                              "gated_residual_norm_backward"));
+        k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
+        return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
+      });
+    }));
+    residual_sums_kernel<<<dim3((c + 31) / 32, 5), 256, 0, ctx->stream>>>(sums, blocks, c, so);
+    ctx->launches += 2;
+    ZJAI_TRY(cuda_check(cudaGetLastError(), "parameter sums"));
+    ZJAI_TRY(finish_bytes_out(ctx, grads->x, gx, bytes, mem));
+    if (gf) ZJAI_TRY(finish_bytes_out(ctx, grads->f, gf, bytes, mem));
+    if (gg) ZJAI_TRY(finish_bytes_out(ctx, grads->gate, gg, grows * p * es, mem));
+    for (int i = 0; i < 5; ++i)
+      if (host[i]) ZJAI_TRY(finish_bytes_out(ctx, host[i], so.p[i], (size_t)c * 4, mem));
+    return finish_call(ctx, mem);
+  });
+}
+
+}  // extern "C"

@@ -64,12 +64,4 @@ __device__ __forceinline__ uint32_t tape_code_bits(float x, float inv) {
   const float magic = 12582912.f;
   return __float_as_uint(fminf(fmaxf(fmaf(x, inv, magic), magic - 127.f), magic + 127.f));
 }
-// code 2^e of the byte `sel` of a word of codes whose sign bits are flipped (word ^ 0x80808080):
-// the byte becomes the low bits of 2^23 + 128 + code, and an exact subtraction takes the offset
-// off (before the scale: 2^23 times a large scale would overflow). Four times the rate of the
-// integer conversion.
-__device__ __forceinline__ float tape_value(uint32_t flipped, int sel, float scale) {
-  return (__uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 | sel)) - 8388736.f) * scale;
-}
-
 }  // namespace zjai

@@ -20,8 +20,9 @@ from ._lib import ZjaiError, check
 GROUP = 32  # positions that share an exponent
 STREAM_LEGACY = 1  # CUDA's handle of the legacy default stream, for `Engine.set_stream`
 
-_TORCH_CODE = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-_NUMPY_CODE = {"float32": 0, "float16": 1}
+_NUMPY_CODE = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
+_I8 = np.dtype(np.int8)
+_torch, _torch_code = None, {}
 
 
 def _bad(msg):
@@ -29,7 +30,15 @@ def _bad(msg):
 
 
 def _is_torch(a):
-    return type(a).__module__.startswith("torch")
+    """Whether a is a torch tensor; torch is imported when the first one comes."""
+    global _torch, _torch_code
+    if _torch is None:
+        if isinstance(a, np.ndarray) or not type(a).__module__.startswith("torch"):
+            return False
+        import torch
+        _torch = torch
+        _torch_code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return isinstance(a, _torch.Tensor)
 
 
 class Tape:
@@ -48,97 +57,91 @@ class Tape:
 
 
 class _Call:
-    """The buffers of one call: their pointers, that they lie on one side, the stream order."""
+    """The buffers of one call: the side they lie on (that of `like`), their checks, their pointers
+    and new ones like them, and the stream order."""
 
-    def __init__(self, engine):
-        self.engine, self.mem, self.device = engine, None, None
+    __slots__ = ("engine", "cuda", "device")
 
-    def _side(self, a, what, code):
-        if _is_torch(a):
-            if not a.is_cuda or a.device.index != self.engine.device:
-                raise _bad("%s must be a CUDA tensor of the engine's GPU" % what)
-            if not a.is_contiguous():
-                raise _bad("%s must be contiguous" % what)
-            ptr, mem = a.data_ptr(), _lib.MEM_DEVICE
-            self.device = a.device
-        elif isinstance(a, np.ndarray):
-            if not a.flags.c_contiguous:
-                raise _bad("%s must be contiguous" % what)
-            ptr, mem = a.ctypes.data, _lib.MEM_HOST
-        else:
-            raise _bad("%s must be a numpy array or a CUDA tensor" % what)
+    def __init__(self, engine, like):
+        self.engine = engine
+        self.cuda = _is_torch(like)
+        if self.cuda:
+            self.device = like.device
+            if not like.is_cuda or self.device.index != engine.device:
+                raise _bad("torch tensors must be CUDA tensors of the engine's GPU")
+        elif not isinstance(like, np.ndarray):
+            raise _bad("arguments are numpy arrays or CUDA tensors")
+
+    def code(self, a, what):
+        """Element type of a map."""
+        code = (_torch_code if self.cuda else _NUMPY_CODE).get(a.dtype)
         if code is None:
             raise _bad("%s has an element type that is not taken" % what)
-        if self.mem is None:
-            self.mem = mem
-        elif self.mem != mem:
-            raise _bad("mixed host and device arguments")
-        return ptr
+        return code
 
-    def map(self, a, what, shape=None, code=None):
-        """(pointer, dtype code) of a map, checked against a shape and a type if given."""
-        if a is None:
-            raise _bad("%s is missing" % what)
-        dt = getattr(a, "dtype", None)
-        got = (_TORCH_CODE if _is_torch(a) else _NUMPY_CODE).get(str(dt))
-        ptr = self._side(a, what, got)
-        if code is not None and got != code:
-            raise _bad("%s has another element type" % what)
-        if shape is not None and tuple(a.shape) != shape:
-            raise _bad("%s has shape %s, expected %s" % (what, tuple(a.shape), shape))
-        return ptr, got
+    def ptr(self, a, what, shape, dtype):
+        """Pointer of an array that must have this shape and type and lie with the others."""
+        if self.cuda:
+            if not isinstance(a, _torch.Tensor) or a.device != self.device:
+                raise _bad("%s must be a tensor of the same GPU" % what)
+            contiguous = a.is_contiguous()
+        else:
+            if not isinstance(a, np.ndarray):
+                raise _bad("%s must be a numpy array like the others" % what)
+            contiguous = a.flags.c_contiguous
+        if a.dtype != dtype:
+            raise _bad("%s has type %s, expected %s" % (what, a.dtype, dtype))
+        if a.shape != shape:
+            raise _bad("%s has shape %s, expected %s" % (what, tuple(a.shape), tuple(shape)))
+        if not contiguous:
+            raise _bad("%s must be contiguous" % what)
+        return a.data_ptr() if self.cuda else a.ctypes.data
 
     def param(self, a, what, c):
-        return self.map(a, what, (c,), 0)[0]
+        return self.ptr(a, what, (c,), self.f32)
 
-    def tape(self, t, what, shape=None):
-        """zjai_tape of a Tape, checked against a map's shape."""
+    @property
+    def f32(self):
+        return _torch.float32 if self.cuda else np.dtype(np.float32)
+
+    @property
+    def i8(self):
+        return _torch.int8 if self.cuda else _I8
+
+    def tape(self, t, what, shape):
+        """zjai_tape of a Tape of a map of this shape."""
         if not isinstance(t, Tape):
             raise _bad("%s must be a Tape" % what)
-        for a in (t.codes, t.exps):
-            if str(getattr(a, "dtype", None)).split(".")[-1] != "int8":
-                raise _bad("a tape's codes and exps are int8")
-        codes = self._side(t.codes, what + ".codes", 0)
-        exps = self._side(t.exps, what + ".exps", 0)
-        got = tuple(t.codes.shape)
-        if len(got) not in (3, 4) or (shape is not None and got != shape):
-            raise _bad("%s has shape %s, expected %s" % (what, got, shape or "[(n,) c, h, w]"))
-        if tuple(t.exps.shape) != _exps_shape(got):
-            raise _bad("%s: exps have shape %s, expected %s" % (what, tuple(t.exps.shape),
-                                                               _exps_shape(got)))
-        return _lib.TapeC(codes, exps)
+        return _lib.TapeC(self.ptr(t.codes, what + ".codes", shape, self.i8),
+                          self.ptr(t.exps, what + ".exps", _exps_shape(shape), self.i8))
 
-    def empty(self, shape, like, dtype=None):
-        if _is_torch(like):
-            import torch
-            return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
-        return np.empty(shape, dtype or like.dtype)
+    def empty(self, shape, dtype):
+        if self.cuda:
+            return _torch.empty(shape, dtype=dtype, device=self.device)
+        return np.empty(shape, dtype)
 
-    def new_tape(self, shape, like):
-        i8 = np.int8
-        if _is_torch(like):
-            import torch
-            i8 = torch.int8
-        return Tape(self.empty(shape, like, i8), self.empty(_exps_shape(shape), like, i8))
+    def at(self, a):
+        """Pointer of an array of `empty`."""
+        return a.data_ptr() if self.cuda else a.ctypes.data
 
-    def floats(self, shape, like):
-        if _is_torch(like):
-            import torch
-            return torch.empty(shape, dtype=torch.float32, device=like.device)
-        return np.empty(shape, np.float32)
+    def new_tape(self, shape):
+        t = Tape(self.empty(shape, self.i8), self.empty(_exps_shape(shape), self.i8))
+        return t, _lib.TapeC(self.at(t.codes), self.at(t.exps))
 
     def __call__(self, f, *args):
         """f(engine, *args, mem), in order with torch's current stream."""
-        if self.mem == _lib.MEM_DEVICE:
-            import torch
-            cur = torch.cuda.current_stream(self.device).cuda_stream or STREAM_LEGACY
-            if cur != self.engine.stream:
-                L, h = _lib.lib(), self.engine.handle
-                check(L.zjai_ctx_wait_stream(h, cur))
-                check(f(h, *args, self.mem))
-                check(L.zjai_ctx_release_stream(h, cur))
-                return
-        check(f(self.engine.handle, *args, self.mem))
+        if not self.cuda:
+            check(f(self.engine.handle, *args, _lib.MEM_HOST))
+            return
+        h = self.engine.handle
+        cur = _torch.cuda.current_stream(self.device).cuda_stream or STREAM_LEGACY
+        if cur == self.engine.stream:
+            check(f(h, *args, _lib.MEM_DEVICE))
+            return
+        L = _lib.lib()
+        check(L.zjai_ctx_wait_stream(h, cur))
+        check(f(h, *args, _lib.MEM_DEVICE))
+        check(L.zjai_ctx_release_stream(h, cur))
 
 
 def _exps_shape(shape):
@@ -146,146 +149,156 @@ def _exps_shape(shape):
 
 
 def _dims(shape, what):
-    if len(shape) not in (3, 4):
+    """(n, c, h, w) of a map's shape."""
+    if len(shape) == 4:
+        return shape
+    if len(shape) != 3:
         raise _bad("%s must be [c, h, w] or [n, c, h, w]" % what)
-    return tuple(shape) if len(shape) == 4 else (1,) + tuple(shape)
+    return (1,) + tuple(shape)
 
 
 def tape_pack(engine, x):
     """`Engine.tape_pack`."""
-    call = _Call(engine)
-    px, dt = call.map(x, "x")
-    n, c, h, w = _dims(tuple(x.shape), "x")
-    t = call.new_tape(tuple(x.shape), x)
-    call(_lib.lib().zjai_tape_pack, px, dt, n, c, h, w,
-         ctypes.byref(_lib.TapeC(call._side(t.codes, "codes", 0), call._side(t.exps, "exps", 0))))
+    call = _Call(engine, x)
+    shape = x.shape
+    n, c, h, w = _dims(shape, "x")
+    px = call.ptr(x, "x", shape, x.dtype)
+    code = call.code(x, "x")
+    t, tc = call.new_tape(tuple(shape))
+    call(_lib.lib().zjai_tape_pack, px, code, n, c, h, w, ctypes.byref(tc))
     return t
 
 
 def tape_unpack(engine, tape, dtype=None):
     """`Engine.tape_unpack`."""
-    call = _Call(engine)
-    tc = call.tape(tape, "tape")
-    if dtype is None:
-        if _is_torch(tape.codes):
-            import torch
-            dtype = torch.float32
-        else:
-            dtype = np.float32
-    x = call.empty(tape.shape, tape.codes, dtype)
-    px, dt = call.map(x, "the unpacked map")
-    n, c, h, w = _dims(tape.shape, "tape")
-    call(_lib.lib().zjai_tape_unpack, ctypes.byref(tc), n, c, h, w, px, dt)
+    if not isinstance(tape, Tape):
+        raise _bad("not a Tape")
+    call = _Call(engine, tape.codes)
+    shape = tape.shape
+    n, c, h, w = _dims(shape, "tape")
+    tc = call.tape(tape, "tape", shape)
+    x = call.empty(shape, dtype or call.f32)
+    call(_lib.lib().zjai_tape_unpack, ctypes.byref(tc), n, c, h, w, call.at(x),
+         call.code(x, "the unpacked map"))
     return x
 
 
 def _params(call, c, post, scale, pre):
     prm = _lib.ResidualParams()
-    for name, pair in (("post", post), ("pre", pre)):
-        if pair is not None:
-            if not isinstance(pair, (tuple, list)) or len(pair) != 2:
-                raise _bad("%s is a pair (weight, bias)" % name)
-            setattr(prm, name + "_weight", call.param(pair[0], name + " weight", c))
-            setattr(prm, name + "_bias", call.param(pair[1], name + " bias", c))
+    if post is not None:
+        weight, bias = _pair(post, "post")
+        prm.post_weight = call.param(weight, "post weight", c)
+        prm.post_bias = call.param(bias, "post bias", c)
     if scale is not None:
         prm.scale = call.param(scale, "scale", c)
+    if pre is not None:
+        weight, bias = _pair(pre, "pre")
+        prm.pre_weight = call.param(weight, "pre weight", c)
+        prm.pre_bias = call.param(bias, "pre bias", c)
     return prm
+
+
+def _pair(p, what):
+    if not isinstance(p, (tuple, list)) or len(p) != 2:
+        raise _bad("%s is a pair (weight, bias)" % what)
+    return p
 
 
 def _gate_shape(gate, shape):
     """Shape of the gate's map: the branch's, or one channel."""
     got = tuple(gate.shape)
-    one = shape[:-3] + (1,) + shape[-2:]
-    if got != shape and got != one:
-        raise _bad("gate has shape %s, expected %s or %s" % (got, shape, one))
+    if got != shape and got != shape[:-3] + (1,) + shape[-2:]:
+        raise _bad("gate has shape %s, expected %s or one channel of it" % (got, shape))
     return got
 
 
 def gated_residual_norm(engine, x, f, post=None, gate=None, scale=None, pre=None, tape=()):
     """`Engine.gated_residual_norm`."""
-    call = _Call(engine)
-    px, dt = call.map(x, "x")
-    shape = tuple(x.shape)
+    call = _Call(engine, x)
+    shape, dt = tuple(x.shape), x.dtype
     n, c, h, w = _dims(shape, "x")
-    pf = call.map(f, "f", shape, dt)[0]
-    pg, gc, gshape = None, 0, None
+    code = call.code(x, "x")
+    px, pf = call.ptr(x, "x", shape, dt), call.ptr(f, "f", shape, dt)
+    pg, gc = None, 0
     if gate is not None:
         gshape = _gate_shape(gate, shape)
-        pg, gc = call.map(gate, "gate", gshape, dt)[0], gshape[-3]
+        pg, gc = call.ptr(gate, "gate", gshape, dt), gshape[-3]
     prm = _params(call, c, post, scale, pre)
-    y = call.empty(shape, x)
-    z = call.empty(shape, x) if pre is not None else None
-    tapes, tc = {}, _lib.ResidualTapes()
+    y = call.empty(shape, dt)
+    z = call.empty(shape, dt) if pre is not None else None
+    tapes, tc = {}, None
     for name in tape:
         if name not in ("f", "gate", "y", "z"):
             raise _bad("tape names are f, gate, y and z")
         if (name == "gate" and gate is None) or (name == "z" and pre is None):
             continue
-        tapes[name] = t = call.new_tape(gshape if name == "gate" else shape, x)
-        setattr(tc, name, call.tape(t, name))
-    call(_lib.lib().zjai_gated_residual_norm, px, pf, pg, gc, dt, n, c, h, w, ctypes.byref(prm),
-         call.map(y, "y")[0], call.map(z, "z")[0] if z is not None else None,
-         ctypes.byref(tc) if tapes else None)
+        tc = tc or _lib.ResidualTapes()
+        tapes[name], one = call.new_tape(gshape if name == "gate" else shape)
+        setattr(tc, name, one)
+    call(_lib.lib().zjai_gated_residual_norm, px, pf, pg, gc, code, n, c, h, w, ctypes.byref(prm),
+         call.at(y), call.at(z) if z is not None else None, ctypes.byref(tc) if tc else None)
     return y, z, tapes
 
 
 def gated_residual_norm_backward(engine, dy, dz=None, f=None, y=None, post=None, gate=None,
                                  scale=None, pre=None):
     """`Engine.gated_residual_norm_backward`."""
-    call = _Call(engine)
-    pdy, dt = call.map(dy, "dy")
-    shape = tuple(dy.shape)
+    call = _Call(engine, dy)
+    shape, dt = tuple(dy.shape), dy.dtype
     n, c, h, w = _dims(shape, "dy")
-    pdz = call.map(dz, "dz", shape, dt)[0] if pre is not None else None
-    if dz is not None and pre is None:
-        raise _bad("dz without pre")
+    code = call.code(dy, "dy")
+    pdy = call.ptr(dy, "dy", shape, dt)
+    if (dz is None) != (pre is None):
+        raise _bad("dz goes with pre")
+    pdz = call.ptr(dz, "dz", shape, dt) if pre is not None else None
     prm = _params(call, c, post, scale, pre)
-    need_f = post is not None or scale is not None or gate is not None
-    kept = {"f": f if need_f else None, "gate": gate, "y": y if pre is not None else None}
-    for name, needed in (("f", need_f), ("y", pre is not None)):
-        if needed and kept[name] is None:
-            raise _bad("%s is missing" % name)
-    used = [v for v in kept.values() if v is not None]
-    taped = bool(used) and isinstance(used[0], Tape)
-    if any(isinstance(v, Tape) != taped for v in used):
-        raise _bad("f, gate and y are all Tapes or all maps")
-    gshape = _gate_shape(gate, shape) if gate is not None else None
-    ptr, tc = {}, _lib.ResidualTapes()
+    kept = {}
+    if post is not None or scale is not None or gate is not None:
+        kept["f"] = f
+    if pre is not None:
+        kept["y"] = y
+    gshape = None
+    if gate is not None:
+        kept["gate"], gshape = gate, _gate_shape(gate, shape)
+    taped = any(isinstance(v, Tape) for v in kept.values())
+    ptr, tc = {"f": None, "y": None, "gate": None}, _lib.ResidualTapes() if taped else None
     for name, v in kept.items():
-        ptr[name] = None
         if v is None:
-            continue
+            raise _bad("%s is missing" % name)
         want = gshape if name == "gate" else shape
-        if taped:
+        if taped:  # all of them
             setattr(tc, name, call.tape(v, name, want))
         else:
-            ptr[name] = call.map(v, name, want, dt)[0]
-    out = {"x": call.empty(shape, dy), "f": call.empty(shape, dy)}
+            ptr[name] = call.ptr(v, name, want, dt)
+    out = {"x": call.empty(shape, dt), "f": call.empty(shape, dt)}
     if gate is not None:
-        out["gate"] = call.empty(gshape, dy)
-    names = [k for k, on in (("post_weight", post), ("post_bias", post), ("scale", scale),
-                             ("pre_weight", pre), ("pre_bias", pre)) if on is not None]
-    for k in names:
-        out[k] = call.floats((c,), dy)
+        out["gate"] = call.empty(gshape, dt)
+    names = ((["post_weight", "post_bias"] if post is not None else [])
+             + (["scale"] if scale is not None else [])
+             + (["pre_weight", "pre_bias"] if pre is not None else []))
+    if names:  # rows of one array
+        out.update(zip(names, call.empty((len(names), c), call.f32)))
     gr = _lib.ResidualGrads()
     for k, v in out.items():
-        setattr(gr, k, call.map(v, k)[0])
+        setattr(gr, k, call.at(v))
     call(_lib.lib().zjai_gated_residual_norm_backward, pdy, pdz, ptr["f"], ptr["gate"],
-         gshape[-3] if gshape else 0, ptr["y"], ctypes.byref(tc) if taped else None, dt, n, c, h, w,
-         ctypes.byref(prm), ctypes.byref(gr))
+         gshape[-3] if gshape else 0, ptr["y"], ctypes.byref(tc) if taped else None, code, n, c, h,
+         w, ctypes.byref(prm), ctypes.byref(gr))
     return out
 
 
 def conv1x1_weight_grad(engine, dout, tape):
     """`Engine.conv1x1_weight_grad`."""
-    call = _Call(engine)
-    pd, dt = call.map(dout, "dout")
-    n, oc, h, w = _dims(tuple(dout.shape), "dout")
-    if not isinstance(tape, Tape):
-        raise _bad("the input must be a Tape")
-    c = tape.shape[-3] if len(tape.shape) in (3, 4) else 0
-    tc = call.tape(tape, "tape", tuple(dout.shape[:-3]) + (c, h, w))
-    dw, db = call.floats((oc, c), dout), call.floats((oc,), dout)
-    call(_lib.lib().zjai_conv1x1_weight_grad, pd, dt, n, oc, c, h, w, ctypes.byref(tc),
-         call.map(dw, "dw")[0], call.map(db, "db")[0])
+    call = _Call(engine, dout)
+    shape = tuple(dout.shape)
+    n, oc, h, w = _dims(shape, "dout")
+    code = call.code(dout, "dout")
+    pd = call.ptr(dout, "dout", shape, dout.dtype)
+    if not isinstance(tape, Tape) or len(tape.shape) != len(shape):
+        raise _bad("the input must be a Tape with dout's dimensions")
+    c = tape.shape[-3]
+    tc = call.tape(tape, "tape", shape[:-3] + (c, h, w))
+    dw, db = call.empty((oc, c), call.f32), call.empty((oc,), call.f32)
+    call(_lib.lib().zjai_conv1x1_weight_grad, pd, code, n, oc, c, h, w, ctypes.byref(tc),
+         call.at(dw), call.at(db))
     return dw, db
