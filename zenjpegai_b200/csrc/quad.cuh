@@ -25,10 +25,8 @@ __device__ __forceinline__ F4 fma4(F4 x, F4 y, F4 z) {
 __device__ __forceinline__ F4 all(float v) {
   return {make_float2(v, v), make_float2(v, v)};
 }
-__device__ __forceinline__ F4 operator-(F4 x) {
-  return {make_float2(-x.a.x, -x.a.y), make_float2(-x.b.x, -x.b.y)};
-}
-__device__ __forceinline__ F4 operator-(F4 x, F4 y) { return x + (-y); }
+// one exact product and one rounding, as a subtraction (packed operands take no sign)
+__device__ __forceinline__ F4 operator-(F4 x, F4 y) { return fma4(y, all(-1.f), x); }
 __device__ __forceinline__ F4 make4(float4 v) {
   return {make_float2(v.x, v.y), make_float2(v.z, v.w)};
 }
@@ -138,16 +136,17 @@ __device__ __forceinline__ uint32_t codes4(F4 v, uint32_t m) {
   return w;
 }
 // Hold four positions of a row (zeros behind its end) as part of a tape's group; the row's eight
-// lanes call together, whole warps (`on`: the row exists).
+// lanes call together, whole warps (`on`: the row exists). e0: the row's first element, ge: the
+// group's place among the exponents.
 template <bool kVec>
-__device__ __forceinline__ void tape_store4(const zjai_tape& t, long long row, int groups, int g,
-                                            int at, int p, F4 v, bool on) {
+__device__ __forceinline__ void tape_store4(const zjai_tape& t, long long e0, long long ge, int at,
+                                            int p, F4 v, bool on) {
   uint32_t m = amax4(v);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (!on) return;
   const uint32_t w = codes4(v, m);
-  int8_t* codes = t.codes + row * p;
+  int8_t* codes = t.codes + e0;
   if constexpr (kVec) {
     if (at < p) *reinterpret_cast<uint32_t*>(codes + at) = w;
   } else {
@@ -155,7 +154,7 @@ __device__ __forceinline__ void tape_store4(const zjai_tape& t, long long row, i
     for (int i = 0; i < 4; ++i)
       if (at + i < p) codes[at + i] = (int8_t)(w >> (8 * i) & 0xffu);
   }
-  if ((threadIdx.x & 7) == 0) t.exps[row * groups + g] = (int8_t)tape_exp(m);
+  if ((threadIdx.x & 7) == 0) t.exps[ge] = (int8_t)tape_exp(m);
 }
 // value of positions behind the row's end set to zero
 template <bool kVec>

@@ -16,20 +16,26 @@ struct FwdArgs {
 };
 
 template <int kRows, bool kVec, class T>
-__global__ void __launch_bounds__(kThreadsMost, kRows == 4 ? 1 : 2)
-    residual_norm_kernel(const FwdArgs<T> a) {
+__global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const FwdArgs<T> a) {
   __shared__ Exchange<2> ex;
+  __shared__ Params<kRows> prm;
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Rows<kRows> rows(a.c, warps);
   constexpr int kHeld = kRows ? kRows : 1;
   const int groups = (int)tape_groups(a.p);
+  const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
+  prm.load(a.prm, a.c);
+  __syncthreads();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const long long img = tile / groups, base = img * a.c;
     const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
+    // a row's first element; its group's place among the exponents
+    auto e0 = [&](int j) { return (base + rows.row(j)) * a.p; };
+    auto ge = [&](int j) { return (base + rows.row(j)) * groups + g; };
     F4 f[kHeld], x[kHeld], q[kHeld];  // branch, input (then y), gate logits
     auto load = [&](const T* v, int j) {
-      return rows.on(j) ? load4<kVec>(v + (base + rows.row(j)) * a.p, at, a.p) : all(0.f);
+      return rows.on(j) ? load4<kVec>(v + e0(j), at, a.p) : all(0.f);
     };
     if (kRows) {
       FOR_ROWS(j) f[j % kHeld] = load(a.f, j);
@@ -43,39 +49,37 @@ __global__ void __launch_bounds__(kThreadsMost, kRows == 4 ? 1 : 2)
       gate1 = load4<kVec>(a.gate + img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
     }
-    F4 m = all(0.f), r = all(1.f);
+    F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
-      stats_part(rows, v, ex, 0);
+      stats_part(rows, v, ex, 0, warps);
       __syncthreads();
-      if (wp == 0) stats_join<kRows>(ex, 0, a.c, warps);
+      stats_join(rows, ex, 0, inv_c, warps, wp, warps);
       __syncthreads();
-      m = total4(ex, 0);
+      nm = total4(ex, 0);
       r = total4(ex, 1);
     };
     if (post) exchange(f_of);
-    const F4 m1 = m, r1 = r;
+    const F4 nm1 = nm, r1 = r;
     auto y_of = [&](int j) {
       const int ch = rows.param(j);
       F4 u = f_of(j), s = sg1;
       if (post)
-        u = fma4((u - m1) * r1, all(__ldg(a.prm.post_weight + ch)), all(__ldg(a.prm.post_bias + ch)));
+        u = fma4((u + nm1) * r1, prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch));
       if (per_row) sigmoid4(gate_of(j), &s, &unused);
-      if (a.prm.scale) s = s * all(__ldg(a.prm.scale + ch));
-      return fma4(s, u, kRows ? x[j % kHeld] : load(a.x, j));
+      return fma4(s * prm.get(a.prm, kScale, ch), u, kRows ? x[j % kHeld] : load(a.x, j));
     };
     // y and the tapes of f, gate and y (whole warps call)
     auto emit = [&](int j, F4 y) {
       const bool on = rows.on(j);
-      const long long row = base + rows.row(j);
-      if (on) store4<kVec>(a.y + row * a.p, at, a.p, y);
-      if (a.tp.f.codes) tape_store4<kVec>(a.tp.f, row, groups, g, at, a.p, f_of(j), on);
+      if (on) store4<kVec>(a.y + e0(j), at, a.p, y);
+      if (a.tp.f.codes) tape_store4<kVec>(a.tp.f, e0(j), ge(j), at, a.p, f_of(j), on);
       if (per_row && a.tp.gate.codes)
-        tape_store4<kVec>(a.tp.gate, row, groups, g, at, a.p, gate_of(j), on);
+        tape_store4<kVec>(a.tp.gate, e0(j), ge(j), at, a.p, gate_of(j), on);
       if (a.tp.y.codes)
-        tape_store4<kVec>(a.tp.y, row, groups, g, at, a.p, clip4<kVec>(y, at, a.p), on);
+        tape_store4<kVec>(a.tp.y, e0(j), ge(j), at, a.p, clip4<kVec>(y, at, a.p), on);
     };
     if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
-      tape_store4<kVec>(a.tp.gate, img, groups, g, at, a.p, gate1, lane < 8);
+      tape_store4<kVec>(a.tp.gate, img * a.p, img * groups + g, at, a.p, gate1, lane < 8);
     if (kRows) {
       FOR_ROWS(j) {
         const F4 y = y_of(j);
@@ -91,11 +95,10 @@ __global__ void __launch_bounds__(kThreadsMost, kRows == 4 ? 1 : 2)
       if (!kRows) emit(j, y);
       if (!pre) continue;
       const int ch = rows.param(j);
-      const F4 z = fma4((y - m) * r, all(__ldg(a.prm.pre_weight + ch)), all(__ldg(a.prm.pre_bias + ch)));
-      const long long row = base + rows.row(j);
-      if (rows.on(j)) store4<kVec>(a.z + row * a.p, at, a.p, z);
+      const F4 z = fma4((y + nm) * r, prm.get(a.prm, kPreW, ch), prm.get(a.prm, kPreB, ch));
+      if (rows.on(j)) store4<kVec>(a.z + e0(j), at, a.p, z);
       if (a.tp.z.codes)
-        tape_store4<kVec>(a.tp.z, row, groups, g, at, a.p, clip4<kVec>(z, at, a.p), rows.on(j));
+        tape_store4<kVec>(a.tp.z, e0(j), ge(j), at, a.p, clip4<kVec>(z, at, a.p), rows.on(j));
     }
   }
 }
@@ -149,7 +152,7 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->codes, tr[i] * p, 1, mem, "codes", &tt[i]->codes));
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->exps, tr[i] * groups, 1, mem, "exps", &tt[i]->exps));
     }
-    const Shape sh = shape_of(c);
+    const Shape sh = shape_of(c, false);
     VecCheck vec(p);
     vec.map(dx, es).map(df, es).map(dg, es).map(dyo, es).map(dzo, es);
     for (zjai_tape* t : tt) vec.map(t->codes, 1);

@@ -16,8 +16,8 @@
 // three times the instructions, and issue slots bounded the kernels, not HBM). Up to 256 channels
 // a block holds its tile in registers (kRows rows a thread) and reads everything once; above, rows
 // are read again for each pass, mostly from the caches. A position's sums go over the warps'
-// shared-memory partials, gathered by one warp. Statistics: a mean and sum of squared deviations
-// per warp, joined by their exact update formula (sums of squares would cancel).
+// shared-memory partials, gathered by four lanes each. Statistics: a mean and sum of squared
+// deviations per warp, joined by their exact update formula (sums of squares would cancel).
 // The products in a - mean a and b - mean b are the ones that were summed (not fused): with one
 // channel they cancel to zero. Both kernels are bound by HBM at large sizes.
 #pragma once
@@ -47,7 +47,7 @@ __device__ __forceinline__ void sigmoid4(F4 g, F4* s, F4* one_minus) {
   sigmoid2(g.b.y, &s->b.y, &one_minus->b.y);
 }
 
-// over the four rows of a warp: lanes with the same positions
+// Sum over the four rows of a warp (lanes with the same positions), to all of them.
 __device__ __forceinline__ F4 over_rows(F4 v) {
   float f[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
 #pragma unroll
@@ -57,37 +57,46 @@ __device__ __forceinline__ F4 over_rows(F4 v) {
   }
   return {make_float2(f[0], f[1]), make_float2(f[2], f[3])};
 }
+// The same sum, one position a lane, to part[position]: halves of the positions are exchanged, so
+// that three shuffles do for four values.
+__device__ __forceinline__ void rows_to_part(F4 v, float* part) {
+  const int lane = threadIdx.x & 31;
+  const bool b3 = lane & 8, b4 = lane & 16;
+  float x = b3 ? v.b.x : v.a.x, y = b3 ? v.b.y : v.a.y;
+  x += __shfl_xor_sync(0xffffffffu, b3 ? v.a.x : v.b.x, 8);
+  y += __shfl_xor_sync(0xffffffffu, b3 ? v.a.y : v.b.y, 8);
+  float t = b4 ? y : x;
+  t += __shfl_xor_sync(0xffffffffu, b4 ? x : y, 16);
+  part[(lane & 7) * 4 + (b3 ? 2 : 0) + (b4 ? 1 : 0)] = t;
+}
 
 // The block's partial sums per warp and position, and their totals.
 template <int kVals>
 struct Exchange {
-  float part[kMaxWarps][kVals][32], total[kVals][32];
+  float part[kVals][kMaxWarps][32], total[kVals][32];
 };
 
 // Rows of the calling thread: row(j) for j < rows(). kRows > 0: held in registers, consecutive
 // groups of four per warp; 0: any number, strided over the block.
 template <int kRows>
 struct Rows {
-  int c, first, step, n, warp_rows;
+  int c, first, step, n;
   __device__ __forceinline__ Rows(int c_, int warps) : c(c_) {
     const int wp = threadIdx.x >> 5, rg = (threadIdx.x & 31) >> 3;
-    if (kRows) {
-      first = wp * 4 * kRows + rg;
-      step = 4;
-      n = kRows;
-      warp_rows = max(0, min(c - wp * 4 * kRows, 4 * kRows));
-    } else {
-      first = wp * 4 + rg;
-      step = 4 * warps;
-      n = (c + step - 1) / step;
-      const int whole = c / step, rest = c - whole * step - wp * 4;
-      warp_rows = whole * 4 + max(0, min(4, rest));
-    }
+    first = wp * 4 * (kRows ? kRows : 1) + rg;
+    step = kRows ? 4 : 4 * warps;
+    n = kRows ? kRows : (c + step - 1) / step;
   }
   __device__ __forceinline__ int row(int j) const { return first + j * step; }
   __device__ __forceinline__ bool on(int j) const { return row(j) < c; }
   // a row that exists, to read for one that does not
   __device__ __forceinline__ int param(int j) const { return min(row(j), c - 1); }
+  // rows of a warp
+  __device__ __forceinline__ int of_warp(int w, int warps) const {
+    if (kRows) return max(0, min(c - w * 4 * kRows, 4 * kRows));
+    const int whole = c / (4 * warps);
+    return whole * 4 + max(0, min(4, c - whole * 4 * warps - w * 4));
+  }
 };
 #define FOR_ROWS(j) _Pragma("unroll") for (int j = 0; j < (kRows ? kRows : rows.n); ++j)
 
@@ -95,63 +104,106 @@ struct Rows {
 // val + 1.
 template <int kRows, int kVals, class V>
 __device__ __forceinline__ void stats_part(const Rows<kRows>& rows, V&& v, Exchange<kVals>& ex,
-                                           int val) {
+                                           int val, int warps) {
   const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   F4 s = all(0.f), q = all(0.f);
   FOR_ROWS(j) if (rows.on(j)) s = s + v(j);
   s = over_rows(s);
-  const F4 m = s * all(rows.warp_rows ? 1.f / (float)rows.warp_rows : 0.f);
+  const int n = rows.of_warp(wp, warps);
+  const F4 nm = s * all(n ? __fdividef(-1.f, (float)n) : 0.f);
   FOR_ROWS(j) if (rows.on(j)) {
-    const F4 d = v(j) - m;
+    const F4 d = v(j) + nm;
     q = fma4(d, d, q);
   }
-  q = over_rows(q);
-  if (lane < 8) {
-    *reinterpret_cast<float4*>(&ex.part[wp][val][lane * 4]) = flat(s);
-    *reinterpret_cast<float4*>(&ex.part[wp][val + 1][lane * 4]) = flat(q);
-  }
+  if (lane < 8) *reinterpret_cast<float4*>(&ex.part[val][wp][lane * 4]) = flat(s);
+  rows_to_part(q, ex.part[val + 1][wp]);
 }
-// Joined by one warp: ex.total at val, val + 1 the mean and 1 / sigma.
-template <int kRows, int kVals>
-__device__ __forceinline__ void stats_join(Exchange<kVals>& ex, int val, int c, int warps) {
+// A quarter of the positions per warp (of `of` that call, the `nth`): four lanes a position, each
+// with every fourth warp's partials.
+template <class F>
+__device__ __forceinline__ void by_position(int nth, int of, F&& f) {
   const int lane = threadIdx.x & 31;
-  float s = 0.f, q = 0.f;
-  for (int w = 0; w < warps; ++w) s += ex.part[w][val][lane];
-  const float m = s / (float)c;
-  for (int w = 0; w < warps; ++w) {
-    // rows of warp w, as in Rows
-    int n;
-    if (kRows) {
-      n = max(0, min(c - w * 4 * kRows, 4 * kRows));
-    } else {
-      const int whole = c / (4 * warps);
-      n = whole * 4 + max(0, min(4, c - whole * 4 * warps - w * 4));
+  for (int b = nth; b < 4; b += of) f(b * 8 + (lane & 7), lane >> 3);
+}
+__device__ __forceinline__ float over_subs(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+// Joined: ex.total at val, val + 1 the negated mean and 1 / sigma. Partials' means are joined by
+// M2 = sum of M2_w + n_w (mean_w - mean)^2.
+template <int kRows, int kVals>
+__device__ __forceinline__ void stats_join(const Rows<kRows>& rows, Exchange<kVals>& ex, int val,
+                                           float inv_c, int warps, int nth, int of) {
+  by_position(nth, of, [&](int pos, int sub) {
+    float s[kMaxWarps / 4], sum = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxWarps / 4; ++i) {
+      const int w = i * 4 + sub;
+      s[i] = w < warps ? ex.part[val][w][pos] : 0.f;
+      sum += s[i];
     }
-    if (!n) continue;
-    const float d = ex.part[w][val][lane] / (float)n - m;
-    q += ex.part[w][val + 1][lane] + (float)n * d * d;
-  }
-  ex.total[val][lane] = m;
-  ex.total[val + 1][lane] = rsqrtf(q / (float)c + kEps);
+    const float m = over_subs(sum) * inv_c;
+#pragma unroll
+    for (int i = 0; i < kMaxWarps / 4; ++i) {
+      const int w = i * 4 + sub, n = w < warps ? rows.of_warp(w, warps) : 0;
+      if (n) {
+        const float d = __fdividef(s[i], (float)n) - m;
+        q += fmaf((float)n * d, d, ex.part[val + 1][w][pos]);
+      }
+    }
+    q = over_subs(q);
+    if (sub == 0) {
+      ex.total[val][pos] = -m;
+      ex.total[val + 1][pos] = rsqrtf(fmaf(q, inv_c, kEps));
+    }
+  });
 }
 template <int kVals>
 __device__ __forceinline__ F4 total4(const Exchange<kVals>& ex, int val) {
   return make4(*reinterpret_cast<const float4*>(&ex.total[val][(threadIdx.x & 7) * 4]));
 }
-// Sums s (already over the thread's rows) to ex.part, and their joining.
+// Sums over the warps of ex.part at val, times k.
 template <int kVals>
-__device__ __forceinline__ void sum_part(F4 s, Exchange<kVals>& ex, int val) {
-  s = over_rows(s);
-  if ((threadIdx.x & 31) < 8)
-    *reinterpret_cast<float4*>(&ex.part[threadIdx.x >> 5][val][(threadIdx.x & 7) * 4]) = flat(s);
+__device__ __forceinline__ void sum_join(Exchange<kVals>& ex, int val, float k, int warps, int nth,
+                                         int of) {
+  by_position(nth, of, [&](int pos, int sub) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxWarps / 4; ++i)
+      if (i * 4 + sub < warps) s += ex.part[val][i * 4 + sub][pos];
+    s = over_subs(s);
+    if (sub == 0) ex.total[val][pos] = s * k;
+  });
 }
-template <int kVals>
-__device__ __forceinline__ void sum_join(Exchange<kVals>& ex, int val, int warps) {
-  const int lane = threadIdx.x & 31;
-  float s = 0.f;
-  for (int w = 0; w < warps; ++w) s += ex.part[w][val][lane];
-  ex.total[val][lane] = s;
-}
+
+// The parameters of a channel in all four positions: doubled in shared memory where rows are held
+// (up to kHeldC channels), else from global memory. Absent ones are those of the identity.
+constexpr int kHeldC = 256;
+enum { kPostW, kPostB, kScale, kPreW, kPreB, kParams };
+template <int kRows>
+struct Params {
+  float2 v[kRows ? kParams : 1][kRows ? kHeldC : 1];
+  static __device__ __forceinline__ const float* of(const zjai_residual_params& p, int k) {
+    return k == kPostW ? p.post_weight : k == kPostB ? p.post_bias : k == kScale ? p.scale
+           : k == kPreW ? p.pre_weight : p.pre_bias;
+  }
+  static __device__ __forceinline__ float one(const zjai_residual_params& p, int k, int ch) {
+    const float* q = of(p, k);
+    return q ? __ldg(q + ch) : (k == kPostB || k == kPreB ? 0.f : 1.f);
+  }
+  __device__ __forceinline__ void load(const zjai_residual_params& p, int c) {
+    if (kRows)
+      for (int i = threadIdx.x; i < kParams * c; i += blockDim.x) {
+        const float x = one(p, i / c, i % c);
+        v[i / c][i % c] = make_float2(x, x);
+      }
+  }
+  __device__ __forceinline__ F4 get(const zjai_residual_params& p, int k, int ch) const {
+    if (!kRows) return all(one(p, k, ch));
+    const float2 x = v[k][ch];
+    return {x, x};
+  }
+};
 
 constexpr int kThreadsMost = 32 * kMaxWarps;
 
@@ -168,21 +220,20 @@ int stage_params(Ctx* ctx, const zjai_residual_params& in, int c, int mem,
   return stage_param(ctx, in.pre_bias, c, mem, "pre_bias", &out->pre_bias);
 }
 
-// Rows a thread holds for c channels (0: not held) and the block's warps.
+// Rows a thread holds for c channels (0: not held) and the block's warps. Sixteen warps an SM are
+// resident at the registers that __launch_bounds__ leaves, so blocks of few warps come in numbers.
 struct Shape {
   int rows, warps, per_sm;
 };
-Shape shape_of(int c) {
-  const int rows = c <= 64 ? 1 : c <= 128 ? 2 : c <= 256 ? 4 : 0;
+Shape shape_of(int c, bool backward) {
+  // the backward pass holds twice as much a row: two rows a thread where the warps allow it
+  const int rows = c > kHeldC ? 0 : backward && c <= kHeldC / 2 ? 2 : 4;
   const int warps = rows ? (c + 4 * rows - 1) / (4 * rows) : kMaxWarps;
-  // blocks that are resident at the register limits of __launch_bounds__
-  const int least = rows == 4 ? 1 : 2;
-  return {rows, warps, std::max(1, std::min(16, least * kMaxWarps / warps))};
+  return {rows, warps, kMaxWarps / warps};
 }
 // f(std::integral_constant) with the rows held
 template <class F>
 int by_rows(int rows, F&& f) {
-  if (rows == 1) return f(std::integral_constant<int, 1>());
   if (rows == 2) return f(std::integral_constant<int, 2>());
   if (rows == 4) return f(std::integral_constant<int, 4>());
   return f(std::integral_constant<int, 0>());

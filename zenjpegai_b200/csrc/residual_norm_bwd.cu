@@ -16,13 +16,13 @@ struct BwdArgs {
   float* sums;  // [blocks][5][c]: scale, post_weight, post_bias, pre_weight, pre_bias
 };
 
-// A row's four positions of a kept map: codes and exponent of a tape, or values.
+// A row's four positions of a kept map, codes and exponent of a tape or values, as loaded.
 template <bool kTaped, bool kVec, class T>
 struct Kept {
   F4 v;
-  __device__ __forceinline__ void load(const T* map, const zjai_tape&, long long row, int, int,
+  __device__ __forceinline__ void load(const T* map, const zjai_tape&, long long e0, long long,
                                        int at, int p) {
-    v = load4<kVec>(map + row * p, at, p);
+    v = load4<kVec>(map + e0, at, p);
   }
   __device__ __forceinline__ F4 get() const { return v; }
 };
@@ -30,10 +30,10 @@ template <bool kVec, class T>
 struct Kept<true, kVec, T> {
   uint32_t w;
   int e;
-  __device__ __forceinline__ void load(const T*, const zjai_tape& t, long long row, int groups,
-                                       int g, int at, int p) {
-    w = load_codes<kVec>(t.codes + row * p, at, p);
-    e = __ldg(t.exps + row * groups + g);
+  __device__ __forceinline__ void load(const T*, const zjai_tape& t, long long e0, long long ge,
+                                       int at, int p) {
+    w = load_codes<kVec>(t.codes + e0, at, p);
+    e = __ldg(t.exps + ge);
   }
   __device__ __forceinline__ F4 get() const { return taped4(w, e); }
 };
@@ -41,9 +41,9 @@ struct Kept<true, kVec, T> {
 // The parameter gradients are summed over a block's tiles (in registers, or per channel in shared
 // memory where rows are not held) and written out per block.
 template <int kRows, bool kTaped, bool kVec, class T>
-__global__ void __launch_bounds__(kThreadsMost, 1)
-    residual_norm_bwd_kernel(const BwdArgs<T> a) {
+__global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(const BwdArgs<T> a) {
   __shared__ Exchange<4> ex;
+  __shared__ Params<kRows> prm;
   extern __shared__ float acc_c[];  // [5][c] where rows are not held
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Rows<kRows> rows(a.c, warps);
@@ -52,122 +52,123 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
   const bool need_f = post || a.gate_c || a.prm.scale;
-  const int second = warps > 1 ? 1 : 0;  // warp that joins the second of two sums
+  // two sums at a time are joined by four warps each where there are eight
+  const bool two = warps >= 8;
+  auto join_first = [&](auto f) {
+    if (!two || wp < 4) f(two ? wp : wp, two ? 4 : warps);
+  };
+  auto join_second = [&](auto f) {
+    if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
+  };
   float acc[kHeld][5];
 #pragma unroll
   for (int j = 0; j < kHeld; ++j)
 #pragma unroll
     for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
-  if (!kRows) {
+  if (!kRows)
     for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
-    __syncthreads();
-  }
+  prm.load(a.prm, a.c);
+  __syncthreads();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const long long img = tile / groups, base = img * a.c;
     const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
     using K = Kept<kTaped, kVec, T>;
-    F4 dy[kHeld], dz[kHeld];
-    K f[kHeld], y[kHeld], q[kHeld];
+    auto e0 = [&](int j) { return (base + rows.param(j)) * a.p; };
     auto grad = [&](const T* v, int j) {
-      return rows.on(j) ? load4<kVec>(v + (base + rows.row(j)) * a.p, at, a.p) : all(0.f);
+      return rows.on(j) ? load4<kVec>(v + e0(j), at, a.p) : all(0.f);
     };
     auto kept = [&](const T* v, const zjai_tape& t, int j) {
       K k;
-      k.load(v, t, base + rows.param(j), groups, g, at, a.p);
+      k.load(v, t, e0(j), (base + rows.param(j)) * groups + g, at, a.p);
       return k;
     };
+    // held: f then LN(f), y then LN(y), dy then b, dz, the gate as kept
+    F4 f[kHeld], y[kHeld], dy[kHeld], dz[kHeld];
+    K q[kHeld];
     if (kRows) {
-      if (pre) FOR_ROWS(j) y[j % kHeld] = kept(a.y, a.tp.y, j);
-      if (need_f) FOR_ROWS(j) f[j % kHeld] = kept(a.f, a.tp.f, j);
+      K kf[kHeld], ky[kHeld];
+      if (pre) FOR_ROWS(j) ky[j % kHeld] = kept(a.y, a.tp.y, j);
+      if (need_f) FOR_ROWS(j) kf[j % kHeld] = kept(a.f, a.tp.f, j);
       if (pre) FOR_ROWS(j) dz[j % kHeld] = grad(a.dz, j);
-      FOR_ROWS(j) dy[j % kHeld] = grad(a.dy, j);
       if (per_row) FOR_ROWS(j) q[j % kHeld] = kept(a.gate, a.tp.gate, j);
+      FOR_ROWS(j) dy[j % kHeld] = grad(a.dy, j);
+      if (pre) FOR_ROWS(j) y[j % kHeld] = ky[j % kHeld].get();
+      if (need_f) FOR_ROWS(j) f[j % kHeld] = kf[j % kHeld].get();
     }
-    auto f_of = [&](int j) { return kRows ? f[j % kHeld].get() : kept(a.f, a.tp.f, j).get(); };
-    auto y_of = [&](int j) { return kRows ? y[j % kHeld].get() : kept(a.y, a.tp.y, j).get(); };
-    auto gate_of = [&](int j) {
-      return kRows ? q[j % kHeld].get() : kept(a.gate, a.tp.gate, j).get();
-    };
+    auto f_of = [&](int j) { return kRows ? f[j % kHeld] : kept(a.f, a.tp.f, j).get(); };
+    auto y_of = [&](int j) { return kRows ? y[j % kHeld] : kept(a.y, a.tp.y, j).get(); };
     auto dz_of = [&](int j) { return kRows ? dz[j % kHeld] : grad(a.dz, j); };
     F4 sg1 = all(1.f), os1 = all(0.f);
     if (a.gate_c == 1) {
       K k;
-      k.load(a.gate, a.tp.gate, img, groups, g, at, a.p);
+      k.load(a.gate, a.tp.gate, img * a.p, img * groups + g, at, a.p);
       sigmoid4(k.get(), &sg1, &os1);
     }
-    F4 m1 = all(0.f), r1 = all(1.f), m2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
-    if (post) stats_part(rows, f_of, ex, 0);
-    if (pre) stats_part(rows, y_of, ex, 2);
+    F4 nm1 = all(0.f), r1 = all(1.f), nm2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
+    if (post) stats_part(rows, f_of, ex, 0, warps);
+    if (pre) stats_part(rows, y_of, ex, 2, warps);
     if (post || pre) {
       __syncthreads();
-      if (post && wp == 0) stats_join<kRows>(ex, 0, a.c, warps);
-      if (pre && wp == second) stats_join<kRows>(ex, 2, a.c, warps);
+      if (post)
+        join_first([&](int n, int of) { stats_join(rows, ex, 0, inv_c, warps, n, of); });
+      if (pre)
+        join_second([&](int n, int of) { stats_join(rows, ex, 2, inv_c, warps, n, of); });
       __syncthreads();
-      if (post) m1 = total4(ex, 0), r1 = total4(ex, 1);
-      if (pre) m2 = total4(ex, 2), r2 = total4(ex, 3);
+      if (post) nm1 = total4(ex, 0), r1 = total4(ex, 1);
+      if (pre) nm2 = total4(ex, 2), r2 = total4(ex, 3);
     }
+    if (kRows && post) FOR_ROWS(j) f[j % kHeld] = (f[j % kHeld] + nm1) * r1;
+    if (kRows && pre) FOR_ROWS(j) y[j % kHeld] = (y[j % kHeld] + nm2) * r2;
+    auto fn_of = [&](int j) { return kRows || !post ? f_of(j) : (f_of(j) + nm1) * r1; };
+    auto yn_of = [&](int j) { return kRows ? y[j % kHeld] : (y_of(j) + nm2) * r2; };
     if (pre) {
       F4 s0 = all(0.f), s1 = all(0.f);
       FOR_ROWS(j) if (rows.on(j)) {
-        const F4 t = dz_of(j) * all(__ldg(a.prm.pre_weight + rows.param(j)));
+        const F4 t = dz_of(j) * prm.get(a.prm, kPreW, rows.param(j));
         s0 = s0 + t;
-        s1 = fma4(t, (y_of(j) - m2) * r2, s1);
+        s1 = fma4(t, yn_of(j), s1);
       }
-      sum_part(s0, ex, 0);
-      sum_part(s1, ex, 1);
+      rows_to_part(s0, ex.part[0][wp]);
+      rows_to_part(s1, ex.part[1][wp]);
       __syncthreads();
-      if (wp == 0) sum_join(ex, 0, warps);
-      if (wp == second) sum_join(ex, 1, warps);
+      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
       __syncthreads();
-      am = total4(ex, 0) * all(inv_c);
-      ay = total4(ex, 1) * all(inv_c);
+      am = total4(ex, 0);  // negated means
+      ay = total4(ex, 1);
     }
-    // everything of a row but d_f's projection
-    struct Row {
-      F4 d, du, fn, u, sg, os, sc, yn, dz;
+    // of a row: D, D q, and b = D q w1
+    auto d_of = [&](int j) {
+      const F4 d = kRows ? dy[j % kHeld] : grad(a.dy, j);
+      if (!pre) return d;
+      const F4 t = dz_of(j) * prm.get(a.prm, kPreW, rows.param(j));
+      return fma4(fma4(yn_of(j), ay, t + am), r2, d);
     };
-    auto row_of = [&](int j) {
-      const int ch = rows.param(j);
-      Row k;
-      k.d = kRows ? dy[j % kHeld] : grad(a.dy, j);
-      k.yn = k.dz = all(0.f);
-      if (pre) {
-        k.dz = dz_of(j);
-        k.yn = (y_of(j) - m2) * r2;
-        const F4 t = k.dz * all(__ldg(a.prm.pre_weight + ch));
-        k.d = fma4(fma4(-k.yn, ay, t - am), r2, k.d);
-      }
-      k.fn = k.u = all(0.f);
-      if (need_f) {
-        k.u = f_of(j);
-        k.fn = (k.u - m1) * r1;
-        if (post)
-          k.u = fma4(k.fn, all(__ldg(a.prm.post_weight + ch)), all(__ldg(a.prm.post_bias + ch)));
-      }
-      k.sg = sg1;
-      k.os = os1;
-      if (per_row) sigmoid4(gate_of(j), &k.sg, &k.os);
-      k.sc = all(a.prm.scale ? __ldg(a.prm.scale + ch) : 1.f);
-      k.du = k.d * k.sc * k.sg;
-      return k;
+    auto gate_of = [&](int j, F4* s, F4* o) {
+      *s = sg1;
+      *o = os1;
+      if (per_row) sigmoid4((kRows ? q[j % kHeld] : kept(a.gate, a.tp.gate, j)).get(), s, o);
     };
     F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
     FOR_ROWS(j) {
-      const Row k = row_of(j);
       const int ch = rows.param(j);
-      const long long e = (base + ch) * a.p;
-      F4 b = k.du;
-      if (post) b = b * all(__ldg(a.prm.post_weight + ch));
-      if (rows.on(j)) {
-        store4<kVec>(a.dx + e, at, a.p, k.d);
-        if (!post && a.df) store4<kVec>(a.df + e, at, a.p, k.du);
-        if (per_row) store4<kVec>(a.dgate + e, at, a.p, k.du * k.u * k.os);
+      const bool on = rows.on(j);
+      const F4 d = d_of(j), fn = need_f ? fn_of(j) : all(0.f);
+      F4 sg, os;
+      gate_of(j, &sg, &os);
+      const F4 u = fma4(fn, prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch));
+      const F4 ds = d * prm.get(a.prm, kScale, ch), du = ds * sg, b = du * prm.get(a.prm, kPostW, ch);
+      if (on) {
+        store4<kVec>(a.dx + e0(j), at, a.p, d);
+        if (!post && a.df) store4<kVec>(a.df + e0(j), at, a.p, du);
+        if (per_row) store4<kVec>(a.dgate + e0(j), at, a.p, du * os * u);
         t0 = t0 + b;
-        t1 = fma4(b, k.fn, t1);
-        t2 = fma4(k.d * k.sc, k.u, t2);
+        t1 = fma4(b, fn, t1);
+        t2 = fma4(ds, u, t2);
       }
-      const float v[5] = {sum4(k.d * k.sg * k.u), sum4(k.du * k.fn), sum4(k.du), sum4(k.dz * k.yn),
-                          sum4(k.dz)};
+      const F4 dzj = pre ? dz_of(j) : all(0.f);
+      const float v[5] = {sum4(d * sg * u), sum4(du * fn), sum4(du),
+                          pre ? sum4(dzj * yn_of(j)) : 0.f, sum4(dzj)};
 #pragma unroll
       for (int i = 0; i < 5; ++i) {
         if (kRows) {
@@ -176,38 +177,34 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
           float s = v[i];
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if ((lane & 7) == 0 && rows.on(j)) acc_c[i * a.c + ch] += s;
+          if ((lane & 7) == 0 && on) acc_c[i * a.c + ch] += s;
         }
       }
-      if (kRows) {
-        dy[j % kHeld] = b;  // from here on b
-      }
+      if (kRows) dy[j % kHeld] = b;
     }
-    if (post || a.gate_c == 1) {
-      if (post) sum_part(t0, ex, 0), sum_part(t1, ex, 1);
-      if (a.gate_c == 1) sum_part(t2, ex, 2);
-      __syncthreads();
-      if (post && wp == 0) sum_join(ex, 0, warps);
-      if (post && wp == second) sum_join(ex, 1, warps);
-      if (a.gate_c == 1 && wp == warps - 1) sum_join(ex, 2, warps);
-      __syncthreads();
-      if (a.gate_c == 1 && threadIdx.x < 8)
-        store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * sg1 * os1);
-      if (post) {
-        const F4 bm = total4(ex, 0) * all(inv_c), bf = total4(ex, 1) * all(inv_c);
-        FOR_ROWS(j) if (rows.on(j)) {
-          const int ch = rows.param(j);
-          F4 b = dy[j % kHeld], fn;
-          if (kRows) {
-            fn = (f_of(j) - m1) * r1;
-          } else {
-            const Row k = row_of(j);
-            fn = k.fn;
-            b = k.du * all(__ldg(a.prm.post_weight + ch));
-          }
-          store4<kVec>(a.df + (base + ch) * a.p, at, a.p, fma4(-fn, bf, b - bm) * r1);
-        }
+    if (!post && a.gate_c != 1) continue;
+    if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
+    if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
+    __syncthreads();
+    if (post) {
+      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+    }
+    if (a.gate_c == 1) sum_join(ex, 2, 1.f, warps, wp, warps);
+    __syncthreads();
+    if (a.gate_c == 1 && threadIdx.x < 8)
+      store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * sg1 * os1);
+    if (!post) continue;
+    const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
+    FOR_ROWS(j) if (rows.on(j)) {
+      F4 b = dy[j % kHeld];
+      if (!kRows) {
+        const int ch = rows.param(j);
+        F4 sg, os;
+        gate_of(j, &sg, &os);
+        b = d_of(j) * prm.get(a.prm, kScale, ch) * sg * prm.get(a.prm, kPostW, ch);
       }
+      store4<kVec>(a.df + e0(j), at, a.p, fma4(fn_of(j), bf, b + bm) * r1);
     }
   }
   float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
@@ -324,7 +321,7 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     for (int i = 0; i < 5; ++i)
       ZJAI_TRY(stage_bytes_out(ctx, host[i], (size_t)c * 4, 4, mem, "parameter gradient", &so.p[i]));
     const long long tiles = (long long)n * (long long)groups;
-    const Shape sh = shape_of(c);
+    const Shape sh = shape_of(c, true);
     const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
     float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
     if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");

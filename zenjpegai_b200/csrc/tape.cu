@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(256) tape_pack_kernel(const T* __restrict__ x,
     const long long row = on ? q / groups : 0;
     const int g = on ? (int)(q - row * groups) : 0, at = g * kTapeGroup + (threadIdx.x & 7) * 4;
     const F4 v = on ? load4<kVec>(x + row * p, at, p) : all(0.f);
-    tape_store4<kVec>(t, row, groups, g, at, p, v, on);
+    tape_store4<kVec>(t, row * p, q, at, p, v, on);
   }
 }
 

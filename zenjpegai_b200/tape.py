@@ -21,8 +21,8 @@ GROUP = 32  # positions that share an exponent
 STREAM_LEGACY = 1  # CUDA's handle of the legacy default stream, for `Engine.set_stream`
 
 _NUMPY_CODE = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
-_I8 = np.dtype(np.int8)
-_torch, _torch_code = None, {}
+_F32, _I8 = np.dtype(np.float32), np.dtype(np.int8)
+_torch, _torch_code, _current_stream = None, {}, None
 
 
 def _bad(msg):
@@ -31,13 +31,16 @@ def _bad(msg):
 
 def _is_torch(a):
     """Whether a is a torch tensor; torch is imported when the first one comes."""
-    global _torch, _torch_code
+    global _torch, _torch_code, _current_stream
     if _torch is None:
         if isinstance(a, np.ndarray) or not type(a).__module__.startswith("torch"):
             return False
         import torch
         _torch = torch
         _torch_code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        # the handle of torch's current stream; the raw form makes no Stream object (3 us a call)
+        _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
     return isinstance(a, _torch.Tensor)
 
 
@@ -60,16 +63,18 @@ class _Call:
     """The buffers of one call: the side they lie on (that of `like`), their checks, their pointers
     and new ones like them, and the stream order."""
 
-    __slots__ = ("engine", "cuda", "device")
+    __slots__ = ("engine", "cuda", "f32", "i8")
 
     def __init__(self, engine, like):
         self.engine = engine
         self.cuda = _is_torch(like)
         if self.cuda:
-            self.device = like.device
-            if not like.is_cuda or self.device.index != engine.device:
+            self.f32, self.i8 = _torch.float32, _torch.int8
+            if like.get_device() != engine.device:
                 raise _bad("torch tensors must be CUDA tensors of the engine's GPU")
-        elif not isinstance(like, np.ndarray):
+        elif isinstance(like, np.ndarray):
+            self.f32, self.i8 = _F32, _I8
+        else:
             raise _bad("arguments are numpy arrays or CUDA tensors")
 
     def code(self, a, what):
@@ -82,7 +87,7 @@ class _Call:
     def ptr(self, a, what, shape, dtype):
         """Pointer of an array that must have this shape and type and lie with the others."""
         if self.cuda:
-            if not isinstance(a, _torch.Tensor) or a.device != self.device:
+            if not isinstance(a, _torch.Tensor) or a.get_device() != self.engine.device:
                 raise _bad("%s must be a tensor of the same GPU" % what)
             contiguous = a.is_contiguous()
         else:
@@ -100,14 +105,6 @@ class _Call:
     def param(self, a, what, c):
         return self.ptr(a, what, (c,), self.f32)
 
-    @property
-    def f32(self):
-        return _torch.float32 if self.cuda else np.dtype(np.float32)
-
-    @property
-    def i8(self):
-        return _torch.int8 if self.cuda else _I8
-
     def tape(self, t, what, shape):
         """zjai_tape of a Tape of a map of this shape."""
         if not isinstance(t, Tape):
@@ -117,7 +114,7 @@ class _Call:
 
     def empty(self, shape, dtype):
         if self.cuda:
-            return _torch.empty(shape, dtype=dtype, device=self.device)
+            return _torch.empty(shape, dtype=dtype, device=self.engine.device)
         return np.empty(shape, dtype)
 
     def at(self, a):
@@ -134,7 +131,7 @@ class _Call:
             check(f(self.engine.handle, *args, _lib.MEM_HOST))
             return
         h = self.engine.handle
-        cur = _torch.cuda.current_stream(self.device).cuda_stream or STREAM_LEGACY
+        cur = _current_stream(self.engine.device) or STREAM_LEGACY
         if cur == self.engine.stream:
             check(f(h, *args, _lib.MEM_DEVICE))
             return
