@@ -70,15 +70,18 @@ __device__ __forceinline__ F4 load4(const T* row, int at, int p) {
     return {make_float2(v[0], v[1]), make_float2(v[2], v[3])};
   }
 }
+// four positions at q, aligned
+template <class T>
+__device__ __forceinline__ void store4_in(T* q, F4 v) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(q) = flat(v);
+  else
+    *reinterpret_cast<uint2*>(q) = words2<T>(v);
+}
 template <bool kVec, class T>
 __device__ __forceinline__ void store4(T* row, int at, int p, F4 v) {
   if constexpr (kVec) {
-    if (at >= p) return;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(row + at) = flat(v);
-    } else {
-      *reinterpret_cast<uint2*>(row + at) = words2<T>(v);
-    }
+    if (at < p) store4_in(row + at, v);
   } else {
     const float f[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
 #pragma unroll
@@ -111,6 +114,11 @@ __device__ __forceinline__ F4 taped4(uint32_t codes, int e) {
 
 __device__ __forceinline__ float sum4(F4 v) {
   const float2 t = __fadd2_rn(v.a, v.b);
+  return t.x + t.y;
+}
+
+__device__ __forceinline__ float dot4(F4 x, F4 y) {
+  const float2 t = __ffma2_rn(x.a, y.a, __fmul2_rn(x.b, y.b));
   return t.x + t.y;
 }
 
@@ -155,6 +163,16 @@ __device__ __forceinline__ void tape_store4(const zjai_tape& t, long long e0, lo
       if (at + i < p) codes[at + i] = (int8_t)(w >> (8 * i) & 0xffu);
   }
   if ((threadIdx.x & 7) == 0) t.exps[ge] = (int8_t)tape_exp(m);
+}
+// The same where the lane's four codes are at `codes`, aligned, and the group's exponent at `exp`;
+// in: the positions are in the row.
+__device__ __forceinline__ void tape_hold4(int8_t* codes, int8_t* exp, F4 v, bool on, bool in) {
+  uint32_t m = amax4(v);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const uint32_t w = codes4(v, m);
+  if (on && in) *reinterpret_cast<uint32_t*>(codes) = w;
+  if (on && (threadIdx.x & 7) == 0) *exp = (int8_t)tape_exp(m);
 }
 // value of positions behind the row's end set to zero
 template <bool kVec>

@@ -15,6 +15,104 @@ struct FwdArgs {
   zjai_residual_tapes tp;
 };
 
+// Rows held, vector accesses, the next tile copied ahead into the other of two slots.
+template <class T>
+constexpr int fwd_slot_bytes() {  // per thread: f, x and the gate's logits
+  return 3 * kStagedRows * 4 * (int)sizeof(T);
+}
+template <class T>
+__global__ void __launch_bounds__(kThreadsMost, 1)
+    residual_norm_staged_kernel(const FwdArgs<T> a) {
+  constexpr int kRows = kStagedRows, kBytes = 4 * sizeof(T);
+  __shared__ Exchange<2> ex;
+  __shared__ Params<kRows> prm;
+  extern __shared__ __align__(16) char slots[];
+  const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Rows<kRows> rows(a.c, warps);
+  const int groups = (int)tape_groups(a.p);
+  const float inv_c = 1.f / (float)a.c;
+  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
+  StagedRow row[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) row[j] = staged_row(j, a.c, a.p, groups);
+  auto place = [&](int slot, int k, int j) {
+    return slots + ((slot * 3 + k) * kRows + j) * (int)blockDim.x * kBytes + threadIdx.x * kBytes;
+  };
+  auto copy = [&](const Tiles& t, int slot) {
+    const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
+    const bool in = t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const bool on = in && row[j].on;
+      stage_copy<kBytes>(place(slot, 0, j), a.f + e + row[j].e, on);
+      stage_copy<kBytes>(place(slot, 1, j), a.x + e + row[j].e, on);
+      if (per_row) stage_copy<kBytes>(place(slot, 2, j), a.gate + e + row[j].e, on);
+    }
+  };
+  prm.load(a.prm, a.c);
+  __syncthreads();
+  Tiles tile(a.tiles, groups), ahead = tile;
+  if (ahead.on()) copy(ahead, 0);
+  stage_commit();
+  for (int slot = 0; tile.on(); tile.next(), slot ^= 1) {
+    ahead.next();
+    if (ahead.on()) copy(ahead, slot ^ 1);
+    stage_commit();
+    const int at = tile.g * kTapeGroup + (lane & 7) * 4;
+    const bool in = at < a.p;
+    const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
+    const long long x0 = (long long)tile.img * a.c * groups + tile.g;
+    F4 gate1 = all(0.f), sg1 = all(1.f), unused;
+    if (a.gate_c == 1) {
+      gate1 = load4<true>(a.gate + (long long)tile.img * a.p, at, a.p);
+      sigmoid4(gate1, &sg1, &unused);
+    }
+    stage_wait<1>();
+    auto hold = [&](const zjai_tape& t, int j, F4 v) {
+      tape_hold4(t.codes + e0 + row[j].e, t.exps + x0 + row[j].x, v, row[j].on, in);
+    };
+    F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
+    auto exchange = [&](auto v) {
+      stats_part(rows, v, ex, 0, warps);
+      __syncthreads();
+      stats_join(rows, ex, 0, inv_c, warps, wp, warps);
+      __syncthreads();
+      nm = total4(ex, 0);
+      r = total4(ex, 1);
+    };
+    if (post) exchange([&](int j) { return staged4<T>(place(slot, 0, j)); });
+    if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
+      tape_store4<true>(a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g,
+                        at, a.p, gate1, lane < 8);
+    F4 y[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const F4 f = staged4<T>(place(slot, 0, j));
+      F4 u = f, s = sg1;
+      if (post)
+        u = fma4((f + nm) * r, prm.get(a.prm, kPostW, row[j].ch), prm.get(a.prm, kPostB, row[j].ch));
+      if (a.tp.f.codes) hold(a.tp.f, j, f);
+      if (per_row) {
+        const F4 g = staged4<T>(place(slot, 2, j));
+        sigmoid4(g, &s, &unused);
+        if (a.tp.gate.codes) hold(a.tp.gate, j, g);
+      }
+      y[j] = fma4(s * prm.get(a.prm, kScale, row[j].ch), u, staged4<T>(place(slot, 1, j)));
+      if (in && row[j].on) store4_in(a.y + e0 + row[j].e, y[j]);
+      if (a.tp.y.codes) hold(a.tp.y, j, clip4<true>(y[j], at, a.p));
+    }
+    if (!pre) continue;
+    exchange([&](int j) { return y[j]; });
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const F4 z =
+          fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row[j].ch), prm.get(a.prm, kPreB, row[j].ch));
+      if (in && row[j].on) store4_in(a.z + e0 + row[j].e, z);
+      if (a.tp.z.codes) hold(a.tp.z, j, clip4<true>(z, at, a.p));
+    }
+  }
+}
+
 template <int kRows, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const FwdArgs<T> a) {
   __shared__ Exchange<2> ex;
@@ -152,21 +250,28 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->codes, tr[i] * p, 1, mem, "codes", &tt[i]->codes));
       ZJAI_TRY(stage_bytes_out(ctx, wt[i]->exps, tr[i] * groups, 1, mem, "exps", &tt[i]->exps));
     }
-    const Shape sh = shape_of(c, false);
     VecCheck vec(p);
     vec.map(dx, es).map(df, es).map(dg, es).map(dyo, es).map(dzo, es);
     for (zjai_tape* t : tt) vec.map(t->codes, 1);
+    const Shape sh = shape_of(c, p, vec.ok, false);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      return by_rows(sh.rows, [&](auto r) -> int {
-        constexpr int kRows = decltype(r)::value;
-        FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
-                        (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
-        const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
-        auto k = vec.ok ? residual_norm_kernel<kRows, true, T> : residual_norm_kernel<kRows, false, T>;
-        k<<<blocks, sh.warps * 32, 0, ctx->stream>>>(a);
+      FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
+                      (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
+      const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
+      if (sh.staged) {
+        auto k = residual_norm_staged_kernel<T>;
+        const int smem = 2 * fwd_slot_bytes<T>() * sh.warps * 32;
+        ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                            "gated_residual_norm"));
+        k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
         return cuda_check(cudaGetLastError(), "gated_residual_norm");
-      });
+      }
+      auto k = sh.rows ? residual_norm_kernel<kStagedRows, false, T>
+               : vec.ok ? residual_norm_kernel<0, true, T> : residual_norm_kernel<0, false, T>;
+      k<<<blocks, sh.warps * 32, 0, ctx->stream>>>(a);
+      return cuda_check(cudaGetLastError(), "gated_residual_norm");
     }));
     ctx->launches++;
     ZJAI_TRY(finish_bytes_out(ctx, y, dyo, bytes, mem));

@@ -34,17 +34,19 @@ constexpr float kEps = 1e-5f;
 constexpr int kMaxC = 8192;  // the parameter sums of a block sit in shared memory, 20 B a channel
 constexpr int kMaxWarps = 16;
 
-// sigmoid(g) and 1 - sigmoid(g), neither by cancellation and both finite for every g but NaN
-__device__ __forceinline__ void sigmoid2(float g, float* s, float* one_minus) {
+// sigmoid(g) and sigmoid(g) (1 - sigmoid(g)), an even function of g: with a = exp(-|g|) and
+// r = 1 / (1 + a), sigmoid is r or a r and the product a r^2, nothing by cancellation and both finite
+// for every g but NaN.
+__device__ __forceinline__ void sigmoid2(float g, float* s, float* slope) {
   const float a = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + a), ar = a * r;
   *s = g >= 0.f ? r : ar;
-  *one_minus = g >= 0.f ? ar : r;
+  *slope = ar * r;
 }
-__device__ __forceinline__ void sigmoid4(F4 g, F4* s, F4* one_minus) {
-  sigmoid2(g.a.x, &s->a.x, &one_minus->a.x);
-  sigmoid2(g.a.y, &s->a.y, &one_minus->a.y);
-  sigmoid2(g.b.x, &s->b.x, &one_minus->b.x);
-  sigmoid2(g.b.y, &s->b.y, &one_minus->b.y);
+__device__ __forceinline__ void sigmoid4(F4 g, F4* s, F4* slope) {
+  sigmoid2(g.a.x, &s->a.x, &slope->a.x);
+  sigmoid2(g.a.y, &s->a.y, &slope->a.y);
+  sigmoid2(g.b.x, &s->b.x, &slope->b.x);
+  sigmoid2(g.b.y, &s->b.y, &slope->b.y);
 }
 
 // Sum over the four rows of a warp (lanes with the same positions), to all of them.
@@ -207,6 +209,73 @@ struct Params {
 
 constexpr int kThreadsMost = 32 * kMaxWarps;
 
+// The tiles of a block, one after the other: picture and group of positions, without a division.
+struct Tiles {
+  int img, g, groups, step_img, step_g;
+  long long left;  // tiles from the current one on, of the whole grid
+  __device__ __forceinline__ Tiles(long long tiles, int groups_) : groups(groups_) {
+    img = (int)(blockIdx.x / (unsigned)groups);
+    g = (int)(blockIdx.x - (unsigned)img * groups);
+    step_img = (int)(gridDim.x / (unsigned)groups);
+    step_g = (int)(gridDim.x - (unsigned)step_img * groups);
+    left = tiles - blockIdx.x;
+  }
+  __device__ __forceinline__ bool on() const { return left > 0; }
+  __device__ __forceinline__ void next() {
+    left -= gridDim.x;
+    img += step_img;
+    g += step_g;
+    if (g >= groups) g -= groups, ++img;
+  }
+};
+
+// Staged loads (rows held, vector accesses): a thread copies what it will itself read of the next
+// tile to its own places in shared memory (cp.async, no thread waits for another) while it works on
+// the current one. A place is four positions of a row, of kBytes.
+template <int kBytes>
+__device__ __forceinline__ void stage_copy(char* dst, const void* src, bool on) {
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(kBytes),
+                 "r"(on ? kBytes : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void stage_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kNewer>
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kNewer) : "memory");
+}
+template <class T>
+__device__ __forceinline__ F4 staged4(const char* src) {
+  if constexpr (sizeof(T) == 4)
+    return make4(*reinterpret_cast<const float4*>(src));
+  else
+    return halves4<T>(*reinterpret_cast<const uint2*>(src));
+}
+// A row of the calling thread in a picture: its offset from the picture's first element, with the
+// lane's four positions, and its exponents' from the picture's first (held rows: 32 bits do)
+constexpr int kStagedRows = 4;
+struct StagedRow {
+  uint32_t e, x;
+  int ch;
+  bool on;
+};
+__device__ __forceinline__ StagedRow staged_row(int j, int c, int p, int groups) {
+  const int lane = threadIdx.x & 31;
+  const int row = (threadIdx.x >> 5) * 4 * kStagedRows + j * 4 + (lane >> 3);
+  StagedRow r;
+  r.on = row < c;
+  r.ch = min(row, c - 1);
+  r.e = (uint32_t)r.ch * (uint32_t)p + (lane & 7) * 4;
+  r.x = (uint32_t)r.ch * (uint32_t)groups;
+  return r;
+}
+
 int stage_param(Ctx* ctx, const float* p, int c, int mem, const char* what, const float** out) {
   return stage_bytes_in(ctx, p, (size_t)c * sizeof(float), sizeof(float), mem, what, out);
 }
@@ -220,23 +289,21 @@ int stage_params(Ctx* ctx, const zjai_residual_params& in, int c, int mem,
   return stage_param(ctx, in.pre_bias, c, mem, "pre_bias", &out->pre_bias);
 }
 
-// Rows a thread holds for c channels (0: not held) and the block's warps. Sixteen warps an SM are
-// resident at the registers that __launch_bounds__ leaves, so blocks of few warps come in numbers.
+// How c channels at p positions are taken. staged: rows held and copied ahead, where vector accesses
+// are possible; else kRows rows of a thread held in registers, or (0) read again. Sixteen warps an
+// SM are resident at the registers that __launch_bounds__ leaves, so blocks of few warps come in
+// numbers.
 struct Shape {
+  bool staged;
   int rows, warps, per_sm;
 };
-Shape shape_of(int c, bool backward) {
-  // the backward pass holds twice as much a row: two rows a thread where the warps allow it
-  const int rows = c > kHeldC ? 0 : backward && c <= kHeldC / 2 ? 2 : 4;
+Shape shape_of(int c, int p, bool vec, bool backward) {
+  // held rows are addressed by 32-bit offsets from their picture
+  const bool held = c <= kHeldC && (long long)c * p < (1LL << 32) - 64;
+  // without vector accesses the backward pass takes two rows a thread where the warps allow it
+  const int rows = !held ? 0 : !vec && backward && c <= kHeldC / 2 ? 2 : kStagedRows;
   const int warps = rows ? (c + 4 * rows - 1) / (4 * rows) : kMaxWarps;
-  return {rows, warps, kMaxWarps / warps};
-}
-// f(std::integral_constant) with the rows held
-template <class F>
-int by_rows(int rows, F&& f) {
-  if (rows == 2) return f(std::integral_constant<int, 2>());
-  if (rows == 4) return f(std::integral_constant<int, 4>());
-  return f(std::integral_constant<int, 0>());
+  return {held && vec, rows, warps, kMaxWarps / warps};
 }
 // Four neighbouring positions can be loaded and stored at once: rows of a multiple of four
 // positions, maps aligned to four elements and codes to four bytes.

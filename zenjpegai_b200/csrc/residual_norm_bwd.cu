@@ -38,8 +38,238 @@ struct Kept<true, kVec, T> {
   __device__ __forceinline__ F4 get() const { return taped4(w, e); }
 };
 
-// The parameter gradients are summed over a block's tiles (in registers, or per channel in shared
-// memory where rows are not held) and written out per block.
+// Rows held, vector accesses, the next tile copied ahead. Per thread a slot has dy, dz, and f, y and
+// the gate as they were kept. Two slots where 16 warps' fit the SM's shared memory; with one (f32
+// maps) the next tile is copied as soon as the current one has been read, before its last exchange.
+// The parameter gradients are summed over a block's tiles in registers, written out per block.
+template <bool kTaped, class T>
+struct BwdSlot {
+  static constexpr int kGrad = 4 * sizeof(T), kKept = kTaped ? 4 : 4 * sizeof(T);
+  static constexpr int kBytes = kStagedRows * (2 * kGrad + 3 * kKept);  // per thread
+  static constexpr int kSlots = 2 * kBytes * kThreadsMost <= 200 * 1024 ? 2 : 1;
+};
+template <bool kTaped, class T>
+__global__ void __launch_bounds__(kThreadsMost, 1)
+    residual_norm_bwd_staged_kernel(const BwdArgs<T> a) {
+  using S = BwdSlot<kTaped, T>;
+  constexpr int kRows = kStagedRows;
+  __shared__ Exchange<4> ex;
+  __shared__ Params<kRows> prm;
+  extern __shared__ __align__(16) char slots[];
+  const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Rows<kRows> rows(a.c, warps);
+  const int groups = (int)tape_groups(a.p);
+  const float inv_c = 1.f / (float)a.c;
+  const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
+  const bool need_f = post || a.gate_c || a.prm.scale;
+  // two sums at a time are joined by four warps each where there are eight
+  const bool two = warps >= 8;
+  auto join_first = [&](auto f) {
+    if (!two || wp < 4) f(wp, two ? 4 : warps);
+  };
+  auto join_second = [&](auto f) {
+    if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
+  };
+  StagedRow row[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) row[j] = staged_row(j, a.c, a.p, groups);
+  auto grad_at = [&](int slot, int k, int j) {
+    return slots + slot * S::kBytes * (int)blockDim.x +
+           ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kGrad;
+  };
+  auto kept_at = [&](int slot, int k, int j) {
+    return slots + slot * S::kBytes * (int)blockDim.x + 2 * kRows * (int)blockDim.x * S::kGrad +
+           ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kKept;
+  };
+  int exps[3][kRows];  // of the tile copied last
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) exps[0][j] = exps[1][j] = exps[2][j] = 0;
+  auto copy = [&](const Tiles& t, int slot) {
+    const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
+    const long long x = (long long)t.img * a.c * groups + t.g;
+    const bool in = t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    auto keep = [&](const T* map, const zjai_tape& tp, int k, int j, bool on) {
+      if constexpr (kTaped) {
+        stage_copy<4>(kept_at(slot, k, j), tp.codes + e + row[j].e, on);
+        if (row[j].on) exps[k][j] = __ldg(tp.exps + x + row[j].x);
+      } else {
+        stage_copy<S::kKept>(kept_at(slot, k, j), map + e + row[j].e, on);
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const bool on = in && row[j].on;
+      if (need_f) keep(a.f, a.tp.f, 0, j, on);
+      if (pre) keep(a.y, a.tp.y, 1, j, on);
+      if (pre) stage_copy<S::kGrad>(grad_at(slot, 1, j), a.dz + e + row[j].e, on);
+      if (per_row) keep(a.gate, a.tp.gate, 2, j, on);
+      stage_copy<S::kGrad>(grad_at(slot, 0, j), a.dy + e + row[j].e, on);
+    }
+  };
+  auto kept = [&](int slot, int k, int j, int e) {
+    if constexpr (kTaped)
+      return taped4(*reinterpret_cast<const uint32_t*>(kept_at(slot, k, j)), e);
+    else
+      return staged4<T>(kept_at(slot, k, j));
+  };
+  float acc[kRows][5];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
+  prm.load(a.prm, a.c);
+  __syncthreads();
+  Tiles tile(a.tiles, groups), ahead = tile;
+  if (ahead.on()) copy(ahead, 0);
+  stage_commit();
+  for (int slot = 0; tile.on(); tile.next(), slot ^= S::kSlots - 1) {
+    const int at = tile.g * kTapeGroup + (lane & 7) * 4;
+    const bool in = at < a.p;
+    const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
+    int ge[kRows], fe[kRows], ye[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) fe[j] = exps[0][j], ye[j] = exps[1][j], ge[j] = exps[2][j];
+    F4 sg1 = all(1.f), slope1 = all(0.f);
+    if (a.gate_c == 1) {
+      Kept<kTaped, true, T> k;
+      k.load(a.gate, a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g, at,
+             a.p);
+      sigmoid4(k.get(), &sg1, &slope1);
+    }
+    ahead.next();
+    if (S::kSlots == 2) {
+      if (ahead.on()) copy(ahead, slot ^ 1);
+      stage_commit();
+    }
+    stage_wait<S::kSlots - 1>();
+    F4 f[kRows], y[kRows];  // then LN(f), LN(y)
+    if (need_f)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) f[j] = kept(slot, 0, j, fe[j]);
+    if (pre)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) y[j] = kept(slot, 1, j, ye[j]);
+    if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0, warps);
+    if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2, warps);
+    if (post || pre) {
+      __syncthreads();
+      if (post) join_first([&](int n, int of) { stats_join(rows, ex, 0, inv_c, warps, n, of); });
+      if (pre) join_second([&](int n, int of) { stats_join(rows, ex, 2, inv_c, warps, n, of); });
+      __syncthreads();
+    }
+    F4 r1 = all(1.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
+    if (post) {
+      const F4 nm = total4(ex, 0);
+      r1 = total4(ex, 1);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) f[j] = (f[j] + nm) * r1;
+    }
+    if (pre) {
+      const F4 nm = total4(ex, 2);
+      r2 = total4(ex, 3);
+      F4 s0 = all(0.f), s1 = all(0.f);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        y[j] = (y[j] + nm) * r2;
+        const F4 t = staged4<T>(grad_at(slot, 1, j)) * prm.get(a.prm, kPreW, row[j].ch);
+        if (row[j].on) {
+          s0 = s0 + t;
+          s1 = fma4(t, y[j], s1);
+        }
+      }
+      rows_to_part(s0, ex.part[0][wp]);
+      rows_to_part(s1, ex.part[1][wp]);
+      __syncthreads();
+      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+      __syncthreads();
+      am = total4(ex, 0);  // negated means
+      ay = total4(ex, 1);
+    }
+    F4 b[kRows], t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const int ch = row[j].ch;
+      const bool on = row[j].on, write = on && in;
+      F4 d = staged4<T>(grad_at(slot, 0, j));
+      if (pre) {
+        const F4 dz = staged4<T>(grad_at(slot, 1, j));
+        acc[j][3] += dot4(dz, y[j]);
+        acc[j][4] += sum4(dz);
+        d = fma4(fma4(y[j], ay, dz * prm.get(a.prm, kPreW, ch) + am), r2, d);
+      }
+      if (write) store4_in(a.dx + e0 + row[j].e, d);
+      if (!need_f) continue;
+      const F4 u = post ? fma4(f[j], prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch)) : f[j];
+      const F4 ds = d * prm.get(a.prm, kScale, ch);
+      F4 sg = sg1, du = ds;
+      if (per_row) {
+        F4 slope;
+        sigmoid4(kept(slot, 2, j, ge[j]), &sg, &slope);
+        if (write) store4_in(a.dgate + e0 + row[j].e, ds * u * slope);
+      }
+      if (a.gate_c) du = ds * sg;
+      acc[j][0] += dot4(d * sg, u);
+      if (a.gate_c == 1 && on) t2 = fma4(ds, u, t2);
+      if (post) {
+        acc[j][1] += dot4(du, f[j]);
+        acc[j][2] += sum4(du);
+        b[j] = du * prm.get(a.prm, kPostW, ch);
+        if (on) {
+          t0 = t0 + b[j];
+          t1 = fma4(b[j], f[j], t1);
+        }
+      } else if (write) {
+        store4_in(a.df + e0 + row[j].e, du);
+      }
+    }
+    if (!need_f && a.df)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (row[j].on && in) {
+          F4 d = staged4<T>(grad_at(slot, 0, j));
+          if (pre)
+            d = fma4(fma4(y[j], ay, staged4<T>(grad_at(slot, 1, j)) *
+                                        prm.get(a.prm, kPreW, row[j].ch) + am), r2, d);
+          store4_in(a.df + e0 + row[j].e, d);
+        }
+    if (S::kSlots == 1) {  // the slot has been read
+      if (ahead.on()) copy(ahead, 0);
+      stage_commit();
+    }
+    if (!post && a.gate_c != 1) continue;
+    if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
+    if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
+    __syncthreads();
+    if (post) {
+      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+    }
+    if (a.gate_c == 1) sum_join(ex, 2, 1.f, warps, wp, warps);
+    __syncthreads();
+    if (a.gate_c == 1 && threadIdx.x < 8)
+      store4<true>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 2) * slope1);
+    if (!post) continue;
+    const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      if (row[j].on && in) store4_in(a.df + e0 + row[j].e, fma4(f[j], bf, b[j] + bm) * r1);
+  }
+  stage_wait<0>();
+  float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
+#pragma unroll
+  for (int j = 0; j < kRows; ++j)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      float s = acc[j][i];
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if ((lane & 7) == 0 && row[j].on) out[i * a.c + row[j].ch] = s;
+    }
+}
+
+// Rows of any alignment, held in registers, or (kRows 0) of any number, read again for each pass:
+// the parameter sums in registers, or per channel in shared memory.
 template <int kRows, bool kTaped, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(const BwdArgs<T> a) {
   __shared__ Exchange<4> ex;
@@ -98,11 +328,11 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     auto f_of = [&](int j) { return kRows ? f[j % kHeld] : kept(a.f, a.tp.f, j).get(); };
     auto y_of = [&](int j) { return kRows ? y[j % kHeld] : kept(a.y, a.tp.y, j).get(); };
     auto dz_of = [&](int j) { return kRows ? dz[j % kHeld] : grad(a.dz, j); };
-    F4 sg1 = all(1.f), os1 = all(0.f);
+    F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
       K k;
       k.load(a.gate, a.tp.gate, img * a.p, img * groups + g, at, a.p);
-      sigmoid4(k.get(), &sg1, &os1);
+      sigmoid4(k.get(), &sg1, &slope1);
     }
     F4 nm1 = all(0.f), r1 = all(1.f), nm2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
     if (post) stats_part(rows, f_of, ex, 0, warps);
@@ -146,7 +376,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     };
     auto gate_of = [&](int j, F4* s, F4* o) {
       *s = sg1;
-      *o = os1;
+      *o = slope1;
       if (per_row) sigmoid4((kRows ? q[j % kHeld] : kept(a.gate, a.tp.gate, j)).get(), s, o);
     };
     F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
@@ -154,14 +384,14 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
       const int ch = rows.param(j);
       const bool on = rows.on(j);
       const F4 d = d_of(j), fn = need_f ? fn_of(j) : all(0.f);
-      F4 sg, os;
-      gate_of(j, &sg, &os);
+      F4 sg, slope;
+      gate_of(j, &sg, &slope);
       const F4 u = fma4(fn, prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch));
       const F4 ds = d * prm.get(a.prm, kScale, ch), du = ds * sg, b = du * prm.get(a.prm, kPostW, ch);
       if (on) {
         store4<kVec>(a.dx + e0(j), at, a.p, d);
         if (!post && a.df) store4<kVec>(a.df + e0(j), at, a.p, du);
-        if (per_row) store4<kVec>(a.dgate + e0(j), at, a.p, du * os * u);
+        if (per_row) store4<kVec>(a.dgate + e0(j), at, a.p, ds * u * slope);
         t0 = t0 + b;
         t1 = fma4(b, fn, t1);
         t2 = fma4(ds, u, t2);
@@ -193,15 +423,15 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     if (a.gate_c == 1) sum_join(ex, 2, 1.f, warps, wp, warps);
     __syncthreads();
     if (a.gate_c == 1 && threadIdx.x < 8)
-      store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * sg1 * os1);
+      store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * slope1);
     if (!post) continue;
     const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
     FOR_ROWS(j) if (rows.on(j)) {
       F4 b = dy[j % kHeld];
       if (!kRows) {
         const int ch = rows.param(j);
-        F4 sg, os;
-        gate_of(j, &sg, &os);
+        F4 sg, slope;
+        gate_of(j, &sg, &slope);
         b = d_of(j) * prm.get(a.prm, kScale, ch) * sg * prm.get(a.prm, kPostW, ch);
       }
       store4<kVec>(a.df + e0(j), at, a.p, fma4(fn_of(j), bf, b + bm) * r1);
@@ -321,33 +551,42 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     for (int i = 0; i < 5; ++i)
       ZJAI_TRY(stage_bytes_out(ctx, host[i], (size_t)c * 4, 4, mem, "parameter gradient", &so.p[i]));
     const long long tiles = (long long)n * (long long)groups;
-    const Shape sh = shape_of(c, true);
-    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
-    float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
-    if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
     VecCheck vec(p);
     vec.map(ddy, es).map(ddz, es).map(df, es).map(dg, es).map(dyy, es);
     vec.map(gx, es).map(gf, es).map(gg, es);
     vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
-    ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
+    const Shape sh = shape_of(c, p, vec.ok, true);
+    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
+    float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
+    if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
+    auto launch = [&](auto t, auto tp) -> int {
       using T = decltype(t);
-      return by_rows(sh.rows, [&](auto r) -> int {
-        constexpr int kRows = decltype(r)::value;
-        BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
-                        gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
-        auto k = taped ? (vec.ok ? residual_norm_bwd_kernel<kRows, true, true, T>
-                                 : residual_norm_bwd_kernel<kRows, true, false, T>)
-                       : (vec.ok ? residual_norm_bwd_kernel<kRows, false, true, T>
-                                 : residual_norm_bwd_kernel<kRows, false, false, T>);
-        const size_t smem = kRows ? 0 : (size_t)5 * c * sizeof(float);
-        if (!kRows)
-          ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   5 * kMaxC * (int)sizeof(float)),
-                              "gated_residual_norm_backward"));
-        k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
-        return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
-      });
+      constexpr bool kTaped = decltype(tp)::value;
+      using S = BwdSlot<kTaped, T>;
+      BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
+                      gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
+      void (*k)(BwdArgs<T>) = nullptr;
+      int smem = 0;
+      if (sh.staged) {
+        k = residual_norm_bwd_staged_kernel<kTaped, T>;
+        smem = S::kSlots * S::kBytes * sh.warps * 32;
+      } else if (sh.rows) {
+        k = sh.rows == 2 ? residual_norm_bwd_kernel<2, kTaped, false, T>
+                         : residual_norm_bwd_kernel<4, kTaped, false, T>;
+      } else {
+        k = vec.ok ? residual_norm_bwd_kernel<0, kTaped, true, T>
+                   : residual_norm_bwd_kernel<0, kTaped, false, T>;
+        smem = 5 * c * (int)sizeof(float);
+      }
+      if (smem)
+        ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                            "gated_residual_norm_backward"));
+      k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
+      return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
+    };
+    ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
+      return taped ? launch(t, std::true_type()) : launch(t, std::false_type());
     }));
     residual_sums_kernel<<<dim3((c + 31) / 32, 5), 256, 0, ctx->stream>>>(sums, blocks, c, so);
     ctx->launches += 2;
