@@ -128,20 +128,22 @@ __device__ __forceinline__ uint32_t amax4(F4 v) {
   return max(max(__float_as_uint(v.a.x) & k, __float_as_uint(v.a.y) & k),
              max(__float_as_uint(v.b.x) & k, __float_as_uint(v.b.y) & k));
 }
-// codes of four positions in a group whose largest magnitude is m
+// Codes of four positions in a group whose largest magnitude is m; whole warps call. Only the
+// largest 1 / 128 of magnitudes can round to 128, and a marked group has no codes: a warp that has
+// neither (one of 30 or so has) saves the clamps.
 __device__ __forceinline__ uint32_t codes4(F4 v, uint32_t m) {
-  // only the largest 1 / 128 of magnitudes can round to 128, and a marked group has no codes
-  if ((m & 0x7fffffu) < 0x7f0000u && m < 0x7f800000u) {
-    const F4 c = fma4(v, all(tape_inv_scale(tape_exp(m))), all(12582912.f));  // see tape_code_bits
-    return __byte_perm(__byte_perm(__float_as_uint(c.a.x), __float_as_uint(c.a.y), 0x0040),
-                       __byte_perm(__float_as_uint(c.b.x), __float_as_uint(c.b.y), 0x0040), 0x5410);
+  const int e = max((int)(m >> 23) - 133, -126);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  F4 c = fma4(v, all(inv), all(12582912.f));  // see tape_code_bits
+  if (__any_sync(0xffffffffu, (m & 0x7fffffu) >= 0x7f0000u || m >= 0x7f800000u)) {
+    const float none = m >= 0x7f800000u ? 0.f : inv;
+    const auto code = [&](float x) {
+      return m >= 0x7f800000u ? 0.f : __uint_as_float(tape_code_bits(x, none));
+    };
+    c = {make_float2(code(v.a.x), code(v.a.y)), make_float2(code(v.b.x), code(v.b.y))};
   }
-  if (m >= 0x7f800000u) return 0u;
-  const float inv = tape_inv_scale(tape_exp(m)), f[4] = {v.a.x, v.a.y, v.b.x, v.b.y};
-  uint32_t w = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= (tape_code_bits(f[i], inv) & 0xffu) << (8 * i);
-  return w;
+  return __byte_perm(__byte_perm(__float_as_uint(c.a.x), __float_as_uint(c.a.y), 0x0040),
+                     __byte_perm(__float_as_uint(c.b.x), __float_as_uint(c.b.y), 0x0040), 0x5410);
 }
 // Hold four positions of a row (zeros behind its end) as part of a tape's group; the row's eight
 // lanes call together, whole warps (`on`: the row exists). e0: the row's first element, ge: the
@@ -152,8 +154,8 @@ __device__ __forceinline__ void tape_store4(const zjai_tape& t, long long e0, lo
   uint32_t m = amax4(v);
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (!on) return;
   const uint32_t w = codes4(v, m);
+  if (!on) return;
   int8_t* codes = t.codes + e0;
   if constexpr (kVec) {
     if (at < p) *reinterpret_cast<uint32_t*>(codes + at) = w;

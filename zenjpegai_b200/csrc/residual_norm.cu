@@ -20,33 +20,31 @@ template <class T>
 constexpr int fwd_slot_bytes() {  // per thread: f, x and the gate's logits
   return 3 * kStagedRows * 4 * (int)sizeof(T);
 }
-template <class T>
+template <bool kWhole, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
     residual_norm_staged_kernel(const FwdArgs<T> a) {
   constexpr int kRows = kStagedRows, kBytes = 4 * sizeof(T);
-  __shared__ Exchange<2> ex;
+  __shared__ Exchange<2, 2> ex;
   __shared__ Params<kRows> prm;
   extern __shared__ __align__(16) char slots[];
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows> rows(a.c, warps);
+  const Rows<kRows, kWhole> rows(a.c, warps);
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
-  StagedRow row[kRows];
-#pragma unroll
-  for (int j = 0; j < kRows; ++j) row[j] = staged_row(j, a.c, a.p, groups);
+  const StagedRows<kWhole> row(a.c, a.p, groups);
   auto place = [&](int slot, int k, int j) {
     return slots + ((slot * 3 + k) * kRows + j) * (int)blockDim.x * kBytes + threadIdx.x * kBytes;
   };
   auto copy = [&](const Tiles& t, int slot) {
     const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
-    const bool in = t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    const bool in = kWhole || t.g * kTapeGroup + (lane & 7) * 4 < a.p;
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const bool on = in && row[j].on;
-      stage_copy<kBytes>(place(slot, 0, j), a.f + e + row[j].e, on);
-      stage_copy<kBytes>(place(slot, 1, j), a.x + e + row[j].e, on);
-      if (per_row) stage_copy<kBytes>(place(slot, 2, j), a.gate + e + row[j].e, on);
+      const bool on = in && row.on(j);
+      stage_copy<kBytes>(place(slot, 0, j), a.f + e + row.e(j), on);
+      stage_copy<kBytes>(place(slot, 1, j), a.x + e + row.e(j), on);
+      if (per_row) stage_copy<kBytes>(place(slot, 2, j), a.gate + e + row.e(j), on);
     }
   };
   prm.load(a.prm, a.c);
@@ -59,7 +57,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     if (ahead.on()) copy(ahead, slot ^ 1);
     stage_commit();
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
-    const bool in = at < a.p;
+    const bool in = kWhole || at < a.p;
     const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
     const long long x0 = (long long)tile.img * a.c * groups + tile.g;
     F4 gate1 = all(0.f), sg1 = all(1.f), unused;
@@ -69,7 +67,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     }
     stage_wait<1>();
     auto hold = [&](const zjai_tape& t, int j, F4 v) {
-      tape_hold4(t.codes + e0 + row[j].e, t.exps + x0 + row[j].x, v, row[j].on, in);
+      tape_hold4(t.codes + e0 + row.e(j), t.exps + x0 + row.x(j), v, row.on(j), in);
     };
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
@@ -90,32 +88,32 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       const F4 f = staged4<T>(place(slot, 0, j));
       F4 u = f, s = sg1;
       if (post)
-        u = fma4((f + nm) * r, prm.get(a.prm, kPostW, row[j].ch), prm.get(a.prm, kPostB, row[j].ch));
+        u = fma4((f + nm) * r, prm.get(a.prm, kPostW, row.ch(j)), prm.get(a.prm, kPostB, row.ch(j)));
       if (a.tp.f.codes) hold(a.tp.f, j, f);
       if (per_row) {
         const F4 g = staged4<T>(place(slot, 2, j));
         sigmoid4(g, &s, &unused);
         if (a.tp.gate.codes) hold(a.tp.gate, j, g);
       }
-      y[j] = fma4(s * prm.get(a.prm, kScale, row[j].ch), u, staged4<T>(place(slot, 1, j)));
-      if (in && row[j].on) store4_in(a.y + e0 + row[j].e, y[j]);
-      if (a.tp.y.codes) hold(a.tp.y, j, clip4<true>(y[j], at, a.p));
+      y[j] = fma4(s * prm.get(a.prm, kScale, row.ch(j)), u, staged4<T>(place(slot, 1, j)));
+      if (in && row.on(j)) store4_in(a.y + e0 + row.e(j), y[j]);
+      if (a.tp.y.codes) hold(a.tp.y, j, in ? y[j] : all(0.f));
     }
     if (!pre) continue;
     exchange([&](int j) { return y[j]; });
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       const F4 z =
-          fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row[j].ch), prm.get(a.prm, kPreB, row[j].ch));
-      if (in && row[j].on) store4_in(a.z + e0 + row[j].e, z);
-      if (a.tp.z.codes) hold(a.tp.z, j, clip4<true>(z, at, a.p));
+          fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row.ch(j)), prm.get(a.prm, kPreB, row.ch(j)));
+      if (in && row.on(j)) store4_in(a.z + e0 + row.e(j), z);
+      if (a.tp.z.codes) hold(a.tp.z, j, in ? z : all(0.f));
     }
   }
 }
 
 template <int kRows, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const FwdArgs<T> a) {
-  __shared__ Exchange<2> ex;
+  __shared__ Exchange<2, 2> ex;
   __shared__ Params<kRows> prm;
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Rows<kRows> rows(a.c, warps);
@@ -260,7 +258,8 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
                       (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
       const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
       if (sh.staged) {
-        auto k = residual_norm_staged_kernel<T>;
+        auto k = sh.whole ? residual_norm_staged_kernel<true, T>
+                          : residual_norm_staged_kernel<false, T>;
         const int smem = 2 * fwd_slot_bytes<T>() * sh.warps * 32;
         ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem),

@@ -73,14 +73,14 @@ __device__ __forceinline__ void rows_to_part(F4 v, float* part) {
 }
 
 // The block's partial sums per warp and position, and their totals.
-template <int kVals>
+template <int kVals, int kTotals>
 struct Exchange {
-  float part[kVals][kMaxWarps][32], total[kVals][32];
+  float part[kVals][kMaxWarps][32], total[kTotals][32];
 };
 
 // Rows of the calling thread: row(j) for j < rows(). kRows > 0: held in registers, consecutive
-// groups of four per warp; 0: any number, strided over the block.
-template <int kRows>
+// groups of four per warp; 0: any number, strided over the block. kAll: all rows exist.
+template <int kRows, bool kAll = false>
 struct Rows {
   int c, first, step, n;
   __device__ __forceinline__ Rows(int c_, int warps) : c(c_) {
@@ -90,11 +90,12 @@ struct Rows {
     n = kRows ? kRows : (c + step - 1) / step;
   }
   __device__ __forceinline__ int row(int j) const { return first + j * step; }
-  __device__ __forceinline__ bool on(int j) const { return row(j) < c; }
+  __device__ __forceinline__ bool on(int j) const { return kAll || row(j) < c; }
   // a row that exists, to read for one that does not
   __device__ __forceinline__ int param(int j) const { return min(row(j), c - 1); }
   // rows of a warp
   __device__ __forceinline__ int of_warp(int w, int warps) const {
+    if (kAll) return 4 * kRows;
     if (kRows) return max(0, min(c - w * 4 * kRows, 4 * kRows));
     const int whole = c / (4 * warps);
     return whole * 4 + max(0, min(4, c - whole * 4 * warps - w * 4));
@@ -104,9 +105,9 @@ struct Rows {
 
 // Per warp the sum and the squared deviations from the warp's own mean of v(j), to ex.part at val,
 // val + 1.
-template <int kRows, int kVals, class V>
-__device__ __forceinline__ void stats_part(const Rows<kRows>& rows, V&& v, Exchange<kVals>& ex,
-                                           int val, int warps) {
+template <int kRows, bool kAll, class V, class E>
+__device__ __forceinline__ void stats_part(const Rows<kRows, kAll>& rows, V&& v, E& ex, int val,
+                                           int warps) {
   const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   F4 s = all(0.f), q = all(0.f);
   FOR_ROWS(j) if (rows.on(j)) s = s + v(j);
@@ -133,8 +134,8 @@ __device__ __forceinline__ float over_subs(float v) {
 }
 // Joined: ex.total at val, val + 1 the negated mean and 1 / sigma. Partials' means are joined by
 // M2 = sum of M2_w + n_w (mean_w - mean)^2.
-template <int kRows, int kVals>
-__device__ __forceinline__ void stats_join(const Rows<kRows>& rows, Exchange<kVals>& ex, int val,
+template <int kRows, bool kAll, class E>
+__device__ __forceinline__ void stats_join(const Rows<kRows, kAll>& rows, E& ex, int val,
                                            float inv_c, int warps, int nth, int of) {
   by_position(nth, of, [&](int pos, int sub) {
     float s[kMaxWarps / 4], sum = 0.f, q = 0.f;
@@ -160,13 +161,13 @@ __device__ __forceinline__ void stats_join(const Rows<kRows>& rows, Exchange<kVa
     }
   });
 }
-template <int kVals>
-__device__ __forceinline__ F4 total4(const Exchange<kVals>& ex, int val) {
+template <class E>
+__device__ __forceinline__ F4 total4(const E& ex, int val) {
   return make4(*reinterpret_cast<const float4*>(&ex.total[val][(threadIdx.x & 7) * 4]));
 }
-// Sums over the warps of ex.part at val, times k.
-template <int kVals>
-__device__ __forceinline__ void sum_join(Exchange<kVals>& ex, int val, float k, int warps, int nth,
+// Sums over the warps of ex.part at val, times k, to ex.total at to.
+template <class E>
+__device__ __forceinline__ void sum_join(E& ex, int val, int to, float k, int warps, int nth,
                                          int of) {
   by_position(nth, of, [&](int pos, int sub) {
     float s = 0.f;
@@ -174,7 +175,7 @@ __device__ __forceinline__ void sum_join(Exchange<kVals>& ex, int val, float k, 
     for (int i = 0; i < kMaxWarps / 4; ++i)
       if (i * 4 + sub < warps) s += ex.part[val][i * 4 + sub][pos];
     s = over_subs(s);
-    if (sub == 0) ex.total[val][pos] = s * k;
+    if (sub == 0) ex.total[to][pos] = s * k;
   });
 }
 
@@ -243,6 +244,13 @@ __device__ __forceinline__ void stage_copy(char* dst, const void* src, bool on) 
                  "r"(on ? kBytes : 0)
                  : "memory");
 }
+// the first `bytes` (1 to 4) of an aligned word, zeros behind them
+__device__ __forceinline__ void stage_copy_some(char* dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src), "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ void stage_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -257,24 +265,30 @@ __device__ __forceinline__ F4 staged4(const char* src) {
   else
     return halves4<T>(*reinterpret_cast<const uint2*>(src));
 }
-// A row of the calling thread in a picture: its offset from the picture's first element, with the
-// lane's four positions, and its exponents' from the picture's first (held rows: 32 bits do)
+// The rows of the calling thread in a picture: their offsets from the picture's first element, with
+// the lane's four positions, and of their exponents from the picture's first (held rows: 32 bits
+// do). kWhole: a multiple of 16 channels and of 32 positions, every row and position there.
 constexpr int kStagedRows = 4;
-struct StagedRow {
-  uint32_t e, x;
-  int ch;
-  bool on;
+template <bool kWhole>
+struct StagedRows {
+  uint32_t e0, x0, e4, x4;
+  int ch0, c;
+  __device__ __forceinline__ StagedRows(int c_, int p, int groups) : c(c_) {
+    const int lane = threadIdx.x & 31;
+    ch0 = (threadIdx.x >> 5) * 4 * kStagedRows + (lane >> 3);
+    e0 = (uint32_t)ch0 * (uint32_t)p + (lane & 7) * 4;
+    x0 = (uint32_t)ch0 * (uint32_t)groups;
+    e4 = 4u * (uint32_t)p;
+    x4 = 4u * (uint32_t)groups;
+  }
+  __device__ __forceinline__ uint32_t e(int j) const { return e0 + j * e4; }
+  __device__ __forceinline__ uint32_t x(int j) const { return x0 + j * x4; }
+  __device__ __forceinline__ bool on(int j) const { return kWhole || ch0 + 4 * j < c; }
+  // a channel that exists, for the parameters
+  __device__ __forceinline__ int ch(int j) const {
+    return kWhole ? ch0 + 4 * j : min(ch0 + 4 * j, c - 1);
+  }
 };
-__device__ __forceinline__ StagedRow staged_row(int j, int c, int p, int groups) {
-  const int lane = threadIdx.x & 31;
-  const int row = (threadIdx.x >> 5) * 4 * kStagedRows + j * 4 + (lane >> 3);
-  StagedRow r;
-  r.on = row < c;
-  r.ch = min(row, c - 1);
-  r.e = (uint32_t)r.ch * (uint32_t)p + (lane & 7) * 4;
-  r.x = (uint32_t)r.ch * (uint32_t)groups;
-  return r;
-}
 
 int stage_param(Ctx* ctx, const float* p, int c, int mem, const char* what, const float** out) {
   return stage_bytes_in(ctx, p, (size_t)c * sizeof(float), sizeof(float), mem, what, out);
@@ -294,7 +308,7 @@ int stage_params(Ctx* ctx, const zjai_residual_params& in, int c, int mem,
 // SM are resident at the registers that __launch_bounds__ leaves, so blocks of few warps come in
 // numbers.
 struct Shape {
-  bool staged;
+  bool staged, whole;
   int rows, warps, per_sm;
 };
 Shape shape_of(int c, int p, bool vec, bool backward) {
@@ -303,7 +317,8 @@ Shape shape_of(int c, int p, bool vec, bool backward) {
   // without vector accesses the backward pass takes two rows a thread where the warps allow it
   const int rows = !held ? 0 : !vec && backward && c <= kHeldC / 2 ? 2 : kStagedRows;
   const int warps = rows ? (c + 4 * rows - 1) / (4 * rows) : kMaxWarps;
-  return {held && vec, rows, warps, kMaxWarps / warps};
+  return {held && vec, c % (4 * kStagedRows) == 0 && p % kTapeGroup == 0, rows, warps,
+          kMaxWarps / warps};
 }
 // Four neighbouring positions can be loaded and stored at once: rows of a multiple of four
 // positions, maps aligned to four elements and codes to four bytes.

@@ -46,18 +46,20 @@ template <bool kTaped, class T>
 struct BwdSlot {
   static constexpr int kGrad = 4 * sizeof(T), kKept = kTaped ? 4 : 4 * sizeof(T);
   static constexpr int kBytes = kStagedRows * (2 * kGrad + 3 * kKept);  // per thread
-  static constexpr int kSlots = 2 * kBytes * kThreadsMost <= 200 * 1024 ? 2 : 1;
+  static constexpr int kExps = kTaped ? 3 * kStagedRows * 4 / 8 : 0;  // per thread, words of rows
+  static constexpr int kB = sizeof(T) == 4 ? 0 : kStagedRows * (int)sizeof(float4);
+  static constexpr int kSlots = 2 * kBytes * kThreadsMost <= 180 * 1024 ? 2 : 1;
 };
-template <bool kTaped, class T>
+template <bool kWhole, bool kTaped, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
     residual_norm_bwd_staged_kernel(const BwdArgs<T> a) {
   using S = BwdSlot<kTaped, T>;
   constexpr int kRows = kStagedRows;
-  __shared__ Exchange<4> ex;
+  __shared__ Exchange<4, 9> ex;  // totals: f 0, 1, y 2, 3, a 4, 5, b 6, 7, gate 8
   __shared__ Params<kRows> prm;
   extern __shared__ __align__(16) char slots[];
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows> rows(a.c, warps);
+  const Rows<kRows, kWhole> rows(a.c, warps);
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
@@ -70,9 +72,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   auto join_second = [&](auto f) {
     if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
   };
-  StagedRow row[kRows];
-#pragma unroll
-  for (int j = 0; j < kRows; ++j) row[j] = staged_row(j, a.c, a.p, groups);
+  const StagedRows<kWhole> row(a.c, a.p, groups);
   auto grad_at = [&](int slot, int k, int j) {
     return slots + slot * S::kBytes * (int)blockDim.x +
            ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kGrad;
@@ -81,36 +81,53 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     return slots + slot * S::kBytes * (int)blockDim.x + 2 * kRows * (int)blockDim.x * S::kGrad +
            ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kKept;
   };
-  int exps[3][kRows];  // of the tile copied last
-#pragma unroll
-  for (int j = 0; j < kRows; ++j) exps[0][j] = exps[1][j] = exps[2][j] = 0;
+  // a row's exponent comes as the aligned word that holds it, copied by the first of its lanes
+  auto exp_at = [&](int slot, int k, int j) {
+    return slots + S::kSlots * S::kBytes * (int)blockDim.x +
+           (((slot * 3 + k) * kRows + j) * (int)blockDim.x / 8 + (int)threadIdx.x / 8) * 4;
+  };
+  // b of a row, until df: where dy was, or (f16, bf16) in a place of its own
+  auto b_at = [&](int slot, int j) {
+    char* q = slots + S::kSlots * (S::kBytes + S::kExps) * (int)blockDim.x;
+    return reinterpret_cast<float4*>(
+        sizeof(T) == 4 ? grad_at(slot, 0, j)
+                       : q + (j * (int)blockDim.x + (int)threadIdx.x) * (int)sizeof(float4));
+  };
+  // exponents of the whole map (the gate's too: this path takes its own rows only where it has c)
+  const long long x_all = a.tiles * a.c;
   auto copy = [&](const Tiles& t, int slot) {
     const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
     const long long x = (long long)t.img * a.c * groups + t.g;
-    const bool in = t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    const bool in = kWhole || t.g * kTapeGroup + (lane & 7) * 4 < a.p;
     auto keep = [&](const T* map, const zjai_tape& tp, int k, int j, bool on) {
       if constexpr (kTaped) {
-        stage_copy<4>(kept_at(slot, k, j), tp.codes + e + row[j].e, on);
-        if (row[j].on) exps[k][j] = __ldg(tp.exps + x + row[j].x);
+        stage_copy<4>(kept_at(slot, k, j), tp.codes + e + row.e(j), on);
+        if ((lane & 7) == 0) {
+          const long long at = (x + row.x(j)) & ~3LL;
+          stage_copy_some(exp_at(slot, k, j), tp.exps + at, (int)min(4LL, x_all - at));
+        }
       } else {
-        stage_copy<S::kKept>(kept_at(slot, k, j), map + e + row[j].e, on);
+        stage_copy<S::kKept>(kept_at(slot, k, j), map + e + row.e(j), on);
       }
     };
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const bool on = in && row[j].on;
+      const bool on = in && row.on(j);
       if (need_f) keep(a.f, a.tp.f, 0, j, on);
       if (pre) keep(a.y, a.tp.y, 1, j, on);
-      if (pre) stage_copy<S::kGrad>(grad_at(slot, 1, j), a.dz + e + row[j].e, on);
+      if (pre) stage_copy<S::kGrad>(grad_at(slot, 1, j), a.dz + e + row.e(j), on);
       if (per_row) keep(a.gate, a.tp.gate, 2, j, on);
-      stage_copy<S::kGrad>(grad_at(slot, 0, j), a.dy + e + row[j].e, on);
+      stage_copy<S::kGrad>(grad_at(slot, 0, j), a.dy + e + row.e(j), on);
     }
   };
-  auto kept = [&](int slot, int k, int j, int e) {
-    if constexpr (kTaped)
+  auto kept = [&](int slot, int k, int j, long long x) {
+    if constexpr (kTaped) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j));
+      const int e = (int)(int8_t)(w >> (((uint32_t)x + row.x(j)) & 3) * 8);
       return taped4(*reinterpret_cast<const uint32_t*>(kept_at(slot, k, j)), e);
-    else
+    } else {
       return staged4<T>(kept_at(slot, k, j));
+    }
   };
   float acc[kRows][5];
 #pragma unroll
@@ -124,11 +141,9 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   stage_commit();
   for (int slot = 0; tile.on(); tile.next(), slot ^= S::kSlots - 1) {
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
-    const bool in = at < a.p;
+    const bool in = kWhole || at < a.p;
     const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
-    int ge[kRows], fe[kRows], ye[kRows];
-#pragma unroll
-    for (int j = 0; j < kRows; ++j) fe[j] = exps[0][j], ye[j] = exps[1][j], ge[j] = exps[2][j];
+    const long long x0 = (long long)tile.img * a.c * groups + tile.g;
     F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
       Kept<kTaped, true, T> k;
@@ -142,13 +157,14 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       stage_commit();
     }
     stage_wait<S::kSlots - 1>();
+    if (kTaped) __syncwarp();  // the exponents of the row's other lanes
     F4 f[kRows], y[kRows];  // then LN(f), LN(y)
     if (need_f)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) f[j] = kept(slot, 0, j, fe[j]);
+      for (int j = 0; j < kRows; ++j) f[j] = kept(slot, 0, j, x0);
     if (pre)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) y[j] = kept(slot, 1, j, ye[j]);
+      for (int j = 0; j < kRows; ++j) y[j] = kept(slot, 1, j, x0);
     if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0, warps);
     if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2, warps);
     if (post || pre) {
@@ -157,10 +173,9 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       if (pre) join_second([&](int n, int of) { stats_join(rows, ex, 2, inv_c, warps, n, of); });
       __syncthreads();
     }
-    F4 r1 = all(1.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
+    F4 r2 = all(1.f), am = all(0.f), ay = all(0.f);
     if (post) {
-      const F4 nm = total4(ex, 0);
-      r1 = total4(ex, 1);
+      const F4 nm = total4(ex, 0), r1 = total4(ex, 1);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) f[j] = (f[j] + nm) * r1;
     }
@@ -171,8 +186,8 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         y[j] = (y[j] + nm) * r2;
-        const F4 t = staged4<T>(grad_at(slot, 1, j)) * prm.get(a.prm, kPreW, row[j].ch);
-        if (row[j].on) {
+        const F4 t = staged4<T>(grad_at(slot, 1, j)) * prm.get(a.prm, kPreW, row.ch(j));
+        if (row.on(j)) {
           s0 = s0 + t;
           s1 = fma4(t, y[j], s1);
         }
@@ -180,17 +195,17 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       rows_to_part(s0, ex.part[0][wp]);
       rows_to_part(s1, ex.part[1][wp]);
       __syncthreads();
-      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+      join_first([&](int n, int of) { sum_join(ex, 0, 4, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 5, -inv_c, warps, n, of); });
       __syncthreads();
-      am = total4(ex, 0);  // negated means
-      ay = total4(ex, 1);
+      am = total4(ex, 4);  // negated means
+      ay = total4(ex, 5);
     }
-    F4 b[kRows], t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
+    F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const int ch = row[j].ch;
-      const bool on = row[j].on, write = on && in;
+      const int ch = row.ch(j);
+      const bool on = row.on(j), write = on && in;
       F4 d = staged4<T>(grad_at(slot, 0, j));
       if (pre) {
         const F4 dz = staged4<T>(grad_at(slot, 1, j));
@@ -198,15 +213,15 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
         acc[j][4] += sum4(dz);
         d = fma4(fma4(y[j], ay, dz * prm.get(a.prm, kPreW, ch) + am), r2, d);
       }
-      if (write) store4_in(a.dx + e0 + row[j].e, d);
+      if (write) store4_in(a.dx + e0 + row.e(j), d);
       if (!need_f) continue;
       const F4 u = post ? fma4(f[j], prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch)) : f[j];
       const F4 ds = d * prm.get(a.prm, kScale, ch);
       F4 sg = sg1, du = ds;
       if (per_row) {
         F4 slope;
-        sigmoid4(kept(slot, 2, j, ge[j]), &sg, &slope);
-        if (write) store4_in(a.dgate + e0 + row[j].e, ds * u * slope);
+        sigmoid4(kept(slot, 2, j, x0), &sg, &slope);
+        if (write) store4_in(a.dgate + e0 + row.e(j), ds * u * slope);
       }
       if (a.gate_c) du = ds * sg;
       acc[j][0] += dot4(d * sg, u);
@@ -214,46 +229,54 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       if (post) {
         acc[j][1] += dot4(du, f[j]);
         acc[j][2] += sum4(du);
-        b[j] = du * prm.get(a.prm, kPostW, ch);
+        const F4 b = du * prm.get(a.prm, kPostW, ch);
+        *b_at(slot, j) = flat(b);
         if (on) {
-          t0 = t0 + b[j];
-          t1 = fma4(b[j], f[j], t1);
+          t0 = t0 + b;
+          t1 = fma4(b, f[j], t1);
         }
       } else if (write) {
-        store4_in(a.df + e0 + row[j].e, du);
+        store4_in(a.df + e0 + row.e(j), du);
       }
     }
     if (!need_f && a.df)
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (row[j].on && in) {
+        if (row.on(j) && in) {
           F4 d = staged4<T>(grad_at(slot, 0, j));
           if (pre)
             d = fma4(fma4(y[j], ay, staged4<T>(grad_at(slot, 1, j)) *
-                                        prm.get(a.prm, kPreW, row[j].ch) + am), r2, d);
-          store4_in(a.df + e0 + row[j].e, d);
+                                        prm.get(a.prm, kPreW, row.ch(j)) + am), r2, d);
+          store4_in(a.df + e0 + row.e(j), d);
         }
-    if (S::kSlots == 1) {  // the slot has been read
-      if (ahead.on()) copy(ahead, 0);
-      stage_commit();
-    }
+    if (kTaped) __syncwarp();  // exponents read, before another lane copies over them
+    // one slot: read now, but for b where dy was
+    auto copy_one = [&]() {
+      if (S::kSlots == 1) {
+        if (ahead.on()) copy(ahead, 0);
+        stage_commit();
+      }
+    };
+    if (sizeof(T) != 4 || !post) copy_one();
     if (!post && a.gate_c != 1) continue;
     if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
     if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
     __syncthreads();
     if (post) {
-      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+      join_first([&](int n, int of) { sum_join(ex, 0, 6, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 7, -inv_c, warps, n, of); });
     }
-    if (a.gate_c == 1) sum_join(ex, 2, 1.f, warps, wp, warps);
+    if (a.gate_c == 1) sum_join(ex, 2, 8, 1.f, warps, wp, warps);
     __syncthreads();
     if (a.gate_c == 1 && threadIdx.x < 8)
-      store4<true>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 2) * slope1);
+      store4<true>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 8) * slope1);
     if (!post) continue;
-    const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
+    const F4 bm = total4(ex, 6), bf = total4(ex, 7), r1 = total4(ex, 1);  // negated means
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      if (row[j].on && in) store4_in(a.df + e0 + row[j].e, fma4(f[j], bf, b[j] + bm) * r1);
+      if (row.on(j) && in)
+        store4_in(a.df + e0 + row.e(j), fma4(f[j], bf, make4(*b_at(slot, j)) + bm) * r1);
+    if (sizeof(T) == 4) copy_one();
   }
   stage_wait<0>();
   float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
@@ -264,7 +287,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       float s = acc[j][i];
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if ((lane & 7) == 0 && row[j].on) out[i * a.c + row[j].ch] = s;
+      if ((lane & 7) == 0 && row.on(j)) out[i * a.c + row.ch(j)] = s;
     }
 }
 
@@ -272,7 +295,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
 // the parameter sums in registers, or per channel in shared memory.
 template <int kRows, bool kTaped, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(const BwdArgs<T> a) {
-  __shared__ Exchange<4> ex;
+  __shared__ Exchange<4, 4> ex;
   __shared__ Params<kRows> prm;
   extern __shared__ float acc_c[];  // [5][c] where rows are not held
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -361,8 +384,8 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
       rows_to_part(s0, ex.part[0][wp]);
       rows_to_part(s1, ex.part[1][wp]);
       __syncthreads();
-      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+      join_first([&](int n, int of) { sum_join(ex, 0, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 1, -inv_c, warps, n, of); });
       __syncthreads();
       am = total4(ex, 0);  // negated means
       ay = total4(ex, 1);
@@ -417,10 +440,10 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
     __syncthreads();
     if (post) {
-      join_first([&](int n, int of) { sum_join(ex, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, -inv_c, warps, n, of); });
+      join_first([&](int n, int of) { sum_join(ex, 0, 0, -inv_c, warps, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 1, -inv_c, warps, n, of); });
     }
-    if (a.gate_c == 1) sum_join(ex, 2, 1.f, warps, wp, warps);
+    if (a.gate_c == 1) sum_join(ex, 2, 2, 1.f, warps, wp, warps);
     __syncthreads();
     if (a.gate_c == 1 && threadIdx.x < 8)
       store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * slope1);
@@ -555,6 +578,7 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     vec.map(ddy, es).map(ddz, es).map(df, es).map(dg, es).map(dyy, es);
     vec.map(gx, es).map(gf, es).map(gg, es);
     vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
+    vec.map(dt.f.exps, 1).map(dt.gate.exps, 1).map(dt.y.exps, 1);
     const Shape sh = shape_of(c, p, vec.ok, true);
     const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
     float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
@@ -568,8 +592,9 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
       void (*k)(BwdArgs<T>) = nullptr;
       int smem = 0;
       if (sh.staged) {
-        k = residual_norm_bwd_staged_kernel<kTaped, T>;
-        smem = S::kSlots * S::kBytes * sh.warps * 32;
+        k = sh.whole ? residual_norm_bwd_staged_kernel<true, kTaped, T>
+                     : residual_norm_bwd_staged_kernel<false, kTaped, T>;
+        smem = (S::kSlots * (S::kBytes + S::kExps) + S::kB) * sh.warps * 32;
       } else if (sh.rows) {
         k = sh.rows == 2 ? residual_norm_bwd_kernel<2, kTaped, false, T>
                          : residual_norm_bwd_kernel<4, kTaped, false, T>;

@@ -59,8 +59,9 @@ __global__ void __launch_bounds__(256) tape_pack_flat_kernel(const T* __restrict
     uint32_t m = max(amax4(v[k][0]), amax4(v[k][1]));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint2 w = make_uint2(codes4(v[k][0], m), codes4(v[k][1], m));
     if (i >= pieces) continue;
-    *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(codes4(v[k][0], m), codes4(v[k][1], m));
+    *reinterpret_cast<uint2*>(codes + i * 8) = w;
     if ((threadIdx.x & 3) == 0) exps[i >> 2] = (int8_t)tape_exp(m);
   }
 }
