@@ -113,7 +113,7 @@ __device__ __forceinline__ void stats_part(const Rows<kRows, kAll>& rows, V&& v,
   FOR_ROWS(j) if (rows.on(j)) s = s + v(j);
   s = over_rows(s);
   const int n = rows.of_warp(wp, warps);
-  const F4 nm = s * all(n ? __fdividef(-1.f, (float)n) : 0.f);
+  const F4 nm = s * all(kAll ? -1.f / (4 * kRows) : n ? __fdividef(-1.f, (float)n) : 0.f);
   FOR_ROWS(j) if (rows.on(j)) {
     const F4 d = v(j) + nm;
     q = fma4(d, d, q);
@@ -150,7 +150,8 @@ __device__ __forceinline__ void stats_join(const Rows<kRows, kAll>& rows, E& ex,
     for (int i = 0; i < kMaxWarps / 4; ++i) {
       const int w = i * 4 + sub, n = w < warps ? rows.of_warp(w, warps) : 0;
       if (n) {
-        const float d = __fdividef(s[i], (float)n) - m;
+        // (whole warps: by a constant)
+        const float d = (kAll ? s[i] * (1.f / (4 * kRows)) : __fdividef(s[i], (float)n)) - m;
         q += fmaf((float)n * d, d, ex.part[val + 1][w][pos]);
       }
     }

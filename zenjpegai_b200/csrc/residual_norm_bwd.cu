@@ -81,10 +81,11 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     return slots + slot * S::kBytes * (int)blockDim.x + 2 * kRows * (int)blockDim.x * S::kGrad +
            ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kKept;
   };
-  // a row's exponent comes as the aligned word that holds it, copied by the first of its lanes
-  auto exp_at = [&](int slot, int k, int j) {
+  // a row's exponent comes as the aligned word that holds it, copied by one lane per row of the warp
+  constexpr int kWarpRows = 4 * kRows;
+  auto exp_at = [&](int slot, int k, int r) {
     return slots + S::kSlots * S::kBytes * (int)blockDim.x +
-           (((slot * 3 + k) * kRows + j) * (int)blockDim.x / 8 + (int)threadIdx.x / 8) * 4;
+           (((slot * 3 + k) * warps + wp) * kWarpRows + r) * 4;
   };
   // b of a row, until df: where dy was, or (f16, bf16) in a place of its own
   auto b_at = [&](int slot, int j) {
@@ -99,13 +100,23 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
     const long long x = (long long)t.img * a.c * groups + t.g;
     const bool in = kWhole || t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    auto keep_exps = [&](const zjai_tape& tp, int k) {
+      const int ch = wp * kWarpRows + lane;
+      if (lane >= kWarpRows || (!kWhole && ch >= a.c)) return;
+      const uint32_t at = ((uint32_t)(x & 3) + (uint32_t)ch * (uint32_t)groups) & ~3u;
+      const int8_t* src = tp.exps + (x & ~3LL) + at;
+      // whole tiles: a multiple of four exponents in all
+      const int bytes = kWhole ? 4 : (int)min(4LL, x_all - (x & ~3LL) - at);
+      stage_copy_some(exp_at(slot, k, lane), src, bytes);
+    };
+    if (kTaped) {
+      if (need_f) keep_exps(a.tp.f, 0);
+      if (pre) keep_exps(a.tp.y, 1);
+      if (per_row) keep_exps(a.tp.gate, 2);
+    }
     auto keep = [&](const T* map, const zjai_tape& tp, int k, int j, bool on) {
       if constexpr (kTaped) {
         stage_copy<4>(kept_at(slot, k, j), tp.codes + e + row.e(j), on);
-        if ((lane & 7) == 0) {
-          const long long at = (x + row.x(j)) & ~3LL;
-          stage_copy_some(exp_at(slot, k, j), tp.exps + at, (int)min(4LL, x_all - at));
-        }
       } else {
         stage_copy<S::kKept>(kept_at(slot, k, j), map + e + row.e(j), on);
       }
@@ -120,10 +131,10 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       stage_copy<S::kGrad>(grad_at(slot, 0, j), a.dy + e + row.e(j), on);
     }
   };
-  auto kept = [&](int slot, int k, int j, long long x) {
+  auto kept = [&](int slot, int k, int j, uint32_t x) {
     if constexpr (kTaped) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j));
-      const int e = (int)(int8_t)(w >> (((uint32_t)x + row.x(j)) & 3) * 8);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j * 4 + (lane >> 3)));
+      const int e = (int)(int8_t)(w >> ((x + row.x(j)) & 3) * 8);
       return taped4(*reinterpret_cast<const uint32_t*>(kept_at(slot, k, j)), e);
     } else {
       return staged4<T>(kept_at(slot, k, j));
@@ -143,7 +154,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
     const bool in = kWhole || at < a.p;
     const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
-    const long long x0 = (long long)tile.img * a.c * groups + tile.g;
+    const uint32_t x0 = (uint32_t)((long long)tile.img * a.c * groups + tile.g);
     F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
       Kept<kTaped, true, T> k;
