@@ -12,22 +12,23 @@
 // what the ones before left (8 + 8 + 8 bits: exact), so every product is exact and the result has
 // the error of its f32 sums alone, like an f32 product of the f32 operands. The tensor core's own
 // accumulation truncates, a bias that grows with the length of the chain: the first terms have an
-// accumulator of their own, and both are drained every kWindow positions and added, rounding to
+// accumulator of their own, and both are drained every 256 or 512 positions and added, rounding to
 // nearest, to f32 sums in registers.
 //
-// One CTA per SM takes a 128 x N tile of dw over a range of positions, in chunks of 64:
+// One CTA per SM takes a 128 x N tile of dw over a share of the positions, every so many chunks of 64
+// (the CTAs of a tile work on neighbouring chunks at a time: rows are far apart in memory, and with
+// ranges of their own they kept opening DRAM pages for 128 bytes):
 //  - the operands come to shared memory some chunks ahead: by TMA where all rows start on 16 bytes
 //    (kVec; bf16 d_out, which needs no conversion, straight into the operand), else by cp.async,
 //    each thread copying what it will itself convert (rows of odd length start anywhere, which a
 //    TMA box cannot);
-//  - 16 converter warps turn a chunk into bf16 in the 128-byte-swizzled K-major layout that the
-//    tensor core reads (16-byte piece j of row r at j ^ (r & 7)), and drain the accumulators, half
-//    a window after they are complete. They are what bounds the kernel below HBM's rate (issue
-//    slots), so a chunk is read, converted and stored in three strokes, with packed arithmetic;
+//  - 16 converter warps, in groups that take turns, turn a chunk into bf16 in the 128-byte-swizzled
+//    K-major layout that the tensor core reads (16-byte piece j of row r at j ^ (r & 7)), and drain
+//    the accumulators, half a window after they are complete;
 //  - one thread issues the MMAs of a chunk, alternating between two accumulator sets in TMEM;
 //  - db comes from the converters' registers, or, where d_out does not pass through them, from a
 //    row of ones below the input's rows in the operand: one more column of the product.
-// Ranges of one tile are summed in order by a second kernel (no atomics). Every wait is bounded.
+// Shares of one tile are summed in order by a second kernel (no atomics). Every wait is bounded.
 #include <algorithm>
 #include <type_traits>
 
@@ -38,37 +39,42 @@ namespace zjai {
 namespace {
 
 constexpr int kM = 128, kN = 128;       // tile of dw
-constexpr int kWindow = 256;            // positions between drains
 constexpr int kWorkers = 16, kMmaWarp = kWorkers, kTmaWarp = kWorkers + 1;
 constexpr int kWorkThreads = 32 * kWorkers;
 constexpr int kThreads = 32 * (kTmaWarp + 1);
 constexpr int kChunk = 64;                 // positions of a pipeline stage
-constexpr int kPerWindow = kWindow / kChunk;
 constexpr int kBlock = kM * kChunk * 2;    // a chunk of 128 rows in bf16
 constexpr int kOnes = 16 * kChunk * 2;     // and of the 16 rows with the ones
 constexpr int kBufCols = 256;              // TMEM columns of an accumulator set
 
-// Per element type and alignment: bf16 terms of a d_out element; stages of converted operands,
-// chunks copied ahead of them (kAhead); 32-bit words a thread copies (cp.async) of 8 positions of
-// d_out (the words that hold them: one more where they start anywhere) and of 16 codes.
+// Per element type and alignment: bf16 terms of a d_out element; groups of converter warps, which
+// take every kGroups-th chunk (a chunk has a fixed cost of waits and hand-offs per warp, about as
+// long as its conversion by 16 warps: with one group the kernel took 1.3 to 1.5 times as long);
+// stages of converted operands and chunks copied ahead of them; chunks between drains. cp.async:
+// 32-bit words a thread copies of 8 positions of d_out (the words that hold them: one more where
+// they start anywhere) and of 16 codes.
 template <bool kVec, class T>
 struct Form;
 template <>
 struct Form<true, float> {
-  static constexpr int kTerms = 3, kStages = 2, kAhead = 2, kRaw = 2 * kBlock + kBlock / 2;
+  static constexpr int kTerms = 3, kGroups = 2, kStages = 2, kAhead = 2, kPerWindow = 4;
+  static constexpr int kRaw = 2 * kBlock + kBlock / 2;
 };
 template <>
 struct Form<true, __half> {
-  static constexpr int kTerms = 2, kStages = 2, kAhead = 4, kRaw = kBlock + kBlock / 2;
+  static constexpr int kTerms = 2, kGroups = 2, kStages = 2, kAhead = 4, kPerWindow = 4;
+  static constexpr int kRaw = kBlock + kBlock / 2;
 };
 template <>
 struct Form<true, __nv_bfloat16> {  // kRaw: the codes alone
-  static constexpr int kTerms = 1, kStages = 5, kAhead = 4, kRaw = kBlock / 2;
+  static constexpr int kTerms = 1, kGroups = 4, kStages = 5, kAhead = 4, kPerWindow = 8;
+  static constexpr int kRaw = kBlock / 2;
 };
 template <class T>
 struct Form<false, T> {
   static constexpr int kTerms = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;
-  static constexpr int kStages = kTerms == 1 ? 3 : 2, kAhead = kTerms == 3 ? 2 : 3;
+  static constexpr int kGroups = 1, kStages = kTerms == 1 ? 3 : 2, kAhead = kTerms == 3 ? 2 : 3;
+  static constexpr int kPerWindow = 4;
   static constexpr int kWordsD = sizeof(T) == 4 ? 8 : 5, kWordsX = 5;
   static constexpr int kRaw = (2 * kWordsD + kWordsX) * 4 * kWorkThreads;
 };
@@ -226,12 +232,33 @@ __device__ __forceinline__ uint2 taped_bf16(uint32_t w, __nv_bfloat162 scale) {
   return out;
 }
 
+// A chunk's picture and place in it, of a sequence with a fixed step.
+struct Chunk {
+  int img, in, step_img, step_in, of;
+  __device__ __forceinline__ Chunk(int first, int step, int chunks_img) : of(chunks_img) {
+    img = first / of;
+    in = first - img * of;
+    step_img = step / of;
+    step_in = step - step_img * of;
+  }
+  __device__ __forceinline__ void next() {
+    img += step_img;
+    in += step_in;
+    if (in >= of) in -= of, ++img;
+  }
+};
+
 template <bool kVec, class T>
 __global__ void __launch_bounds__(kThreads, 1)
     weight_grad_kernel(const __grid_constant__ CUtensorMap map_d,
                        const __grid_constant__ CUtensorMap map_x, const WgArgs a) {
   using F = Form<kVec, T>;
   constexpr int kTerms = F::kTerms, kStages = F::kStages, kAhead = F::kAhead, kRaw = F::kRaw;
+  constexpr int kGroups = F::kGroups, kPerWindow = F::kPerWindow;
+  // a slot is always read by the same group: another one's parity test would take the phase before
+  // the last for the one it waits for
+  static_assert(kAhead % kGroups == 0, "slots change groups");
+  constexpr int kGroupWarps = kWorkers / kGroups, kGroupThreads = kWorkThreads / kGroups;
   constexpr int kStageBytes = stage_bytes<kVec, T>();
   constexpr bool kDirect = direct<kVec, T>();
   constexpr int kSets = kTerms > 1 ? 2 : 1;  // accumulators of a set: first terms, the others
@@ -244,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x, split = blockIdx.y;
   const int o0 = (tile % a.m_tiles) * kM, i0 = (tile / a.m_tiles) * kN;
-  const long long q0 = a.chunks * split / a.splits, q1 = a.chunks * (split + 1) / a.splits;
-  const int count = (int)(q1 - q0), windows = (count + kPerWindow - 1) / kPerWindow;
-  const int img0 = (int)(q0 / a.chunks_img), in_img0 = (int)(q0 - (long long)img0 * a.chunks_img);
+  // chunks split, split + splits, ..
+  const int count = (int)((a.chunks - split + a.splits - 1) / a.splits);
+  const int windows = (count + kPerWindow - 1) / kPerWindow;
   const bool want_db = a.db && i0 == 0;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t raw_base = smem + kStages * kStageBytes;
@@ -259,13 +286,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + 8 * i, kWorkers);
+      mbar_init(full + 8 * i, kGroupWarps);
       mbar_init(empty + 8 * i, 1);
       mbar_init(d_full + 8 * i, 1);
     }
     for (int i = 0; i < kAhead; ++i) {
       mbar_init(raw_full + 8 * i, 1);
-      mbar_init(raw_empty + 8 * i, kWorkers);
+      mbar_init(raw_empty + 8 * i, kGroupWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
@@ -335,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (kVec && lane == 0) {
       tma_prefetch_desc(&map_d);
       tma_prefetch_desc(&map_x);
-      int img = img0, at = in_img0 * kChunk, k = 0;
+      Chunk q(split, a.splits, a.chunks_img);
+      int k = 0;
       for (; k < count; ++k) {
         const int sl = k % kAhead, st = k % kStages;
         if (k >= kAhead &&
@@ -347,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        a.limit))
           break;
         const uint32_t raw = raw_base + sl * kRaw, bar = raw_full + 8 * sl;
+        const int img = q.img, at = q.in * kChunk;
         mbar_arrive_expect_tx(bar, kRaw);
         if constexpr (kDirect) {
           mbar_arrive_expect_tx(d_full + 8 * st, kBlock);
@@ -356,11 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (sizeof(T) == 4) tma_load_3d(raw + kBlock, &map_d, bar, at + 32, o0, img);
         }
         tma_load_3d(raw + kRaw - kBlock / 2, &map_x, bar, at, i0, img);
-        at += kChunk;
-        if (at >= a.p) {
-          at = 0;
-          ++img;
-        }
+        q.next();
       }
       // all copies landed before the CTA goes, also after a wait that gave up
       for (int j = max(0, k - kAhead); j < k; ++j)
@@ -371,77 +396,61 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    const int tid = threadIdx.x;
-    // d_out: rows dr and dr + 64, positions 8 dj ..; f32 from TMA: row dr, positions 8 dj .. of
-    // each half of the chunk, rows spread over a warp's lanes such that eight lanes' 16 bytes lie
-    // in different banks both as read (two pieces of four of a half row) and as stored
+    // this thread's group of converters takes the chunks `group`, group + kGroups, ..; pieces of a
+    // chunk: d_out rows dr + u kRowsD, positions 8 dj .. (f32 from TMA: of each half of the chunk,
+    // rows spread over a warp's lanes such that eight lanes' 16 bytes lie in different banks both as
+    // read, two pieces of four of a half row, and as stored); input rows xr + u kRowsX, positions
+    // 16 xj ..
+    const int group = warp / kGroupWarps, tid = threadIdx.x % kGroupThreads;
     constexpr bool kHalves = kVec && sizeof(T) == 4;
+    constexpr int kRowsD = kHalves ? kGroupThreads / 4 : kGroupThreads / 8, kUnitsD = kM / kRowsD;
+    constexpr int kRowsX = kGroupThreads / 4, kUnitsX = kN / kRowsX;
     const int l8 = lane >> 2;
-    const int dr = kHalves ? warp * 8 + ((l8 >> 1) ^ (l8 & 1 ? 5 : 0)) : tid >> 3;
+    const int dr = kHalves ? (tid >> 5) * 8 + ((l8 >> 1) ^ (l8 & 1 ? 5 : 0)) : tid >> 3;
     const int dj = kHalves ? lane & 3 : tid & 7;
-    const int xr = tid >> 2, xj = tid & 3;  // input: row xr, positions 16 xj ..
-    const bool d_ok[2] = {o0 + dr < a.oc, o0 + 64 + dr < a.oc};
-    const bool x_ok = xr < min(a.nb, a.c - i0), x_in = xr < a.nb;
+    const int xr = tid >> 2, xj = tid & 3;
+    const int x_rows = min(a.nb, a.c - i0);
     auto swizzled = [](uint32_t base, int r, int j) { return base + r * 128 + ((j ^ (r & 7)) << 4); };
 
     // cp.async: the chunk being copied, and the one being converted
-    struct Place {
-      const T* d;
-      const uint8_t* x;
-      int at;
-    };
     const T* d_lo = static_cast<const T*>(a.dout);
     const T* d_hi = d_lo + a.d_elems;
     const uint8_t* x_lo = reinterpret_cast<const uint8_t*>(a.codes);
     const uint8_t* x_hi = x_lo + a.x_elems;
     const long long d64 = 64LL * a.p;
-    Place next = {d_lo + ((long long)img0 * a.oc + o0 + dr) * a.p,
-                  x_lo + ((long long)img0 * a.c + i0 + xr) * a.p, in_img0 * kChunk};
-    Place cur = next;
+    Chunk next(split, a.splits, a.chunks_img), cur = next;
+    auto row_d = [&](const Chunk& q) { return d_lo + ((long long)q.img * a.oc + o0 + dr) * a.p; };
+    auto row_x = [&](const Chunk& q) { return x_lo + ((long long)q.img * a.c + i0 + xr) * a.p; };
     int copied = 0;
-    auto advance = [&](Place& pl) {
-      pl.at += kChunk;
-      if (pl.at >= a.p) {
-        pl.at = 0;
-        pl.d += (long long)a.oc * a.p;
-        pl.x += (long long)a.c * a.p;
-      }
-    };
     auto copy_chunk = [&]() {
       if constexpr (!kVec) {
         if (copied < count) {
           const uint32_t raw = raw_base + copied % kAhead * kRaw + tid * 4;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            copy_piece<T>(raw + u * F::kWordsD * 4 * kWorkThreads, next.d + u * d64,
-                          next.at + dj * 8, a.p, d_ok[u], d_lo, d_hi);
-          const int at = next.at + xj * 16;
-          copy_words5(raw + 2 * F::kWordsD * 4 * kWorkThreads, next.x + at,
-                      x_ok ? max(0, min(16, a.p - at)) : 0, x_lo, x_hi);
+            copy_piece<T>(raw + u * F::kWordsD * 4 * kWorkThreads, row_d(next) + u * d64,
+                          next.in * kChunk + dj * 8, a.p, o0 + u * 64 + dr < a.oc, d_lo, d_hi);
+          const int at = next.in * kChunk + xj * 16;
+          copy_words5(raw + 2 * F::kWordsD * 4 * kWorkThreads, row_x(next) + at,
+                      xr < x_rows ? max(0, min(16, a.p - at)) : 0, x_lo, x_hi);
           ++copied;
-          advance(next);
+          next.next();
         }
         copy_commit();
       }
     };
-    // what a chunk's exponents are taken from: a quad of lanes shares a row, and holds the row's 16
-    // exponent bytes of 8 chunks, 4 a lane, loaded 8 chunks ahead
-    const int8_t* pe = a.exps + ((long long)img0 * a.c + i0 + xr) * a.groups;
-    int exp_at = in_img0 & ~7;             // chunk in the picture of the window to load next
-    int exp_left = count + (in_img0 & 7);  // chunks from there on
-    uint32_t eb[4], ew = 0u;
-    auto load_exps = [&]() {
-      if (exp_left <= 0) return;
-      const int g0 = exp_at * 2 + xj * 4;
+    // the exponents of the group's next chunk, loaded while it converts the current one
+    Chunk ahead(split + group * a.splits, kGroups * a.splits, a.chunks_img);
+    int eb[kUnitsX];
+    auto load_exps = [&](bool on) {
+      const int8_t* pe = a.exps + ((long long)ahead.img * a.c + i0 + xr) * a.groups;
+      const int g = 2 * ahead.in + (xj >> 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        eb[i] = x_ok && g0 + i < a.groups ? (uint32_t)(uint8_t)__ldg(pe + g0 + i) : 0u;
-      exp_left -= min(8, a.chunks_img - exp_at);
-      exp_at += 8;
-      if (exp_at >= a.chunks_img) {
-        exp_at = 0;
-        pe += (long long)a.c * a.groups;
-      }
+      for (int u = 0; u < kUnitsX; ++u)
+        eb[u] = on && g < a.groups && u * kRowsX + xr < x_rows
+                    ? __ldg(pe + (long long)(u * kRowsX) * a.groups + g)
+                    : 0;
+      ahead.next();
     };
 
     // accumulator rows 32 (warp % 4) + lane, columns 32 (warp / 4) ..
@@ -481,97 +490,96 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++drained;
       return true;
     };
-    constexpr int kRows = kHalves ? 1 : 2;
-    float2 bsum[kRows] = {};
-    float btot[kRows] = {};
+    float2 bsum[kUnitsD] = {};
+    float btot[kUnitsD] = {};
 
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) copy_chunk();
-    load_exps();
-    int in = in_img0;  // the chunk's place in its picture
-    bool fresh = true, ok = true;
-    for (int k = 0; k < count && ok; ++k) {
+    load_exps(group < count);
+    bool ok = true;
+    for (int k = group, turn = 0; k < count && ok; k += kGroups, ++turn) {
       const int st = k % kStages, sl = k % kAhead;
       const uint32_t stage = smem + st * kStageBytes;
       const uint32_t raw = raw_base + sl * kRaw;
-      // read
-      uint32_t wd[2][2 * sizeof(T)], wx[4];
+      int e[kUnitsX];
+#pragma unroll
+      for (int u = 0; u < kUnitsX; ++u) e[u] = eb[u];
+      load_exps(k + kGroups < count);
+      // read all of it, so that the slot is free for the next copy while this one is converted
+      constexpr int kParts = kDirect ? 0 : kUnitsD * (kHalves ? 2 : 1);  // f32: part i of half i & 1
+      uint32_t wx[kUnitsX][4], wd[kParts ? kParts : 1][2 * sizeof(T)];
       if constexpr (kVec) {
         ok = mbar_wait_sleep(raw_full + 8 * sl, (k / kAhead) & 1, abort, a.err, DEV_TIMEOUT_FULL,
                              a.limit);
         if (!ok) break;
-        ld_shared16(raw + kRaw - kBlock / 2 + xr * 64 + xj * 16, wx);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kUnitsX; ++u)
+          ld_shared16(raw + kRaw - kBlock / 2 + (u * kRowsX + xr) * 64 + xj * 16, wx[u]);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
           if constexpr (kHalves) {
-            ld_shared16(swizzled(raw + u * kBlock, dr, 2 * dj), wd[u]);
-            ld_shared16(swizzled(raw + u * kBlock, dr, 2 * dj + 1), wd[u] + 4);
-          } else if constexpr (!kDirect) {
-            ld_shared16(swizzled(raw, u * 64 + dr, dj), wd[u]);
+            const uint32_t at = raw + (i & 1) * kBlock;
+            ld_shared16(swizzled(at, (i >> 1) * kRowsD + dr, 2 * dj), wd[i]);
+            ld_shared16(swizzled(at, (i >> 1) * kRowsD + dr, 2 * dj + 1), wd[i] + 4);
+          } else {
+            ld_shared16(swizzled(raw, i * kRowsD + dr, dj), wd[i]);
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(raw_empty + 8 * sl);
       } else {
         copy_wait<kAhead - 1>();
-        const uint32_t mine = raw + tid * 4;
-        const int at = cur.at + xj * 16;
-        place_words5(mine + 2 * F::kWordsD * 4 * kWorkThreads, cur.x + at,
-                     x_ok ? max(0, min(16, a.p - at)) : 0, wx);
+        const int at = cur.in * kChunk + xj * 16;
+        place_words5(raw + tid * 4 + 2 * F::kWordsD * 4 * kWorkThreads, row_x(cur) + at,
+                     xr < x_rows ? max(0, min(16, a.p - at)) : 0, wx[0]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          get_piece<T>(mine + u * F::kWordsD * 4 * kWorkThreads, cur.d + u * d64, cur.at + dj * 8,
-                       a.p, d_ok[u], wd[u]);
-        advance(cur);
-      }
-      if (fresh || (in & 7) == 0) {
-        ew = eb[0] | eb[1] << 8 | eb[2] << 16 | eb[3] << 24;
-        load_exps();
-        fresh = false;
-      }
-      const int g = 2 * (in & 7) + (xj >> 1);
-      const int e = (int)(int8_t)(__shfl_sync(0xffffffffu, ew, (lane & ~3) + (g >> 2)) >> (8 * (g & 3)));
-      if (++in == a.chunks_img) in = 0;
-      // convert
-      const uint32_t sb = e == kTapeNan ? 0x7fc0u : (uint32_t)(max(e, -126) + 127) << 7;
-      const uint32_t s2 = sb | sb << 16;
-      const __nv_bfloat162 sc = reinterpret_cast<const __nv_bfloat162&>(s2);
-      const uint2 v0 = taped_bf16(wx[0], sc), v1 = taped_bf16(wx[1], sc);
-      const uint2 v2 = taped_bf16(wx[2], sc), v3 = taped_bf16(wx[3], sc);
-      if constexpr (kVec) {  // the slot is read out once its words are used
-        __syncwarp();
-        if (kDirect && lane == 0) mbar_arrive(raw_empty + 8 * sl);
+        for (int i = 0; i < kParts; ++i)
+          get_piece<T>(raw + tid * 4 + i * F::kWordsD * 4 * kWorkThreads, row_d(cur) + i * d64,
+                       cur.in * kChunk + dj * 8, a.p, o0 + i * 64 + dr < a.oc, wd[i]);
       }
       if (k >= kStages) {
         ok = mbar_wait_sleep(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
                              a.limit);
         if (!ok) break;
       }
-      if (x_in) {
-        const uint32_t to = stage + kTerms * kBlock;
-        st_shared16(swizzled(to, xr, 2 * xj), make_uint4(v0.x, v0.y, v1.x, v1.y));
-        st_shared16(swizzled(to, xr, 2 * xj + 1), make_uint4(v2.x, v2.y, v3.x, v3.y));
+#pragma unroll
+      for (int u = 0; u < kUnitsX; ++u) {
+        const uint32_t sb = e[u] == kTapeNan ? 0x7fc0u : (uint32_t)(max(e[u], -126) + 127) << 7;
+        const uint32_t s2 = sb | sb << 16;
+        const __nv_bfloat162 sc = reinterpret_cast<const __nv_bfloat162&>(s2);
+        const uint2 v0 = taped_bf16(wx[u][0], sc), v1 = taped_bf16(wx[u][1], sc);
+        const uint2 v2 = taped_bf16(wx[u][2], sc), v3 = taped_bf16(wx[u][3], sc);
+        const int r = u * kRowsX + xr;
+        if (r < a.nb) {
+          const uint32_t to = stage + kTerms * kBlock;
+          st_shared16(swizzled(to, r, 2 * xj), make_uint4(v0.x, v0.y, v1.x, v1.y));
+          st_shared16(swizzled(to, r, 2 * xj + 1), make_uint4(v2.x, v2.y, v3.x, v3.y));
+        }
       }
       if constexpr (!kDirect) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint32_t at = kHalves ? swizzled(stage, dr, 4 * u + dj)
-                                      : swizzled(stage, u * 64 + dr, dj);
-          const uint32_t* w = wd[u];
+        for (int i = 0; i < kParts; ++i) {
+          const int u = kHalves ? i >> 1 : i, r = u * kRowsD + dr;
+          const uint32_t at = kHalves ? swizzled(stage, r, 4 * (i & 1) + dj) : swizzled(stage, r, dj);
+          const uint32_t* w = wd[i];
           float2 f[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int q = 0; q < 4; ++q) {
             if constexpr (sizeof(T) == 4)
-              f[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+              f[q] = make_float2(__uint_as_float(w[2 * q]), __uint_as_float(w[2 * q + 1]));
             else if constexpr (kTerms == 2)
-              f[i] = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+              f[q] = __half22float2(reinterpret_cast<const __half2&>(w[q]));
             else
-              f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+              f[q] = make_float2(__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xffff0000u));
           }
           const float2 s = __fadd2_rn(__fadd2_rn(f[0], f[1]), __fadd2_rn(f[2], f[3]));
-          bsum[u % kRows] = __fadd2_rn(bsum[u % kRows], s);
+          bsum[u] = __fadd2_rn(bsum[u], s);
           if constexpr (kTerms == 1) {
             st_shared16(at, make_uint4(w[0], w[1], w[2], w[3]));
           } else {
-            const bool finite = fabsf(s.x + s.y) < __uint_as_float(0x7f800000u);
+            // an infinity or NaN anywhere makes the sum one: then each rest is looked at
+            const bool finite =
+                __all_sync(0xffffffffu, fabsf(s.x + s.y) < __uint_as_float(0x7f800000u));
 #pragma unroll
             for (int t = 0; t < kTerms; ++t) {
               st_shared16(at + t * kBlock, make_uint4(bf2(f[0].x, f[0].y), bf2(f[1].x, f[1].y),
@@ -579,56 +587,68 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (t + 1 == kTerms) continue;
               if (finite) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  f[i] = __fadd2_rn(f[i], make_float2(-trunc_bf(f[i].x), -trunc_bf(f[i].y)));
+                for (int q = 0; q < 4; ++q)
+                  f[q] = __fadd2_rn(f[q], make_float2(-trunc_bf(f[q].x), -trunc_bf(f[q].y)));
               } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  f[i] = make_float2(rest_bf_any(f[i].x), rest_bf_any(f[i].y));
+                for (int q = 0; q < 4; ++q)
+                  f[q] = make_float2(rest_bf_any(f[q].x), rest_bf_any(f[q].y));
               }
             }
           }
         }
       }
+      if (!kVec) cur.next();
       copy_chunk();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(full + 8 * st);
-        if (kVec && !kDirect) mbar_arrive(raw_empty + 8 * sl);
-      }
-      if (!kDirect && (k & 31) == 31) {  // two levels: chains of 32 chunks, and of the chains
+      if (lane == 0) mbar_arrive(full + 8 * st);
+      if (!kDirect && (turn & 31) == 31) {  // two levels: chains of 32 chunks, and of the chains
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kUnitsD; ++i) {
           btot[i] += bsum[i].x + bsum[i].y;
           bsum[i] = make_float2(0.f, 0.f);
         }
       }
-      if (k % kPerWindow == kPerWindow / 2 && k >= kPerWindow) ok = drain_window();
+      if (k % kPerWindow >= kPerWindow / 2 && drained < k / kPerWindow) ok = drain_window();
     }
     if (!kVec) copy_wait<0>();
     while (ok && drained < windows) ok = drain_window();
+    // the operands' stages are free now
+    float* stage_f = reinterpret_cast<float*>(smem_raw + (smem - smem_u32(smem_raw)));
     const int o = o0 + (warp & 3) * 32 + lane;
     if (want_db) {
       float* db = a.db + (long long)split * a.oc;
       if constexpr (kDirect) {
         if (c0 == 0 && o < a.oc) db[o] = acc_db;
       } else {
+        // each group's sums of the rows, then their sum
+        float* rows = stage_f + kWorkers * 32 * 33;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kUnitsD; ++i) {
           float s = btot[i] + (bsum[i].x + bsum[i].y);
 #pragma unroll
           for (int x = kHalves ? 2 : 4; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-          if (dj == 0 && d_ok[i]) db[o0 + i * 64 + dr] = s;
+          if (dj == 0) rows[group * kM + i * kRowsD + dr] = s;
+        }
+        named_bar_sync(1, kWorkThreads);
+        if (threadIdx.x < kM && o0 + (int)threadIdx.x < a.oc) {
+          float s = 0.f;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) s += rows[g * kM + threadIdx.x];
+          db[o0 + threadIdx.x] = s;
         }
       }
     }
-    if (o < a.oc) {
-      float* out = a.dw + ((long long)split * a.oc + o) * a.c + i0 + c0;
+    // a warp's 32 x 32 sums through shared memory, to whole 128-byte lines
+    float* mine = stage_f + warp * 32 * 33;
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (i0 + c0 + j < a.c) out[j] = acc[j];
-    }
+    for (int j = 0; j < 32; ++j) mine[lane * 33 + j] = acc[j];
+    __syncwarp();
+    const int o1 = o0 + (warp & 3) * 32, col = i0 + c0 + lane;
+    float* out = a.dw + ((long long)split * a.oc + o1) * a.c + col;
+    if (col < a.c)
+      for (int r = 0; r < min(32, a.oc - o1); ++r) out[(long long)r * a.c] = mine[r * 33 + lane];
   }
   tc_fence_before();
   __syncthreads();
@@ -665,7 +685,7 @@ int choose_splits(long long tiles, long long chunks, int sms) {
   const long long most = std::min<long long>({chunks, std::max<long long>(1, 4LL * sms / tiles), 1024});
   for (long long s = 1; s <= most; ++s) {
     const double rounds = (double)((tiles * s + sms - 1) / sms);
-    const double t = rounds * ((double)((chunks + s - 1) / s) + 4.0) + (s > 1 ? 2.0 : 0.0);
+    const double t = rounds * ((double)((chunks + s - 1) / s) + 8.0) + (s > 1 ? 2.0 : 0.0);
     if (t < cost) cost = t, best = s;
   }
   return (int)best;
