@@ -15,15 +15,17 @@ struct FwdArgs {
   zjai_residual_tapes tp;
 };
 
-// Rows held, vector accesses, the next tile copied ahead into the other of two slots.
-template <class T>
+// Rows held, the next tile copied ahead into the other of two slots.
+template <int kMode, class T>
 constexpr int fwd_slot_bytes() {  // per thread: f, x and the gate's logits
-  return 3 * kStagedRows * 4 * (int)sizeof(T);
+  return 3 * kStagedRows * Place<kMode, T>::kBytes;
 }
-template <bool kWhole, class T>
+template <int kMode, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
     residual_norm_staged_kernel(const FwdArgs<T> a) {
-  constexpr int kRows = kStagedRows, kBytes = 4 * sizeof(T);
+  using P = Place<kMode, T>;
+  constexpr int kRows = kStagedRows;
+  constexpr bool kWhole = kMode == kWholeTiles, kVec = kMode != kAnywhere;
   __shared__ Exchange<2, 2> ex;
   __shared__ Params<kRows> prm;
   extern __shared__ __align__(16) char slots[];
@@ -32,19 +34,20 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
-  const StagedRows<kWhole> row(a.c, a.p, groups);
+  const StagedRows<kMode> row(a.c, a.p, groups);
   auto place = [&](int slot, int k, int j) {
-    return slots + ((slot * 3 + k) * kRows + j) * (int)blockDim.x * kBytes + threadIdx.x * kBytes;
+    return slots + ((slot * 3 + k) * kRows + j) * (int)blockDim.x * P::kBytes + threadIdx.x * P::kBytes;
   };
+  const long long elems = a.tiles / groups * a.c * a.p;
   auto copy = [&](const Tiles& t, int slot) {
     const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
-    const bool in = kWhole || t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    const int nv = kWhole ? 4 : a.p - (t.g * kTapeGroup + (lane & 7) * 4);
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const bool on = in && row.on(j);
-      stage_copy<kBytes>(place(slot, 0, j), a.f + e + row.e(j), on);
-      stage_copy<kBytes>(place(slot, 1, j), a.x + e + row.e(j), on);
-      if (per_row) stage_copy<kBytes>(place(slot, 2, j), a.gate + e + row.e(j), on);
+      const bool on = row.on(j);
+      P::copy(place(slot, 0, j), a.f + e + row.e(j), on, nv, a.f + elems);
+      P::copy(place(slot, 1, j), a.x + e + row.e(j), on, nv, a.x + elems);
+      if (per_row) P::copy(place(slot, 2, j), a.gate + e + row.e(j), on, nv, a.gate + elems);
     }
   };
   prm.load(a.prm, a.c);
@@ -57,47 +60,50 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     if (ahead.on()) copy(ahead, slot ^ 1);
     stage_commit();
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
-    const bool in = kWhole || at < a.p;
+    const int nv = kWhole ? 4 : a.p - at;
     const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
     const long long x0 = (long long)tile.img * a.c * groups + tile.g;
     F4 gate1 = all(0.f), sg1 = all(1.f), unused;
     if (a.gate_c == 1) {
-      gate1 = load4<true>(a.gate + (long long)tile.img * a.p, at, a.p);
+      gate1 = load4<kVec>(a.gate + (long long)tile.img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
     }
     stage_wait<1>();
     auto hold = [&](const zjai_tape& t, int j, F4 v) {
-      tape_hold4(t.codes + e0 + row.e(j), t.exps + x0 + row.x(j), v, row.on(j), in);
+      tape_hold4<kVec>(t.codes + e0 + row.e(j), t.exps + x0 + row.x(j), v, row.on(j), nv);
     };
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
-      stats_part(rows, v, ex, 0, warps);
+      stats_part(rows, v, ex, 0);
       __syncthreads();
       stats_join(rows, ex, 0, inv_c, warps, wp, warps);
       __syncthreads();
       nm = total4(ex, 0);
       r = total4(ex, 1);
     };
-    if (post) exchange([&](int j) { return staged4<T>(place(slot, 0, j)); });
+    auto get = [&](const T* map, int k, int j) {
+      return P::get(place(slot, k, j), map + e0 + row.e(j), nv);
+    };
+    if (post) exchange([&](int j) { return get(a.f, 0, j); });
     if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
-      tape_store4<true>(a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g,
+      tape_store4<kVec>(a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g,
                         at, a.p, gate1, lane < 8);
     F4 y[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const F4 f = staged4<T>(place(slot, 0, j));
+      const F4 f = get(a.f, 0, j);
       F4 u = f, s = sg1;
       if (post)
         u = fma4((f + nm) * r, prm.get(a.prm, kPostW, row.ch(j)), prm.get(a.prm, kPostB, row.ch(j)));
       if (a.tp.f.codes) hold(a.tp.f, j, f);
       if (per_row) {
-        const F4 g = staged4<T>(place(slot, 2, j));
+        const F4 g = get(a.gate, 2, j);
         sigmoid4(g, &s, &unused);
         if (a.tp.gate.codes) hold(a.tp.gate, j, g);
       }
-      y[j] = fma4(s * prm.get(a.prm, kScale, row.ch(j)), u, staged4<T>(place(slot, 1, j)));
-      if (in && row.on(j)) store4_in(a.y + e0 + row.e(j), y[j]);
-      if (a.tp.y.codes) hold(a.tp.y, j, in ? y[j] : all(0.f));
+      y[j] = fma4(s * prm.get(a.prm, kScale, row.ch(j)), u, get(a.x, 1, j));
+      staged_store<kMode>(a.y + e0 + row.e(j), y[j], row.on(j), nv);
+      if (a.tp.y.codes) hold(a.tp.y, j, kWhole ? y[j] : clip4<kVec>(y[j], at, a.p));
     }
     if (!pre) continue;
     exchange([&](int j) { return y[j]; });
@@ -105,96 +111,74 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     for (int j = 0; j < kRows; ++j) {
       const F4 z =
           fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row.ch(j)), prm.get(a.prm, kPreB, row.ch(j)));
-      if (in && row.on(j)) store4_in(a.z + e0 + row.e(j), z);
-      if (a.tp.z.codes) hold(a.tp.z, j, in ? z : all(0.f));
+      staged_store<kMode>(a.z + e0 + row.e(j), z, row.on(j), nv);
+      if (a.tp.z.codes) hold(a.tp.z, j, kWhole ? z : clip4<kVec>(z, at, a.p));
     }
   }
 }
 
-template <int kRows, bool kVec, class T>
+// Any channel count and alignment: rows are read again for each pass.
+template <bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const FwdArgs<T> a) {
+  constexpr int kRows = 0;
   __shared__ Exchange<2, 2> ex;
   __shared__ Params<kRows> prm;
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Rows<kRows> rows(a.c, warps);
-  constexpr int kHeld = kRows ? kRows : 1;
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
-  prm.load(a.prm, a.c);
-  __syncthreads();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const long long img = tile / groups, base = img * a.c;
     const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
     // a row's first element; its group's place among the exponents
     auto e0 = [&](int j) { return (base + rows.row(j)) * a.p; };
     auto ge = [&](int j) { return (base + rows.row(j)) * groups + g; };
-    F4 f[kHeld], x[kHeld], q[kHeld];  // branch, input (then y), gate logits
     auto load = [&](const T* v, int j) {
       return rows.on(j) ? load4<kVec>(v + e0(j), at, a.p) : all(0.f);
     };
-    if (kRows) {
-      FOR_ROWS(j) f[j % kHeld] = load(a.f, j);
-      FOR_ROWS(j) x[j % kHeld] = load(a.x, j);
-      if (per_row) FOR_ROWS(j) q[j % kHeld] = load(a.gate, j);
-    }
-    auto f_of = [&](int j) { return kRows ? f[j % kHeld] : load(a.f, j); };
-    auto gate_of = [&](int j) { return kRows ? q[j % kHeld] : load(a.gate, j); };
     F4 gate1 = all(0.f), sg1 = all(1.f), unused;
     if (a.gate_c == 1) {
       gate1 = load4<kVec>(a.gate + img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
+      if (a.tp.gate.codes && wp == 0)
+        tape_store4<kVec>(a.tp.gate, img * a.p, img * groups + g, at, a.p, gate1, lane < 8);
     }
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
-      stats_part(rows, v, ex, 0, warps);
+      stats_part(rows, v, ex, 0);
       __syncthreads();
       stats_join(rows, ex, 0, inv_c, warps, wp, warps);
       __syncthreads();
       nm = total4(ex, 0);
       r = total4(ex, 1);
     };
-    if (post) exchange(f_of);
+    if (post) exchange([&](int j) { return load(a.f, j); });
     const F4 nm1 = nm, r1 = r;
     auto y_of = [&](int j) {
       const int ch = rows.param(j);
-      F4 u = f_of(j), s = sg1;
+      F4 u = load(a.f, j), s = sg1;
       if (post)
         u = fma4((u + nm1) * r1, prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch));
-      if (per_row) sigmoid4(gate_of(j), &s, &unused);
-      return fma4(s * prm.get(a.prm, kScale, ch), u, kRows ? x[j % kHeld] : load(a.x, j));
+      if (per_row) sigmoid4(load(a.gate, j), &s, &unused);
+      return fma4(s * prm.get(a.prm, kScale, ch), u, load(a.x, j));
     };
-    // y and the tapes of f, gate and y (whole warps call)
-    auto emit = [&](int j, F4 y) {
+    if (pre) exchange(y_of);
+    FOR_ROWS(j) {
       const bool on = rows.on(j);
+      const F4 y = y_of(j);
       if (on) store4<kVec>(a.y + e0(j), at, a.p, y);
-      if (a.tp.f.codes) tape_store4<kVec>(a.tp.f, e0(j), ge(j), at, a.p, f_of(j), on);
+      if (a.tp.f.codes) tape_store4<kVec>(a.tp.f, e0(j), ge(j), at, a.p, load(a.f, j), on);
       if (per_row && a.tp.gate.codes)
-        tape_store4<kVec>(a.tp.gate, e0(j), ge(j), at, a.p, gate_of(j), on);
+        tape_store4<kVec>(a.tp.gate, e0(j), ge(j), at, a.p, load(a.gate, j), on);
       if (a.tp.y.codes)
         tape_store4<kVec>(a.tp.y, e0(j), ge(j), at, a.p, clip4<kVec>(y, at, a.p), on);
-    };
-    if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
-      tape_store4<kVec>(a.tp.gate, img * a.p, img * groups + g, at, a.p, gate1, lane < 8);
-    if (kRows) {
-      FOR_ROWS(j) {
-        const F4 y = y_of(j);
-        emit(j, y);
-        x[j % kHeld] = y;
-      }
-    }
-    auto done_y = [&](int j) { return kRows ? x[j % kHeld] : y_of(j); };
-    if (pre) exchange(done_y);
-    if (kRows && !pre) continue;
-    FOR_ROWS(j) {
-      const F4 y = done_y(j);
-      if (!kRows) emit(j, y);
       if (!pre) continue;
       const int ch = rows.param(j);
       const F4 z = fma4((y + nm) * r, prm.get(a.prm, kPreW, ch), prm.get(a.prm, kPreB, ch));
-      if (rows.on(j)) store4<kVec>(a.z + e0(j), at, a.p, z);
+      if (on) store4<kVec>(a.z + e0(j), at, a.p, z);
       if (a.tp.z.codes)
-        tape_store4<kVec>(a.tp.z, e0(j), ge(j), at, a.p, clip4<kVec>(z, at, a.p), rows.on(j));
+        tape_store4<kVec>(a.tp.z, e0(j), ge(j), at, a.p, clip4<kVec>(z, at, a.p), on);
     }
   }
 }
@@ -251,26 +235,26 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
     VecCheck vec(p);
     vec.map(dx, es).map(df, es).map(dg, es).map(dyo, es).map(dzo, es);
     for (zjai_tape* t : tt) vec.map(t->codes, 1);
-    const Shape sh = shape_of(c, p, vec.ok, false);
+    const Shape sh = shape_of(c, p, vec.ok, vec.words);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
       FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
                       (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
       const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
-      if (sh.staged) {
-        auto k = sh.whole ? residual_norm_staged_kernel<true, T>
-                          : residual_norm_staged_kernel<false, T>;
-        const int smem = 2 * fwd_slot_bytes<T>() * sh.warps * 32;
+      void (*k)(FwdArgs<T>) = vec.ok ? residual_norm_kernel<true, T> : residual_norm_kernel<false, T>;
+      int smem = 0;
+      if (sh.mode >= 0) {
+        smem = by_mode(sh.mode, [&](auto m) {
+          constexpr int kMode = decltype(m)::value;
+          k = residual_norm_staged_kernel<kMode, T>;
+          return 2 * fwd_slot_bytes<kMode, T>() * sh.warps * 32;
+        });
         ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                            "gated_residual_norm"));
-        k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
-        return cuda_check(cudaGetLastError(), "gated_residual_norm");
+                            me));
       }
-      auto k = sh.rows ? residual_norm_kernel<kStagedRows, false, T>
-               : vec.ok ? residual_norm_kernel<0, true, T> : residual_norm_kernel<0, false, T>;
-      k<<<blocks, sh.warps * 32, 0, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), "gated_residual_norm");
+      k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
+      return cuda_check(cudaGetLastError(), me);
     }));
     ctx->launches++;
     ZJAI_TRY(finish_bytes_out(ctx, y, dyo, bytes, mem));

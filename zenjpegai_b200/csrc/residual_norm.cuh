@@ -33,6 +33,7 @@ namespace {
 constexpr float kEps = 1e-5f;
 constexpr int kMaxC = 8192;  // the parameter sums of a block sit in shared memory, 20 B a channel
 constexpr int kMaxWarps = 16;
+constexpr int kStagedRows = 4;  // rows a thread holds
 
 // sigmoid(g) and sigmoid(g) (1 - sigmoid(g)), an even function of g: with a = exp(-|g|) and
 // r = 1 / (1 + a), sigmoid is r or a r and the product a r^2, nothing by cancellation and both finite
@@ -78,27 +79,23 @@ struct Exchange {
   float part[kVals][kMaxWarps][32], total[kTotals][32];
 };
 
-// Rows of the calling thread: row(j) for j < rows(). kRows > 0: held in registers, consecutive
-// groups of four per warp; 0: any number, strided over the block. kAll: all rows exist.
+// Rows of the calling thread: row(j) for j < n, a warp's consecutive groups of four. kRows > 0: as
+// many, held; 0: as many as c takes. kAll: all rows exist. The same rows to the same warps either way
+// (up to 256 channels), so that results do not depend on alignment.
 template <int kRows, bool kAll = false>
 struct Rows {
-  int c, first, step, n;
+  int c, first, n;
   __device__ __forceinline__ Rows(int c_, int warps) : c(c_) {
-    const int wp = threadIdx.x >> 5, rg = (threadIdx.x & 31) >> 3;
-    first = wp * 4 * (kRows ? kRows : 1) + rg;
-    step = kRows ? 4 : 4 * warps;
-    n = kRows ? kRows : (c + step - 1) / step;
+    n = kRows ? kRows : max(kStagedRows, (c + 4 * warps - 1) / (4 * warps));
+    first = (threadIdx.x >> 5) * 4 * n + ((threadIdx.x & 31) >> 3);
   }
-  __device__ __forceinline__ int row(int j) const { return first + j * step; }
+  __device__ __forceinline__ int row(int j) const { return first + j * 4; }
   __device__ __forceinline__ bool on(int j) const { return kAll || row(j) < c; }
   // a row that exists, to read for one that does not
   __device__ __forceinline__ int param(int j) const { return min(row(j), c - 1); }
   // rows of a warp
-  __device__ __forceinline__ int of_warp(int w, int warps) const {
-    if (kAll) return 4 * kRows;
-    if (kRows) return max(0, min(c - w * 4 * kRows, 4 * kRows));
-    const int whole = c / (4 * warps);
-    return whole * 4 + max(0, min(4, c - whole * 4 * warps - w * 4));
+  __device__ __forceinline__ int of_warp(int w) const {
+    return kAll ? 4 * kRows : max(0, min(c - w * 4 * n, 4 * n));
   }
 };
 #define FOR_ROWS(j) _Pragma("unroll") for (int j = 0; j < (kRows ? kRows : rows.n); ++j)
@@ -106,13 +103,12 @@ struct Rows {
 // Per warp the sum and the squared deviations from the warp's own mean of v(j), to ex.part at val,
 // val + 1.
 template <int kRows, bool kAll, class V, class E>
-__device__ __forceinline__ void stats_part(const Rows<kRows, kAll>& rows, V&& v, E& ex, int val,
-                                           int warps) {
+__device__ __forceinline__ void stats_part(const Rows<kRows, kAll>& rows, V&& v, E& ex, int val) {
   const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   F4 s = all(0.f), q = all(0.f);
   FOR_ROWS(j) if (rows.on(j)) s = s + v(j);
   s = over_rows(s);
-  const int n = rows.of_warp(wp, warps);
+  const int n = rows.of_warp(wp);
   const F4 nm = s * all(kAll ? -1.f / (4 * kRows) : n ? __fdividef(-1.f, (float)n) : 0.f);
   FOR_ROWS(j) if (rows.on(j)) {
     const F4 d = v(j) + nm;
@@ -145,14 +141,15 @@ __device__ __forceinline__ void stats_join(const Rows<kRows, kAll>& rows, E& ex,
       s[i] = w < warps ? ex.part[val][w][pos] : 0.f;
       sum += s[i];
     }
-    const float m = over_subs(sum) * inv_c;
+    // products rounded on their own: the same bits wherever this is compiled in
+    const float m = __fmul_rn(over_subs(sum), inv_c);
 #pragma unroll
     for (int i = 0; i < kMaxWarps / 4; ++i) {
-      const int w = i * 4 + sub, n = w < warps ? rows.of_warp(w, warps) : 0;
+      const int w = i * 4 + sub, n = w < warps ? rows.of_warp(w) : 0;
       if (n) {
         // (whole warps: by a constant)
-        const float d = (kAll ? s[i] * (1.f / (4 * kRows)) : __fdividef(s[i], (float)n)) - m;
-        q += fmaf((float)n * d, d, ex.part[val + 1][w][pos]);
+        const float d = __fsub_rn(kAll ? __fmul_rn(s[i], 1.f / (4 * kRows)) : __fdividef(s[i], (float)n), m);
+        q = __fadd_rn(q, fmaf(__fmul_rn((float)n, d), d, ex.part[val + 1][w][pos]));
       }
     }
     q = over_subs(q);
@@ -231,20 +228,14 @@ struct Tiles {
   }
 };
 
-// Staged loads (rows held, vector accesses): a thread copies what it will itself read of the next
-// tile to its own places in shared memory (cp.async, no thread waits for another) while it works on
-// the current one. A place is four positions of a row, of kBytes.
-template <int kBytes>
-__device__ __forceinline__ void stage_copy(char* dst, const void* src, bool on) {
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(on ? 16 : 0)
-                 : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(kBytes),
-                 "r"(on ? kBytes : 0)
-                 : "memory");
-}
+// Staged loads (rows held): a thread copies what it will itself read of the next tile to its own
+// places in shared memory (cp.async, no thread waits for another) while it works on the current one.
+// A place holds four positions of a row. By alignment:
+//   kWholeTiles: a multiple of 16 channels and of 32 positions, all aligned: no bounds to check;
+//   kAligned: rows of a multiple of four positions on aligned bases: all four in the row or behind;
+//   kAnywhere: rows start anywhere, on bases of whole words: f32 comes one by one, f16 and bf16 as
+//     the three words and codes as the two words that hold the four, shifted into place when read.
+enum { kWholeTiles, kAligned, kAnywhere };
 // the first `bytes` (1 to 4) of an aligned word, zeros behind them
 __device__ __forceinline__ void stage_copy_some(char* dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
@@ -259,19 +250,84 @@ template <int kNewer>
 __device__ __forceinline__ void stage_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kNewer) : "memory");
 }
-template <class T>
-__device__ __forceinline__ F4 staged4(const char* src) {
-  if constexpr (sizeof(T) == 4)
-    return make4(*reinterpret_cast<const float4*>(src));
+template <int kBytes>
+__device__ __forceinline__ void stage_copy_all(char* dst, const void* src, bool on) {
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
   else
-    return halves4<T>(*reinterpret_cast<const uint2*>(src));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(kBytes),
+                 "r"(on ? kBytes : 0)
+                 : "memory");
 }
+// Places of E (float, __half, __nv_bfloat16, or int8_t for codes): bytes, copies and reads. on: the
+// row exists; nv: how many of the four positions lie in it; end: behind the tensor's last element.
+template <int kMode, class E>
+struct Place {
+  static constexpr int kSize = (int)sizeof(E);
+  static constexpr int kBytes =
+      kMode != kAnywhere || kSize == 4 ? 4 * kSize : kSize == 2 ? 16 : 8;
+  static __device__ __forceinline__ void copy(char* dst, const E* src, bool on, int nv,
+                                              const E* end) {
+    if constexpr (kMode != kAnywhere) {
+      stage_copy_all<4 * kSize>(dst, src, kMode == kWholeTiles || (on && nv > 0));
+    } else if constexpr (kSize == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) stage_copy_some(dst + 4 * i, src + i, on && i < nv ? 4 : 0);
+    } else {
+      const char* a = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)3);
+      const long long left = reinterpret_cast<const char*>(end) - a;
+      const int l = on ? (int)min(left, 12LL) : 0;
+#pragma unroll
+      for (int j = 0; j < (kSize == 2 ? 3 : 2); ++j)
+        stage_copy_some(dst + 4 * j, a + 4 * j, max(0, min(4, l - 4 * j)));
+    }
+  }
+  // two words (halves) or one (codes) in place; src: where it was copied from
+  static __device__ __forceinline__ uint2 words(const char* q, const E* src, int nv) {
+    if constexpr (kMode != kAnywhere) {
+      if constexpr (kSize == 2) return *reinterpret_cast<const uint2*>(q);
+      else return make_uint2(*reinterpret_cast<const uint32_t*>(q), 0u);
+    } else {
+      const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 3) * 8;
+      if constexpr (kSize == 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(q);
+        const uint32_t lo = nv >= 2 ? ~0u : nv == 1 ? 0xffffu : 0u;
+        const uint32_t hi = nv >= 4 ? ~0u : nv == 3 ? 0xffffu : 0u;
+        return make_uint2(__funnelshift_r(w.x, w.y, sh) & lo, __funnelshift_r(w.y, w.z, sh) & hi);
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(q);
+        const uint32_t in = nv >= 4 ? ~0u : nv <= 0 ? 0u : ~0u >> (32 - 8 * nv);
+        return make_uint2(__funnelshift_r(w.x, w.y, sh) & in, 0u);
+      }
+    }
+  }
+  static __device__ __forceinline__ F4 get(const char* q, const E* src, int nv) {
+    if constexpr (kSize == 4)
+      return make4(*reinterpret_cast<const float4*>(q));
+    else
+      return halves4<E>(words(q, src, nv));
+  }
+};
+// four positions of a row to q, nv of them in the row
+template <int kMode, class T>
+__device__ __forceinline__ void staged_store(T* q, F4 v, bool on, int nv) {
+  if constexpr (kMode == kWholeTiles) {
+    store4_in(q, v);
+  } else if constexpr (kMode == kAligned) {
+    if (on && nv > 0) store4_in(q, v);
+  } else {
+    if (on) store4<false>(q, 0, nv, v);
+  }
+}
+
 // The rows of the calling thread in a picture: their offsets from the picture's first element, with
 // the lane's four positions, and of their exponents from the picture's first (held rows: 32 bits
-// do). kWhole: a multiple of 16 channels and of 32 positions, every row and position there.
-constexpr int kStagedRows = 4;
-template <bool kWhole>
+// do).
+template <int kMode>
 struct StagedRows {
+  static constexpr bool kWhole = kMode == kWholeTiles;
   uint32_t e0, x0, e4, x4;
   int ch0, c;
   __device__ __forceinline__ StagedRows(int c_, int p, int groups) : c(c_) {
@@ -304,30 +360,38 @@ int stage_params(Ctx* ctx, const zjai_residual_params& in, int c, int mem,
   return stage_param(ctx, in.pre_bias, c, mem, "pre_bias", &out->pre_bias);
 }
 
-// How c channels at p positions are taken. staged: rows held and copied ahead, where vector accesses
-// are possible; else kRows rows of a thread held in registers, or (0) read again. Sixteen warps an
-// SM are resident at the registers that __launch_bounds__ leaves, so blocks of few warps come in
-// numbers.
+// How c channels at p positions are taken: staged (rows held) in a mode, or read again for each
+// pass (mode -1). Sixteen warps an SM are resident at the registers that __launch_bounds__ leaves,
+// so blocks of few warps come in numbers.
 struct Shape {
-  bool staged, whole;
-  int rows, warps, per_sm;
+  int mode, warps, per_sm;
 };
-Shape shape_of(int c, int p, bool vec, bool backward) {
+Shape shape_of(int c, int p, bool vec, bool words) {
   // held rows are addressed by 32-bit offsets from their picture
   const bool held = c <= kHeldC && (long long)c * p < (1LL << 32) - 64;
-  // without vector accesses the backward pass takes two rows a thread where the warps allow it
-  const int rows = !held ? 0 : !vec && backward && c <= kHeldC / 2 ? 2 : kStagedRows;
-  const int warps = rows ? (c + 4 * rows - 1) / (4 * rows) : kMaxWarps;
-  return {held && vec, c % (4 * kStagedRows) == 0 && p % kTapeGroup == 0, rows, warps,
-          kMaxWarps / warps};
+  const int mode = !held                                                  ? -1
+                   : vec && c % (4 * kStagedRows) == 0 && p % kTapeGroup == 0 ? kWholeTiles
+                   : vec                                                  ? kAligned
+                   : words                                                ? kAnywhere
+                                                                          : -1;
+  const int warps = std::min(kMaxWarps, (c + 4 * kStagedRows - 1) / (4 * kStagedRows));
+  return {mode, warps, kMaxWarps / warps};
 }
-// Four neighbouring positions can be loaded and stored at once: rows of a multiple of four
-// positions, maps aligned to four elements and codes to four bytes.
+// f(std::integral_constant) with a staged mode
+template <class F>
+auto by_mode(int mode, F&& f) {
+  if (mode == kWholeTiles) return f(std::integral_constant<int, kWholeTiles>());
+  if (mode == kAligned) return f(std::integral_constant<int, kAligned>());
+  return f(std::integral_constant<int, kAnywhere>());
+}
+// ok: four neighbouring positions can be loaded and stored at once (rows of a multiple of four
+// positions, maps aligned to four elements and codes to four bytes); words: all on whole words.
 struct VecCheck {
-  bool ok;
+  bool ok, words = true;
   explicit VecCheck(int p) : ok(p % 4 == 0) {}
   VecCheck& map(const void* q, size_t es) {
     ok = ok && reinterpret_cast<uintptr_t>(q) % (4 * es) == 0;
+    words = words && reinterpret_cast<uintptr_t>(q) % 4 == 0;
     return *this;
   }
 };

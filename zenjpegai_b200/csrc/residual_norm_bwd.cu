@@ -38,22 +38,25 @@ struct Kept<true, kVec, T> {
   __device__ __forceinline__ F4 get() const { return taped4(w, e); }
 };
 
-// Rows held, vector accesses, the next tile copied ahead. Per thread a slot has dy, dz, and f, y and
-// the gate as they were kept. Two slots where 16 warps' fit the SM's shared memory; with one (f32
-// maps) the next tile is copied as soon as the current one has been read, before its last exchange.
+// Rows held, the next tile copied ahead. Per thread a slot has dy, dz, and f, y and the gate as they
+// were kept. Two slots where 16 warps' fit the SM's shared memory; with one the next tile is copied
+// as soon as the current one has been read.
 // The parameter gradients are summed over a block's tiles in registers, written out per block.
-template <bool kTaped, class T>
+template <int kMode, bool kTaped, class T>
 struct BwdSlot {
-  static constexpr int kGrad = 4 * sizeof(T), kKept = kTaped ? 4 : 4 * sizeof(T);
+  using Grad = Place<kMode, T>;
+  using Kept = Place<kMode, typename std::conditional<kTaped, int8_t, T>::type>;
+  static constexpr int kGrad = Grad::kBytes, kKept = Kept::kBytes;
   static constexpr int kBytes = kStagedRows * (2 * kGrad + 3 * kKept);  // per thread
   static constexpr int kExps = kTaped ? 3 * kStagedRows * 4 / 8 : 0;  // per thread, words of rows
   static constexpr int kB = sizeof(T) == 4 ? 0 : kStagedRows * (int)sizeof(float4);
   static constexpr int kSlots = 2 * kBytes * kThreadsMost <= 180 * 1024 ? 2 : 1;
 };
-template <bool kWhole, bool kTaped, class T>
+template <int kMode, bool kTaped, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
     residual_norm_bwd_staged_kernel(const BwdArgs<T> a) {
-  using S = BwdSlot<kTaped, T>;
+  using S = BwdSlot<kMode, kTaped, T>;
+  constexpr bool kWhole = kMode == kWholeTiles, kVec = kMode != kAnywhere;
   constexpr int kRows = kStagedRows;
   __shared__ Exchange<4, 9> ex;  // totals: f 0, 1, y 2, 3, a 4, 5, b 6, 7, gate 8
   __shared__ Params<kRows> prm;
@@ -72,7 +75,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   auto join_second = [&](auto f) {
     if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
   };
-  const StagedRows<kWhole> row(a.c, a.p, groups);
+  const StagedRows<kMode> row(a.c, a.p, groups);
   auto grad_at = [&](int slot, int k, int j) {
     return slots + slot * S::kBytes * (int)blockDim.x +
            ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kGrad;
@@ -95,11 +98,11 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
                        : q + (j * (int)blockDim.x + (int)threadIdx.x) * (int)sizeof(float4));
   };
   // exponents of the whole map (the gate's too: this path takes its own rows only where it has c)
-  const long long x_all = a.tiles * a.c;
+  const long long x_all = a.tiles * a.c, elems = a.tiles / groups * a.c * a.p;
   auto copy = [&](const Tiles& t, int slot) {
     const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
     const long long x = (long long)t.img * a.c * groups + t.g;
-    const bool in = kWhole || t.g * kTapeGroup + (lane & 7) * 4 < a.p;
+    const int nv = kWhole ? 4 : a.p - (t.g * kTapeGroup + (lane & 7) * 4);
     auto keep_exps = [&](const zjai_tape& tp, int k) {
       const int ch = wp * kWarpRows + lane;
       if (lane >= kWarpRows || (!kWhole && ch >= a.c)) return;
@@ -114,30 +117,22 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       if (pre) keep_exps(a.tp.y, 1);
       if (per_row) keep_exps(a.tp.gate, 2);
     }
-    auto keep = [&](const T* map, const zjai_tape& tp, int k, int j, bool on) {
-      if constexpr (kTaped) {
-        stage_copy<4>(kept_at(slot, k, j), tp.codes + e + row.e(j), on);
-      } else {
-        stage_copy<S::kKept>(kept_at(slot, k, j), map + e + row.e(j), on);
-      }
+    auto keep = [&](const T* map, const zjai_tape& tp, int k, int j) {
+      if constexpr (kTaped)
+        S::Kept::copy(kept_at(slot, k, j), tp.codes + e + row.e(j), row.on(j), nv, tp.codes + elems);
+      else
+        S::Kept::copy(kept_at(slot, k, j), map + e + row.e(j), row.on(j), nv, map + elems);
+    };
+    auto grad = [&](const T* map, int k, int j) {
+      S::Grad::copy(grad_at(slot, k, j), map + e + row.e(j), row.on(j), nv, map + elems);
     };
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const bool on = in && row.on(j);
-      if (need_f) keep(a.f, a.tp.f, 0, j, on);
-      if (pre) keep(a.y, a.tp.y, 1, j, on);
-      if (pre) stage_copy<S::kGrad>(grad_at(slot, 1, j), a.dz + e + row.e(j), on);
-      if (per_row) keep(a.gate, a.tp.gate, 2, j, on);
-      stage_copy<S::kGrad>(grad_at(slot, 0, j), a.dy + e + row.e(j), on);
-    }
-  };
-  auto kept = [&](int slot, int k, int j, uint32_t x) {
-    if constexpr (kTaped) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j * 4 + (lane >> 3)));
-      const int e = (int)(int8_t)(w >> ((x + row.x(j)) & 3) * 8);
-      return taped4(*reinterpret_cast<const uint32_t*>(kept_at(slot, k, j)), e);
-    } else {
-      return staged4<T>(kept_at(slot, k, j));
+      if (need_f) keep(a.f, a.tp.f, 0, j);
+      if (pre) keep(a.y, a.tp.y, 1, j);
+      if (pre) grad(a.dz, 1, j);
+      if (per_row) keep(a.gate, a.tp.gate, 2, j);
+      grad(a.dy, 0, j);
     }
   };
   float acc[kRows][5];
@@ -152,12 +147,24 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   stage_commit();
   for (int slot = 0; tile.on(); tile.next(), slot ^= S::kSlots - 1) {
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
-    const bool in = kWhole || at < a.p;
+    const int nv = kWhole ? 4 : a.p - at;
     const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
     const uint32_t x0 = (uint32_t)((long long)tile.img * a.c * groups + tile.g);
+    auto kept = [&](const T* map, const zjai_tape& tp, int k, int j) {
+      if constexpr (kTaped) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j * 4 + (lane >> 3)));
+        const int e = (int)(int8_t)(w >> ((x0 + row.x(j)) & 3) * 8);
+        return taped4(S::Kept::words(kept_at(slot, k, j), tp.codes + e0 + row.e(j), nv).x, e);
+      } else {
+        return S::Kept::get(kept_at(slot, k, j), map + e0 + row.e(j), nv);
+      }
+    };
+    auto grad = [&](const T* map, int k, int j) {
+      return S::Grad::get(grad_at(slot, k, j), map + e0 + row.e(j), nv);
+    };
     F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
-      Kept<kTaped, true, T> k;
+      Kept<kTaped, kVec, T> k;
       k.load(a.gate, a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g, at,
              a.p);
       sigmoid4(k.get(), &sg1, &slope1);
@@ -172,12 +179,12 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     F4 f[kRows], y[kRows];  // then LN(f), LN(y)
     if (need_f)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) f[j] = kept(slot, 0, j, x0);
+      for (int j = 0; j < kRows; ++j) f[j] = kept(a.f, a.tp.f, 0, j);
     if (pre)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) y[j] = kept(slot, 1, j, x0);
-    if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0, warps);
-    if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2, warps);
+      for (int j = 0; j < kRows; ++j) y[j] = kept(a.y, a.tp.y, 1, j);
+    if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0);
+    if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2);
     if (post || pre) {
       __syncthreads();
       if (post) join_first([&](int n, int of) { stats_join(rows, ex, 0, inv_c, warps, n, of); });
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         y[j] = (y[j] + nm) * r2;
-        const F4 t = staged4<T>(grad_at(slot, 1, j)) * prm.get(a.prm, kPreW, row.ch(j));
+        const F4 t = grad(a.dz, 1, j) * prm.get(a.prm, kPreW, row.ch(j));
         if (row.on(j)) {
           s0 = s0 + t;
           s1 = fma4(t, y[j], s1);
@@ -216,23 +223,23 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       const int ch = row.ch(j);
-      const bool on = row.on(j), write = on && in;
-      F4 d = staged4<T>(grad_at(slot, 0, j));
+      const bool on = row.on(j);
+      F4 d = grad(a.dy, 0, j);
       if (pre) {
-        const F4 dz = staged4<T>(grad_at(slot, 1, j));
+        const F4 dz = grad(a.dz, 1, j);
         acc[j][3] += dot4(dz, y[j]);
         acc[j][4] += sum4(dz);
         d = fma4(fma4(y[j], ay, dz * prm.get(a.prm, kPreW, ch) + am), r2, d);
       }
-      if (write) store4_in(a.dx + e0 + row.e(j), d);
+      staged_store<kMode>(a.dx + e0 + row.e(j), d, on, nv);
       if (!need_f) continue;
       const F4 u = post ? fma4(f[j], prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch)) : f[j];
       const F4 ds = d * prm.get(a.prm, kScale, ch);
       F4 sg = sg1, du = ds;
       if (per_row) {
         F4 slope;
-        sigmoid4(kept(slot, 2, j, x0), &sg, &slope);
-        if (write) store4_in(a.dgate + e0 + row.e(j), ds * u * slope);
+        sigmoid4(kept(a.gate, a.tp.gate, 2, j), &sg, &slope);
+        staged_store<kMode>(a.dgate + e0 + row.e(j), ds * u * slope, on, nv);
       }
       if (a.gate_c) du = ds * sg;
       acc[j][0] += dot4(d * sg, u);
@@ -246,20 +253,18 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
           t0 = t0 + b;
           t1 = fma4(b, f[j], t1);
         }
-      } else if (write) {
-        store4_in(a.df + e0 + row.e(j), du);
+      } else {
+        staged_store<kMode>(a.df + e0 + row.e(j), du, on, nv);
       }
     }
     if (!need_f && a.df)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j)
-        if (row.on(j) && in) {
-          F4 d = staged4<T>(grad_at(slot, 0, j));
-          if (pre)
-            d = fma4(fma4(y[j], ay, staged4<T>(grad_at(slot, 1, j)) *
-                                        prm.get(a.prm, kPreW, row.ch(j)) + am), r2, d);
-          store4_in(a.df + e0 + row.e(j), d);
-        }
+      for (int j = 0; j < kRows; ++j) {
+        F4 d = grad(a.dy, 0, j);
+        if (pre)
+          d = fma4(fma4(y[j], ay, grad(a.dz, 1, j) * prm.get(a.prm, kPreW, row.ch(j)) + am), r2, d);
+        staged_store<kMode>(a.df + e0 + row.e(j), d, row.on(j), nv);
+      }
     if (kTaped) __syncwarp();  // exponents read, before another lane copies over them
     // one slot: read now, but for b where dy was
     auto copy_one = [&]() {
@@ -280,13 +285,13 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     if (a.gate_c == 1) sum_join(ex, 2, 8, 1.f, warps, wp, warps);
     __syncthreads();
     if (a.gate_c == 1 && threadIdx.x < 8)
-      store4<true>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 8) * slope1);
+      store4<kVec>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 8) * slope1);
     if (!post) continue;
     const F4 bm = total4(ex, 6), bf = total4(ex, 7), r1 = total4(ex, 1);  // negated means
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      if (row.on(j) && in)
-        store4_in(a.df + e0 + row.e(j), fma4(f[j], bf, make4(*b_at(slot, j)) + bm) * r1);
+      staged_store<kMode>(a.df + e0 + row.e(j), fma4(f[j], bf, make4(*b_at(slot, j)) + bm) * r1,
+                          row.on(j), nv);
     if (sizeof(T) == 4) copy_one();
   }
   stage_wait<0>();
@@ -302,36 +307,21 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     }
 }
 
-// Rows of any alignment, held in registers, or (kRows 0) of any number, read again for each pass:
-// the parameter sums in registers, or per channel in shared memory.
-template <int kRows, bool kTaped, bool kVec, class T>
+// Any channel count and alignment: rows are read again for each pass, the parameter sums per channel
+// in shared memory.
+template <bool kTaped, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(const BwdArgs<T> a) {
+  constexpr int kRows = 0;
   __shared__ Exchange<4, 4> ex;
   __shared__ Params<kRows> prm;
-  extern __shared__ float acc_c[];  // [5][c] where rows are not held
+  extern __shared__ float acc_c[];  // [5][c]
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Rows<kRows> rows(a.c, warps);
-  constexpr int kHeld = kRows ? kRows : 1;
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
   const bool need_f = post || a.gate_c || a.prm.scale;
-  // two sums at a time are joined by four warps each where there are eight
-  const bool two = warps >= 8;
-  auto join_first = [&](auto f) {
-    if (!two || wp < 4) f(two ? wp : wp, two ? 4 : warps);
-  };
-  auto join_second = [&](auto f) {
-    if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
-  };
-  float acc[kHeld][5];
-#pragma unroll
-  for (int j = 0; j < kHeld; ++j)
-#pragma unroll
-    for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
-  if (!kRows)
-    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
-  prm.load(a.prm, a.c);
+  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
   __syncthreads();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const long long img = tile / groups, base = img * a.c;
@@ -344,24 +334,8 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     auto kept = [&](const T* v, const zjai_tape& t, int j) {
       K k;
       k.load(v, t, e0(j), (base + rows.param(j)) * groups + g, at, a.p);
-      return k;
+      return k.get();
     };
-    // held: f then LN(f), y then LN(y), dy then b, dz, the gate as kept
-    F4 f[kHeld], y[kHeld], dy[kHeld], dz[kHeld];
-    K q[kHeld];
-    if (kRows) {
-      K kf[kHeld], ky[kHeld];
-      if (pre) FOR_ROWS(j) ky[j % kHeld] = kept(a.y, a.tp.y, j);
-      if (need_f) FOR_ROWS(j) kf[j % kHeld] = kept(a.f, a.tp.f, j);
-      if (pre) FOR_ROWS(j) dz[j % kHeld] = grad(a.dz, j);
-      if (per_row) FOR_ROWS(j) q[j % kHeld] = kept(a.gate, a.tp.gate, j);
-      FOR_ROWS(j) dy[j % kHeld] = grad(a.dy, j);
-      if (pre) FOR_ROWS(j) y[j % kHeld] = ky[j % kHeld].get();
-      if (need_f) FOR_ROWS(j) f[j % kHeld] = kf[j % kHeld].get();
-    }
-    auto f_of = [&](int j) { return kRows ? f[j % kHeld] : kept(a.f, a.tp.f, j).get(); };
-    auto y_of = [&](int j) { return kRows ? y[j % kHeld] : kept(a.y, a.tp.y, j).get(); };
-    auto dz_of = [&](int j) { return kRows ? dz[j % kHeld] : grad(a.dz, j); };
     F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
       K k;
@@ -369,49 +343,47 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
       sigmoid4(k.get(), &sg1, &slope1);
     }
     F4 nm1 = all(0.f), r1 = all(1.f), nm2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
-    if (post) stats_part(rows, f_of, ex, 0, warps);
-    if (pre) stats_part(rows, y_of, ex, 2, warps);
+    if (post) stats_part(rows, [&](int j) { return kept(a.f, a.tp.f, j); }, ex, 0);
+    if (pre) stats_part(rows, [&](int j) { return kept(a.y, a.tp.y, j); }, ex, 2);
     if (post || pre) {
       __syncthreads();
-      if (post)
-        join_first([&](int n, int of) { stats_join(rows, ex, 0, inv_c, warps, n, of); });
-      if (pre)
-        join_second([&](int n, int of) { stats_join(rows, ex, 2, inv_c, warps, n, of); });
+      if (post) stats_join(rows, ex, 0, inv_c, warps, wp, warps);
+      if (pre) stats_join(rows, ex, 2, inv_c, warps, wp, warps);
       __syncthreads();
       if (post) nm1 = total4(ex, 0), r1 = total4(ex, 1);
       if (pre) nm2 = total4(ex, 2), r2 = total4(ex, 3);
     }
-    if (kRows && post) FOR_ROWS(j) f[j % kHeld] = (f[j % kHeld] + nm1) * r1;
-    if (kRows && pre) FOR_ROWS(j) y[j % kHeld] = (y[j % kHeld] + nm2) * r2;
-    auto fn_of = [&](int j) { return kRows || !post ? f_of(j) : (f_of(j) + nm1) * r1; };
-    auto yn_of = [&](int j) { return kRows ? y[j % kHeld] : (y_of(j) + nm2) * r2; };
+    auto fn_of = [&](int j) {
+      const F4 f = kept(a.f, a.tp.f, j);
+      return post ? (f + nm1) * r1 : f;
+    };
+    auto yn_of = [&](int j) { return (kept(a.y, a.tp.y, j) + nm2) * r2; };
     if (pre) {
       F4 s0 = all(0.f), s1 = all(0.f);
       FOR_ROWS(j) if (rows.on(j)) {
-        const F4 t = dz_of(j) * prm.get(a.prm, kPreW, rows.param(j));
+        const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, rows.param(j));
         s0 = s0 + t;
         s1 = fma4(t, yn_of(j), s1);
       }
       rows_to_part(s0, ex.part[0][wp]);
       rows_to_part(s1, ex.part[1][wp]);
       __syncthreads();
-      join_first([&](int n, int of) { sum_join(ex, 0, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, 1, -inv_c, warps, n, of); });
+      sum_join(ex, 0, 0, -inv_c, warps, wp, warps);
+      sum_join(ex, 1, 1, -inv_c, warps, wp, warps);
       __syncthreads();
       am = total4(ex, 0);  // negated means
       ay = total4(ex, 1);
     }
-    // of a row: D, D q, and b = D q w1
     auto d_of = [&](int j) {
-      const F4 d = kRows ? dy[j % kHeld] : grad(a.dy, j);
+      const F4 d = grad(a.dy, j);
       if (!pre) return d;
-      const F4 t = dz_of(j) * prm.get(a.prm, kPreW, rows.param(j));
+      const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, rows.param(j));
       return fma4(fma4(yn_of(j), ay, t + am), r2, d);
     };
-    auto gate_of = [&](int j, F4* s, F4* o) {
+    auto gate_of = [&](int j, F4* s, F4* slope) {
       *s = sg1;
-      *o = slope1;
-      if (per_row) sigmoid4((kRows ? q[j % kHeld] : kept(a.gate, a.tp.gate, j)).get(), s, o);
+      *slope = slope1;
+      if (per_row) sigmoid4(kept(a.gate, a.tp.gate, j), s, slope);
     };
     F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
     FOR_ROWS(j) {
@@ -430,29 +402,24 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
         t1 = fma4(b, fn, t1);
         t2 = fma4(ds, u, t2);
       }
-      const F4 dzj = pre ? dz_of(j) : all(0.f);
-      const float v[5] = {sum4(d * sg * u), sum4(du * fn), sum4(du),
-                          pre ? sum4(dzj * yn_of(j)) : 0.f, sum4(dzj)};
+      const F4 dz = pre ? grad(a.dz, j) : all(0.f);
+      const float v[5] = {dot4(d * sg, u), dot4(du, fn), sum4(du), pre ? dot4(dz, yn_of(j)) : 0.f,
+                          sum4(dz)};
 #pragma unroll
       for (int i = 0; i < 5; ++i) {
-        if (kRows) {
-          acc[j % kHeld][i] += v[i];
-        } else {
-          float s = v[i];
+        float s = v[i];
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if ((lane & 7) == 0 && on) acc_c[i * a.c + ch] += s;
-        }
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if ((lane & 7) == 0 && on) acc_c[i * a.c + ch] += s;
       }
-      if (kRows) dy[j % kHeld] = b;
     }
     if (!post && a.gate_c != 1) continue;
     if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
     if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
     __syncthreads();
     if (post) {
-      join_first([&](int n, int of) { sum_join(ex, 0, 0, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, 1, -inv_c, warps, n, of); });
+      sum_join(ex, 0, 0, -inv_c, warps, wp, warps);
+      sum_join(ex, 1, 1, -inv_c, warps, wp, warps);
     }
     if (a.gate_c == 1) sum_join(ex, 2, 2, 1.f, warps, wp, warps);
     __syncthreads();
@@ -461,31 +428,16 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     if (!post) continue;
     const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
     FOR_ROWS(j) if (rows.on(j)) {
-      F4 b = dy[j % kHeld];
-      if (!kRows) {
-        const int ch = rows.param(j);
-        F4 sg, slope;
-        gate_of(j, &sg, &slope);
-        b = d_of(j) * prm.get(a.prm, kScale, ch) * sg * prm.get(a.prm, kPostW, ch);
-      }
+      const int ch = rows.param(j);
+      F4 sg, slope;
+      gate_of(j, &sg, &slope);
+      const F4 b = d_of(j) * prm.get(a.prm, kScale, ch) * sg * prm.get(a.prm, kPostW, ch);
       store4<kVec>(a.df + e0(j), at, a.p, fma4(fn_of(j), bf, b + bm) * r1);
     }
   }
   float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
-  if (kRows) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-#pragma unroll
-      for (int i = 0; i < 5; ++i) {
-        float s = acc[j][i];
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if ((lane & 7) == 0 && rows.on(j)) out[i * a.c + rows.row(j)] = s;
-      }
-  } else {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) out[i] = acc_c[i];
-  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) out[i] = acc_c[i];
 }
 
 struct SumOut {
@@ -590,36 +542,29 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     vec.map(gx, es).map(gf, es).map(gg, es);
     vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
     vec.map(dt.f.exps, 1).map(dt.gate.exps, 1).map(dt.y.exps, 1);
-    const Shape sh = shape_of(c, p, vec.ok, true);
+    const Shape sh = shape_of(c, p, vec.ok, vec.words);
     const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
     float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
     if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
     auto launch = [&](auto t, auto tp) -> int {
       using T = decltype(t);
       constexpr bool kTaped = decltype(tp)::value;
-      using S = BwdSlot<kTaped, T>;
       BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
                       gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
-      void (*k)(BwdArgs<T>) = nullptr;
-      int smem = 0;
-      if (sh.staged) {
-        k = sh.whole ? residual_norm_bwd_staged_kernel<true, kTaped, T>
-                     : residual_norm_bwd_staged_kernel<false, kTaped, T>;
-        smem = (S::kSlots * (S::kBytes + S::kExps) + S::kB) * sh.warps * 32;
-      } else if (sh.rows) {
-        k = sh.rows == 2 ? residual_norm_bwd_kernel<2, kTaped, false, T>
-                         : residual_norm_bwd_kernel<4, kTaped, false, T>;
-      } else {
-        k = vec.ok ? residual_norm_bwd_kernel<0, kTaped, true, T>
-                   : residual_norm_bwd_kernel<0, kTaped, false, T>;
-        smem = 5 * c * (int)sizeof(float);
-      }
-      if (smem)
-        ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                            "gated_residual_norm_backward"));
+      void (*k)(BwdArgs<T>) = vec.ok ? residual_norm_bwd_kernel<kTaped, true, T>
+                                     : residual_norm_bwd_kernel<kTaped, false, T>;
+      int smem = 5 * c * (int)sizeof(float);
+      if (sh.mode >= 0)
+        smem = by_mode(sh.mode, [&](auto m) {
+          using S = BwdSlot<decltype(m)::value, kTaped, T>;
+          k = residual_norm_bwd_staged_kernel<decltype(m)::value, kTaped, T>;
+          return (S::kSlots * (S::kBytes + S::kExps) + S::kB) * sh.warps * 32;
+        });
+      ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                          me));
       k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), "gated_residual_norm_backward");
+      return cuda_check(cudaGetLastError(), me);
     };
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       return taped ? launch(t, std::true_type()) : launch(t, std::false_type());
