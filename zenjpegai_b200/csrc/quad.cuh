@@ -166,24 +166,6 @@ __device__ __forceinline__ void tape_store4(const zjai_tape& t, long long e0, lo
   }
   if ((threadIdx.x & 7) == 0) t.exps[ge] = (int8_t)tape_exp(m);
 }
-// The same where the lane's four codes are at `codes` and the group's exponent at `exp`; nv: how many
-// of the four positions lie in the row.
-template <bool kVec>
-__device__ __forceinline__ void tape_hold4(int8_t* codes, int8_t* exp, F4 v, bool on, int nv) {
-  uint32_t m = amax4(v);
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const uint32_t w = codes4(v, m);
-  if (!on) return;
-  if constexpr (kVec) {
-    if (nv > 0) *reinterpret_cast<uint32_t*>(codes) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < nv) codes[i] = (int8_t)(w >> (8 * i) & 0xffu);
-  }
-  if ((threadIdx.x & 7) == 0) *exp = (int8_t)tape_exp(m);
-}
 // value of positions behind the row's end set to zero
 template <bool kVec>
 __device__ __forceinline__ F4 clip4(F4 v, int at, int p) {

@@ -8,7 +8,7 @@ namespace {
 template <class T>
 struct FwdArgs {
   const T *x, *f, *gate;
-  int gate_c, c, p;
+  int gate_c, c, p, cluster, share;
   long long tiles;
   zjai_residual_params prm;
   T *y, *z;
@@ -17,75 +17,80 @@ struct FwdArgs {
 
 // Rows held, the next tile copied ahead into the other of two slots.
 template <int kMode, class T>
-constexpr int fwd_slot_bytes() {  // per thread: f, x and the gate's logits
-  return 3 * kStagedRows * Place<kMode, T>::kBytes;
+constexpr int fwd_slot_bytes() {  // per warp: f, x and the gate's logits
+  return 3 * kStagedRows * Region<kMode, T>::kBytes;
 }
 template <int kMode, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
     residual_norm_staged_kernel(const FwdArgs<T> a) {
-  using P = Place<kMode, T>;
+  using R = Region<kMode, T>;
   constexpr int kRows = kStagedRows;
   constexpr bool kWhole = kMode == kWholeTiles, kVec = kMode != kAnywhere;
-  __shared__ Exchange<2, 2> ex;
-  __shared__ Params<kRows> prm;
+  __shared__ __align__(16) float totals[2 * 32];
   extern __shared__ __align__(16) char slots[];
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows, kWhole> rows(a.c, warps);
+  const Cluster cl(a.cluster);
+  const int ch0 = cl.rank * a.share, c = min(a.share, a.c - ch0);  // of the block
+  const Rows<kRows, kWhole> rows(c, a.share, a.c, warps);
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
-  const StagedRows<kMode> row(a.c, a.p, groups);
+  const StagedRows<kMode> row(c, a.p, groups);
+  char* mine = slots + wp * 2 * fwd_slot_bytes<kMode, T>();
+  Params<kRows> prm = {nullptr, a.share};
+  Exchange<2> ex = {nullptr, totals};
+  take_tail(slots + warps * 2 * fwd_slot_bytes<kMode, T>(), a.share, &prm.v, &ex);
   auto place = [&](int slot, int k, int j) {
-    return slots + ((slot * 3 + k) * kRows + j) * (int)blockDim.x * P::kBytes + threadIdx.x * P::kBytes;
+    return mine + ((slot * 3 + k) * kRows + j) * R::kBytes;
   };
   const long long elems = a.tiles / groups * a.c * a.p;
   auto copy = [&](const Tiles& t, int slot) {
-    const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
+    const long long e = ((long long)t.img * a.c + ch0) * a.p + t.g * kTapeGroup;
     const int nv = kWhole ? 4 : a.p - (t.g * kTapeGroup + (lane & 7) * 4);
-#pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      const bool on = row.on(j);
-      P::copy(place(slot, 0, j), a.f + e + row.e(j), on, nv, a.f + elems);
-      P::copy(place(slot, 1, j), a.x + e + row.e(j), on, nv, a.x + elems);
-      if (per_row) P::copy(place(slot, 2, j), a.gate + e + row.e(j), on, nv, a.gate + elems);
-    }
+    R::copy(place(slot, 0, 0), a.f + e, row, nv, a.f + elems);
+    R::copy(place(slot, 1, 0), a.x + e, row, nv, a.x + elems);
+    if (per_row) R::copy(place(slot, 2, 0), a.gate + e, row, nv, a.gate + elems);
   };
-  prm.load(a.prm, a.c);
+  prm.load(a.prm, ch0, c);
   __syncthreads();
-  Tiles tile(a.tiles, groups), ahead = tile;
+  Tiles tile(a.tiles, groups, cl.size), ahead = tile;
   if (ahead.on()) copy(ahead, 0);
   stage_commit();
   for (int slot = 0; tile.on(); tile.next(), slot ^= 1) {
     ahead.next();
+    if (!kVec) __syncwarp();  // the other slot has been read by all lanes
     if (ahead.on()) copy(ahead, slot ^ 1);
     stage_commit();
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
     const int nv = kWhole ? 4 : a.p - at;
-    const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
-    const long long x0 = (long long)tile.img * a.c * groups + tile.g;
+    const long long e0 = ((long long)tile.img * a.c + ch0) * a.p + tile.g * kTapeGroup;
+    const long long x0 = ((long long)tile.img * a.c + ch0) * groups + tile.g;
     F4 gate1 = all(0.f), sg1 = all(1.f), unused;
     if (a.gate_c == 1) {
       gate1 = load4<kVec>(a.gate + (long long)tile.img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
     }
     stage_wait<1>();
+    if (!kVec) __syncwarp();  // and the current one copied by all
+    // a row's f has been read before anything of it is stored: its place is free
+    auto scratch = [&](int j) { return reinterpret_cast<float*>(place(slot, 0, j)); };
     auto hold = [&](const zjai_tape& t, int j, F4 v) {
-      tape_hold4<kVec>(t.codes + e0 + row.e(j), t.exps + x0 + row.x(j), v, row.on(j), nv);
+      staged_hold<kMode>(t.codes + e0, t.exps + x0, v, row, j, nv, scratch(j));
     };
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
-      stats_part(rows, v, ex, 0);
-      __syncthreads();
-      stats_join(rows, ex, 0, inv_c, warps, wp, warps);
-      __syncthreads();
+      stats_part(rows, v, ex, 0, cl.rank);
+      cl.sync();
+      stats_join(rows, ex, 0, 0, inv_c, warps, cl, wp, warps);
+      cl.sync();
       nm = total4(ex, 0);
       r = total4(ex, 1);
     };
     auto get = [&](const T* map, int k, int j) {
-      return P::get(place(slot, k, j), map + e0 + row.e(j), nv);
+      return R::get(place(slot, k, j), map + e0, row, j, nv);
     };
     if (post) exchange([&](int j) { return get(a.f, 0, j); });
-    if (a.gate_c == 1 && a.tp.gate.codes && wp == 0)
+    if (a.gate_c == 1 && a.tp.gate.codes && wp == 0 && cl.rank == 0)
       tape_store4<kVec>(a.tp.gate, (long long)tile.img * a.p, (long long)tile.img * groups + tile.g,
                         at, a.p, gate1, lane < 8);
     F4 y[kRows];
@@ -102,7 +107,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
         if (a.tp.gate.codes) hold(a.tp.gate, j, g);
       }
       y[j] = fma4(s * prm.get(a.prm, kScale, row.ch(j)), u, get(a.x, 1, j));
-      staged_store<kMode>(a.y + e0 + row.e(j), y[j], row.on(j), nv);
+      staged_store<kMode>(a.y + e0, y[j], row, j, nv, scratch(j));
       if (a.tp.y.codes) hold(a.tp.y, j, kWhole ? y[j] : clip4<kVec>(y[j], at, a.p));
     }
     if (!pre) continue;
@@ -111,26 +116,30 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     for (int j = 0; j < kRows; ++j) {
       const F4 z =
           fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row.ch(j)), prm.get(a.prm, kPreB, row.ch(j)));
-      staged_store<kMode>(a.z + e0 + row.e(j), z, row.on(j), nv);
+      staged_store<kMode>(a.z + e0, z, row, j, nv, scratch(j));
       if (a.tp.z.codes) hold(a.tp.z, j, kWhole ? z : clip4<kVec>(z, at, a.p));
     }
   }
+  stage_wait<0>();
 }
 
 // Any channel count and alignment: rows are read again for each pass.
 template <bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const FwdArgs<T> a) {
   constexpr int kRows = 0;
-  __shared__ Exchange<2, 2> ex;
-  __shared__ Params<kRows> prm;
+  __shared__ __align__(16) float parts[kMaxWarps * Exchange<2>::kPitch], totals[2 * 32];
+  const Params<kRows> prm = {};
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows> rows(a.c, warps);
+  const Cluster cl(a.cluster);
+  const int ch0 = cl.rank * a.share, c = min(a.share, a.c - ch0);  // of the block
+  const Rows<kRows> rows(c, a.share, a.c, warps);
+  const Exchange<2> ex = {parts, totals};
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
-  for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const long long img = tile / groups, base = img * a.c;
-    const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
+  for (Tiles tile(a.tiles, groups, cl.size); tile.on(); tile.next()) {
+    const long long img = tile.img, base = img * a.c + ch0;
+    const int g = tile.g, at = g * kTapeGroup + (lane & 7) * 4;
     // a row's first element; its group's place among the exponents
     auto e0 = [&](int j) { return (base + rows.row(j)) * a.p; };
     auto ge = [&](int j) { return (base + rows.row(j)) * groups + g; };
@@ -141,22 +150,22 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const Fw
     if (a.gate_c == 1) {
       gate1 = load4<kVec>(a.gate + img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
-      if (a.tp.gate.codes && wp == 0)
+      if (a.tp.gate.codes && wp == 0 && cl.rank == 0)
         tape_store4<kVec>(a.tp.gate, img * a.p, img * groups + g, at, a.p, gate1, lane < 8);
     }
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
-      stats_part(rows, v, ex, 0);
-      __syncthreads();
-      stats_join(rows, ex, 0, inv_c, warps, wp, warps);
-      __syncthreads();
+      stats_part(rows, v, ex, 0, cl.rank);
+      cl.sync();
+      stats_join(rows, ex, 0, 0, inv_c, warps, cl, wp, warps);
+      cl.sync();
       nm = total4(ex, 0);
       r = total4(ex, 1);
     };
     if (post) exchange([&](int j) { return load(a.f, j); });
     const F4 nm1 = nm, r1 = r;
     auto y_of = [&](int j) {
-      const int ch = rows.param(j);
+      const int ch = ch0 + rows.param(j);
       F4 u = load(a.f, j), s = sg1;
       if (post)
         u = fma4((u + nm1) * r1, prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch));
@@ -174,7 +183,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_kernel(const Fw
       if (a.tp.y.codes)
         tape_store4<kVec>(a.tp.y, e0(j), ge(j), at, a.p, clip4<kVec>(y, at, a.p), on);
       if (!pre) continue;
-      const int ch = rows.param(j);
+      const int ch = ch0 + rows.param(j);
       const F4 z = fma4((y + nm) * r, prm.get(a.prm, kPreW, ch), prm.get(a.prm, kPreB, ch));
       if (on) store4<kVec>(a.z + e0(j), at, a.p, z);
       if (a.tp.z.codes)
@@ -235,26 +244,24 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
     VecCheck vec(p);
     vec.map(dx, es).map(df, es).map(dg, es).map(dyo, es).map(dzo, es);
     for (zjai_tape* t : tt) vec.map(t->codes, 1);
-    const Shape sh = shape_of(c, p, vec.ok, vec.words);
+    const long long tiles = (long long)n * (long long)groups;
+    const Shape sh = shape_of(c, p, vec.ok);
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p,
-                      (long long)n * (long long)groups, dp, (T*)dyo, (T*)dzo, dt};
-      const int blocks = (int)std::min<long long>(a.tiles, (long long)ctx->sms * sh.per_sm);
+      FwdArgs<T> a = {(const T*)dx, (const T*)df, (const T*)dg, gate_channels, c, p, sh.cluster,
+                      sh.share, tiles, dp, (T*)dyo, (T*)dzo, dt};
       void (*k)(FwdArgs<T>) = vec.ok ? residual_norm_kernel<true, T> : residual_norm_kernel<false, T>;
       int smem = 0;
-      if (sh.mode >= 0) {
+      if (sh.mode >= 0)
         smem = by_mode(sh.mode, [&](auto m) {
           constexpr int kMode = decltype(m)::value;
           k = residual_norm_staged_kernel<kMode, T>;
-          return 2 * fwd_slot_bytes<kMode, T>() * sh.warps * 32;
+          return 2 * fwd_slot_bytes<kMode, T>() * sh.warps +
+                 tail_bytes<2>(sh.share, sh.warps);
         });
-        ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                            me));
-      }
-      k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), me);
+      int count = 0;
+      ZJAI_TRY(cuda_check(blocks_of(sh, k, smem, tiles, ctx->sms, &count), me));
+      return cuda_check(launch(sh, k, smem, count, ctx->stream, a), me);
     }));
     ctx->launches++;
     ZJAI_TRY(finish_bytes_out(ctx, y, dyo, bytes, mem));

@@ -9,7 +9,7 @@ template <class T>
 struct BwdArgs {
   const T *dy, *dz, *f, *gate, *y;
   zjai_residual_tapes tp;  // taped f, gate, y
-  int gate_c, c, p;
+  int gate_c, c, p, cluster, share;
   long long tiles;
   zjai_residual_params prm;
   T *dx, *df, *dgate;
@@ -44,13 +44,17 @@ struct Kept<true, kVec, T> {
 // The parameter gradients are summed over a block's tiles in registers, written out per block.
 template <int kMode, bool kTaped, class T>
 struct BwdSlot {
-  using Grad = Place<kMode, T>;
-  using Kept = Place<kMode, typename std::conditional<kTaped, int8_t, T>::type>;
-  static constexpr int kGrad = Grad::kBytes, kKept = Kept::kBytes;
-  static constexpr int kBytes = kStagedRows * (2 * kGrad + 3 * kKept);  // per thread
-  static constexpr int kExps = kTaped ? 3 * kStagedRows * 4 / 8 : 0;  // per thread, words of rows
-  static constexpr int kB = sizeof(T) == 4 ? 0 : kStagedRows * (int)sizeof(float4);
-  static constexpr int kSlots = 2 * kBytes * kThreadsMost <= 180 * 1024 ? 2 : 1;
+  using Grad = Region<kMode, T>;
+  using Kept = Region<kMode, typename std::conditional<kTaped, int8_t, T>::type>;
+  // bytes per warp: of a slot's maps and exponents (words), and of b
+  static constexpr int kMaps = kStagedRows * (2 * Grad::kBytes + 3 * Kept::kBytes);
+  static constexpr int kExps = kTaped ? 3 * 4 * kStagedRows * 4 : 0;
+  static constexpr int kB = sizeof(T) == 4 ? 0 : kStagedRows * 32 * (int)sizeof(float4);
+  // two slots where 227 KB hold them
+  static constexpr int kRest = tail_bytes<4>(kBlockC, kMaxWarps) + 9 * 32 * (int)sizeof(float);
+  static constexpr int kSlots =
+      (2 * (kMaps + kExps) + kB) * kMaxWarps + kRest <= 227 * 1024 ? 2 : 1;
+  static constexpr int kBytes = kSlots * (kMaps + kExps) + kB;
 };
 template <int kMode, bool kTaped, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1)
@@ -58,11 +62,12 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   using S = BwdSlot<kMode, kTaped, T>;
   constexpr bool kWhole = kMode == kWholeTiles, kVec = kMode != kAnywhere;
   constexpr int kRows = kStagedRows;
-  __shared__ Exchange<4, 9> ex;  // totals: f 0, 1, y 2, 3, a 4, 5, b 6, 7, gate 8
-  __shared__ Params<kRows> prm;
+  __shared__ __align__(16) float totals[9 * 32];  // f 0, 1, y 2, 3, a 4, 5, b 6, 7, gate 8
   extern __shared__ __align__(16) char slots[];
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows, kWhole> rows(a.c, warps);
+  const Cluster cl(a.cluster);
+  const int ch0 = cl.rank * a.share, c = min(a.share, a.c - ch0);  // of the block
+  const Rows<kRows, kWhole> rows(c, a.share, a.c, warps);
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
@@ -75,37 +80,39 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   auto join_second = [&](auto f) {
     if (!two || (wp >= 4 && wp < 8)) f(two ? wp - 4 : wp, two ? 4 : warps);
   };
-  const StagedRows<kMode> row(a.c, a.p, groups);
+  const StagedRows<kMode> row(c, a.p, groups);
+  // the warp's shared memory: slots of maps, slots of exponents, b
+  char* mine = slots + wp * S::kBytes;
+  Params<kRows> prm = {nullptr, a.share};
+  Exchange<4> ex = {nullptr, totals};
+  take_tail(slots + warps * S::kBytes, a.share, &prm.v, &ex);
   auto grad_at = [&](int slot, int k, int j) {
-    return slots + slot * S::kBytes * (int)blockDim.x +
-           ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kGrad;
+    return mine + slot * S::kMaps + (k * kRows + j) * S::Grad::kBytes;
   };
   auto kept_at = [&](int slot, int k, int j) {
-    return slots + slot * S::kBytes * (int)blockDim.x + 2 * kRows * (int)blockDim.x * S::kGrad +
-           ((k * kRows + j) * (int)blockDim.x + threadIdx.x) * S::kKept;
+    return mine + slot * S::kMaps + 2 * kRows * S::Grad::kBytes + (k * kRows + j) * S::Kept::kBytes;
   };
   // a row's exponent comes as the aligned word that holds it, copied by one lane per row of the warp
   constexpr int kWarpRows = 4 * kRows;
   auto exp_at = [&](int slot, int k, int r) {
-    return slots + S::kSlots * S::kBytes * (int)blockDim.x +
-           (((slot * 3 + k) * warps + wp) * kWarpRows + r) * 4;
+    return mine + S::kSlots * S::kMaps + ((slot * 3 + k) * kWarpRows + r) * 4;
   };
   // b of a row, until df: where dy was, or (f16, bf16) in a place of its own
   auto b_at = [&](int slot, int j) {
-    char* q = slots + S::kSlots * (S::kBytes + S::kExps) * (int)blockDim.x;
-    return reinterpret_cast<float4*>(
-        sizeof(T) == 4 ? grad_at(slot, 0, j)
-                       : q + (j * (int)blockDim.x + (int)threadIdx.x) * (int)sizeof(float4));
+    return reinterpret_cast<float4*>(sizeof(T) == 4 ? grad_at(slot, 0, j)
+                                                    : mine + S::kSlots * (S::kMaps + S::kExps) +
+                                                          j * 32 * (int)sizeof(float4)) +
+           lane;
   };
   // exponents of the whole map (the gate's too: this path takes its own rows only where it has c)
   const long long x_all = a.tiles * a.c, elems = a.tiles / groups * a.c * a.p;
   auto copy = [&](const Tiles& t, int slot) {
-    const long long e = (long long)t.img * a.c * a.p + t.g * kTapeGroup;
-    const long long x = (long long)t.img * a.c * groups + t.g;
+    const long long e = ((long long)t.img * a.c + ch0) * a.p + t.g * kTapeGroup;
+    const long long x = ((long long)t.img * a.c + ch0) * groups + t.g;
     const int nv = kWhole ? 4 : a.p - (t.g * kTapeGroup + (lane & 7) * 4);
     auto keep_exps = [&](const zjai_tape& tp, int k) {
       const int ch = wp * kWarpRows + lane;
-      if (lane >= kWarpRows || (!kWhole && ch >= a.c)) return;
+      if (lane >= kWarpRows || (!kWhole && ch >= c)) return;
       const uint32_t at = ((uint32_t)(x & 3) + (uint32_t)ch * (uint32_t)groups) & ~3u;
       const int8_t* src = tp.exps + (x & ~3LL) + at;
       // whole tiles: a multiple of four exponents in all
@@ -117,50 +124,47 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       if (pre) keep_exps(a.tp.y, 1);
       if (per_row) keep_exps(a.tp.gate, 2);
     }
-    auto keep = [&](const T* map, const zjai_tape& tp, int k, int j) {
+    auto keep = [&](const T* map, const zjai_tape& tp, int k) {
       if constexpr (kTaped)
-        S::Kept::copy(kept_at(slot, k, j), tp.codes + e + row.e(j), row.on(j), nv, tp.codes + elems);
+        S::Kept::copy(kept_at(slot, k, 0), tp.codes + e, row, nv, tp.codes + elems);
       else
-        S::Kept::copy(kept_at(slot, k, j), map + e + row.e(j), row.on(j), nv, map + elems);
+        S::Kept::copy(kept_at(slot, k, 0), map + e, row, nv, map + elems);
     };
-    auto grad = [&](const T* map, int k, int j) {
-      S::Grad::copy(grad_at(slot, k, j), map + e + row.e(j), row.on(j), nv, map + elems);
+    auto grad = [&](const T* map, int k) {
+      S::Grad::copy(grad_at(slot, k, 0), map + e, row, nv, map + elems);
     };
-#pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      if (need_f) keep(a.f, a.tp.f, 0, j);
-      if (pre) keep(a.y, a.tp.y, 1, j);
-      if (pre) grad(a.dz, 1, j);
-      if (per_row) keep(a.gate, a.tp.gate, 2, j);
-      grad(a.dy, 0, j);
-    }
+    if (need_f) keep(a.f, a.tp.f, 0);
+    if (pre) keep(a.y, a.tp.y, 1);
+    if (pre) grad(a.dz, 1);
+    if (per_row) keep(a.gate, a.tp.gate, 2);
+    grad(a.dy, 0);
   };
   float acc[kRows][5];
 #pragma unroll
   for (int j = 0; j < kRows; ++j)
 #pragma unroll
     for (int i = 0; i < 5; ++i) acc[j][i] = 0.f;
-  prm.load(a.prm, a.c);
+  prm.load(a.prm, ch0, c);
   __syncthreads();
-  Tiles tile(a.tiles, groups), ahead = tile;
+  Tiles tile(a.tiles, groups, cl.size), ahead = tile;
   if (ahead.on()) copy(ahead, 0);
   stage_commit();
   for (int slot = 0; tile.on(); tile.next(), slot ^= S::kSlots - 1) {
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
     const int nv = kWhole ? 4 : a.p - at;
-    const long long e0 = (long long)tile.img * a.c * a.p + tile.g * kTapeGroup;
-    const uint32_t x0 = (uint32_t)((long long)tile.img * a.c * groups + tile.g);
+    const long long e0 = ((long long)tile.img * a.c + ch0) * a.p + tile.g * kTapeGroup;
+    const uint32_t x0 = (uint32_t)(((long long)tile.img * a.c + ch0) * groups + tile.g);
     auto kept = [&](const T* map, const zjai_tape& tp, int k, int j) {
       if constexpr (kTaped) {
         const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j * 4 + (lane >> 3)));
         const int e = (int)(int8_t)(w >> ((x0 + row.x(j)) & 3) * 8);
-        return taped4(S::Kept::words(kept_at(slot, k, j), tp.codes + e0 + row.e(j), nv).x, e);
+        return taped4(S::Kept::words(kept_at(slot, k, j), tp.codes + e0, row, j, nv).x, e);
       } else {
-        return S::Kept::get(kept_at(slot, k, j), map + e0 + row.e(j), nv);
+        return S::Kept::get(kept_at(slot, k, j), map + e0, row, j, nv);
       }
     };
     auto grad = [&](const T* map, int k, int j) {
-      return S::Grad::get(grad_at(slot, k, j), map + e0 + row.e(j), nv);
+      return S::Grad::get(grad_at(slot, k, j), map + e0, row, j, nv);
     };
     F4 sg1 = all(1.f), slope1 = all(0.f);
     if (a.gate_c == 1) {
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       stage_commit();
     }
     stage_wait<S::kSlots - 1>();
-    if (kTaped) __syncwarp();  // the exponents of the row's other lanes
+    if (kTaped || !kVec) __syncwarp();  // what other lanes copied
     F4 f[kRows], y[kRows];  // then LN(f), LN(y)
     if (need_f)
 #pragma unroll
@@ -183,13 +187,15 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     if (pre)
 #pragma unroll
       for (int j = 0; j < kRows; ++j) y[j] = kept(a.y, a.tp.y, 1, j);
-    if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0);
-    if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2);
+    if (post) stats_part(rows, [&](int j) { return f[j]; }, ex, 0, cl.rank);
+    if (pre) stats_part(rows, [&](int j) { return y[j]; }, ex, 2, cl.rank);
     if (post || pre) {
-      __syncthreads();
-      if (post) join_first([&](int n, int of) { stats_join(rows, ex, 0, inv_c, warps, n, of); });
-      if (pre) join_second([&](int n, int of) { stats_join(rows, ex, 2, inv_c, warps, n, of); });
-      __syncthreads();
+      cl.sync();
+      if (post)
+        join_first([&](int n, int of) { stats_join(rows, ex, 0, 0, inv_c, warps, cl, n, of); });
+      if (pre)
+        join_second([&](int n, int of) { stats_join(rows, ex, 2, 2, inv_c, warps, cl, n, of); });
+      cl.sync();
     }
     F4 r2 = all(1.f), am = all(0.f), ay = all(0.f);
     if (post) {
@@ -210,12 +216,12 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
           s1 = fma4(t, y[j], s1);
         }
       }
-      rows_to_part(s0, ex.part[0][wp]);
-      rows_to_part(s1, ex.part[1][wp]);
-      __syncthreads();
-      join_first([&](int n, int of) { sum_join(ex, 0, 4, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, 5, -inv_c, warps, n, of); });
-      __syncthreads();
+      rows_to_part(s0, ex.at(0, wp));
+      rows_to_part(s1, ex.at(1, wp));
+      cl.sync();
+      join_first([&](int n, int of) { sum_join(ex, 0, 4, -inv_c, warps, cl, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 5, -inv_c, warps, cl, n, of); });
+      cl.sync();
       am = total4(ex, 4);  // negated means
       ay = total4(ex, 5);
     }
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
         acc[j][4] += sum4(dz);
         d = fma4(fma4(y[j], ay, dz * prm.get(a.prm, kPreW, ch) + am), r2, d);
       }
-      staged_store<kMode>(a.dx + e0 + row.e(j), d, on, nv);
+      staged_store<kMode>(a.dx + e0, d, row, j, nv, ex.at(0, wp));
       if (!need_f) continue;
       const F4 u = post ? fma4(f[j], prm.get(a.prm, kPostW, ch), prm.get(a.prm, kPostB, ch)) : f[j];
       const F4 ds = d * prm.get(a.prm, kScale, ch);
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       if (per_row) {
         F4 slope;
         sigmoid4(kept(a.gate, a.tp.gate, 2, j), &sg, &slope);
-        staged_store<kMode>(a.dgate + e0 + row.e(j), ds * u * slope, on, nv);
+        staged_store<kMode>(a.dgate + e0, ds * u * slope, row, j, nv, ex.at(0, wp));
       }
       if (a.gate_c) du = ds * sg;
       acc[j][0] += dot4(d * sg, u);
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
           t1 = fma4(b, f[j], t1);
         }
       } else {
-        staged_store<kMode>(a.df + e0 + row.e(j), du, on, nv);
+        staged_store<kMode>(a.df + e0, du, row, j, nv, ex.at(0, wp));
       }
     }
     if (!need_f && a.df)
@@ -263,9 +269,9 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
         F4 d = grad(a.dy, 0, j);
         if (pre)
           d = fma4(fma4(y[j], ay, grad(a.dz, 1, j) * prm.get(a.prm, kPreW, row.ch(j)) + am), r2, d);
-        staged_store<kMode>(a.df + e0 + row.e(j), d, row.on(j), nv);
+        staged_store<kMode>(a.df + e0, d, row, j, nv, ex.at(0, wp));
       }
-    if (kTaped) __syncwarp();  // exponents read, before another lane copies over them
+    if (kTaped || !kVec) __syncwarp();  // read, before another lane copies over it
     // one slot: read now, but for b where dy was
     auto copy_one = [&]() {
       if (S::kSlots == 1) {
@@ -275,27 +281,27 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     };
     if (sizeof(T) != 4 || !post) copy_one();
     if (!post && a.gate_c != 1) continue;
-    if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
-    if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
-    __syncthreads();
+    if (post) rows_to_part(t0, ex.at(0, wp)), rows_to_part(t1, ex.at(1, wp));
+    if (a.gate_c == 1) rows_to_part(t2, ex.at(2, wp));
+    cl.sync();
     if (post) {
-      join_first([&](int n, int of) { sum_join(ex, 0, 6, -inv_c, warps, n, of); });
-      join_second([&](int n, int of) { sum_join(ex, 1, 7, -inv_c, warps, n, of); });
+      join_first([&](int n, int of) { sum_join(ex, 0, 6, -inv_c, warps, cl, n, of); });
+      join_second([&](int n, int of) { sum_join(ex, 1, 7, -inv_c, warps, cl, n, of); });
     }
-    if (a.gate_c == 1) sum_join(ex, 2, 8, 1.f, warps, wp, warps);
-    __syncthreads();
-    if (a.gate_c == 1 && threadIdx.x < 8)
+    if (a.gate_c == 1) sum_join(ex, 2, 8, 1.f, warps, cl, wp, warps);
+    cl.sync();
+    if (a.gate_c == 1 && threadIdx.x < 8 && cl.rank == 0)
       store4<kVec>(a.dgate + (long long)tile.img * a.p, at, a.p, total4(ex, 8) * slope1);
     if (!post) continue;
     const F4 bm = total4(ex, 6), bf = total4(ex, 7), r1 = total4(ex, 1);  // negated means
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      staged_store<kMode>(a.df + e0 + row.e(j), fma4(f[j], bf, make4(*b_at(slot, j)) + bm) * r1,
-                          row.on(j), nv);
+      staged_store<kMode>(a.df + e0, fma4(f[j], bf, make4(*b_at(slot, j)) + bm) * r1, row, j, nv,
+                          ex.at(0, wp));
     if (sizeof(T) == 4) copy_one();
   }
   stage_wait<0>();
-  float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
+  float* out = a.sums + (long long)(blockIdx.x / (unsigned)cl.size) * 5 * a.c + ch0;
 #pragma unroll
   for (int j = 0; j < kRows; ++j)
 #pragma unroll
@@ -312,20 +318,23 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
 template <bool kTaped, bool kVec, class T>
 __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(const BwdArgs<T> a) {
   constexpr int kRows = 0;
-  __shared__ Exchange<4, 4> ex;
-  __shared__ Params<kRows> prm;
-  extern __shared__ float acc_c[];  // [5][c]
+  __shared__ __align__(16) float parts[kMaxWarps * Exchange<4>::kPitch], totals[4 * 32];
+  const Params<kRows> prm = {};
+  extern __shared__ float acc_c[];  // [5][c of the block]
   const int warps = blockDim.x >> 5, wp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows<kRows> rows(a.c, warps);
+  const Cluster cl(a.cluster);
+  const int ch0 = cl.rank * a.share, c = min(a.share, a.c - ch0);  // of the block
+  const Rows<kRows> rows(c, a.share, a.c, warps);
+  const Exchange<4> ex = {parts, totals};
   const int groups = (int)tape_groups(a.p);
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
   const bool need_f = post || a.gate_c || a.prm.scale;
-  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) acc_c[i] = 0.f;
+  for (int i = threadIdx.x; i < 5 * c; i += blockDim.x) acc_c[i] = 0.f;
   __syncthreads();
-  for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const long long img = tile / groups, base = img * a.c;
-    const int g = (int)(tile - img * groups), at = g * kTapeGroup + (lane & 7) * 4;
+  for (Tiles tile(a.tiles, groups, cl.size); tile.on(); tile.next()) {
+    const long long img = tile.img, base = img * a.c + ch0;
+    const int g = tile.g, at = g * kTapeGroup + (lane & 7) * 4;
     using K = Kept<kTaped, kVec, T>;
     auto e0 = [&](int j) { return (base + rows.param(j)) * a.p; };
     auto grad = [&](const T* v, int j) {
@@ -343,13 +352,13 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
       sigmoid4(k.get(), &sg1, &slope1);
     }
     F4 nm1 = all(0.f), r1 = all(1.f), nm2 = all(0.f), r2 = all(1.f), am = all(0.f), ay = all(0.f);
-    if (post) stats_part(rows, [&](int j) { return kept(a.f, a.tp.f, j); }, ex, 0);
-    if (pre) stats_part(rows, [&](int j) { return kept(a.y, a.tp.y, j); }, ex, 2);
+    if (post) stats_part(rows, [&](int j) { return kept(a.f, a.tp.f, j); }, ex, 0, cl.rank);
+    if (pre) stats_part(rows, [&](int j) { return kept(a.y, a.tp.y, j); }, ex, 2, cl.rank);
     if (post || pre) {
-      __syncthreads();
-      if (post) stats_join(rows, ex, 0, inv_c, warps, wp, warps);
-      if (pre) stats_join(rows, ex, 2, inv_c, warps, wp, warps);
-      __syncthreads();
+      cl.sync();
+      if (post) stats_join(rows, ex, 0, 0, inv_c, warps, cl, wp, warps);
+      if (pre) stats_join(rows, ex, 2, 2, inv_c, warps, cl, wp, warps);
+      cl.sync();
       if (post) nm1 = total4(ex, 0), r1 = total4(ex, 1);
       if (pre) nm2 = total4(ex, 2), r2 = total4(ex, 3);
     }
@@ -361,23 +370,23 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     if (pre) {
       F4 s0 = all(0.f), s1 = all(0.f);
       FOR_ROWS(j) if (rows.on(j)) {
-        const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, rows.param(j));
+        const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, ch0 + rows.param(j));
         s0 = s0 + t;
         s1 = fma4(t, yn_of(j), s1);
       }
-      rows_to_part(s0, ex.part[0][wp]);
-      rows_to_part(s1, ex.part[1][wp]);
-      __syncthreads();
-      sum_join(ex, 0, 0, -inv_c, warps, wp, warps);
-      sum_join(ex, 1, 1, -inv_c, warps, wp, warps);
-      __syncthreads();
+      rows_to_part(s0, ex.at(0, wp));
+      rows_to_part(s1, ex.at(1, wp));
+      cl.sync();
+      sum_join(ex, 0, 0, -inv_c, warps, cl, wp, warps);
+      sum_join(ex, 1, 1, -inv_c, warps, cl, wp, warps);
+      cl.sync();
       am = total4(ex, 0);  // negated means
       ay = total4(ex, 1);
     }
     auto d_of = [&](int j) {
       const F4 d = grad(a.dy, j);
       if (!pre) return d;
-      const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, rows.param(j));
+      const F4 t = grad(a.dz, j) * prm.get(a.prm, kPreW, ch0 + rows.param(j));
       return fma4(fma4(yn_of(j), ay, t + am), r2, d);
     };
     auto gate_of = [&](int j, F4* s, F4* slope) {
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
     };
     F4 t0 = all(0.f), t1 = all(0.f), t2 = all(0.f);
     FOR_ROWS(j) {
-      const int ch = rows.param(j);
+      const int ch = ch0 + rows.param(j);
       const bool on = rows.on(j);
       const F4 d = d_of(j), fn = need_f ? fn_of(j) : all(0.f);
       F4 sg, slope;
@@ -410,34 +419,34 @@ __global__ void __launch_bounds__(kThreadsMost, 1) residual_norm_bwd_kernel(cons
         float s = v[i];
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if ((lane & 7) == 0 && on) acc_c[i * a.c + ch] += s;
+        if ((lane & 7) == 0 && on) acc_c[i * c + ch - ch0] += s;
       }
     }
     if (!post && a.gate_c != 1) continue;
-    if (post) rows_to_part(t0, ex.part[0][wp]), rows_to_part(t1, ex.part[1][wp]);
-    if (a.gate_c == 1) rows_to_part(t2, ex.part[2][wp]);
-    __syncthreads();
+    if (post) rows_to_part(t0, ex.at(0, wp)), rows_to_part(t1, ex.at(1, wp));
+    if (a.gate_c == 1) rows_to_part(t2, ex.at(2, wp));
+    cl.sync();
     if (post) {
-      sum_join(ex, 0, 0, -inv_c, warps, wp, warps);
-      sum_join(ex, 1, 1, -inv_c, warps, wp, warps);
+      sum_join(ex, 0, 0, -inv_c, warps, cl, wp, warps);
+      sum_join(ex, 1, 1, -inv_c, warps, cl, wp, warps);
     }
-    if (a.gate_c == 1) sum_join(ex, 2, 2, 1.f, warps, wp, warps);
-    __syncthreads();
-    if (a.gate_c == 1 && threadIdx.x < 8)
+    if (a.gate_c == 1) sum_join(ex, 2, 2, 1.f, warps, cl, wp, warps);
+    cl.sync();
+    if (a.gate_c == 1 && threadIdx.x < 8 && cl.rank == 0)
       store4<kVec>(a.dgate + img * a.p, at, a.p, total4(ex, 2) * slope1);
     if (!post) continue;
     const F4 bm = total4(ex, 0), bf = total4(ex, 1);  // negated means
     FOR_ROWS(j) if (rows.on(j)) {
-      const int ch = rows.param(j);
+      const int ch = ch0 + rows.param(j);
       F4 sg, slope;
       gate_of(j, &sg, &slope);
       const F4 b = d_of(j) * prm.get(a.prm, kScale, ch) * sg * prm.get(a.prm, kPostW, ch);
       store4<kVec>(a.df + e0(j), at, a.p, fma4(fn_of(j), bf, b + bm) * r1);
     }
   }
-  float* out = a.sums + (long long)blockIdx.x * 5 * a.c;
+  float* out = a.sums + (long long)(blockIdx.x / (unsigned)cl.size) * 5 * a.c + ch0;
   __syncthreads();
-  for (int i = threadIdx.x; i < 5 * a.c; i += blockDim.x) out[i] = acc_c[i];
+  for (int i = threadIdx.x; i < 5 * c; i += blockDim.x) out[(i / c) * a.c + i % c] = acc_c[i];
 }
 
 struct SumOut {
@@ -542,32 +551,32 @@ int zjai_gated_residual_norm_backward(zjai_ctx* ctx, const void* dy, const void*
     vec.map(gx, es).map(gf, es).map(gg, es);
     vec.map(dt.f.codes, 1).map(dt.gate.codes, 1).map(dt.y.codes, 1);
     vec.map(dt.f.exps, 1).map(dt.gate.exps, 1).map(dt.y.exps, 1);
-    const Shape sh = shape_of(c, p, vec.ok, vec.words);
-    const int blocks = (int)std::min<long long>(tiles, (long long)ctx->sms * sh.per_sm);
-    float* sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
-    if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
-    auto launch = [&](auto t, auto tp) -> int {
+    const Shape sh = shape_of(c, p, vec.ok);
+    int blocks = 0;
+    float* sums = nullptr;
+    auto run = [&](auto t, auto tp) -> int {
       using T = decltype(t);
       constexpr bool kTaped = decltype(tp)::value;
       BwdArgs<T> a = {(const T*)ddy, (const T*)ddz, (const T*)df, (const T*)dg, (const T*)dyy, dt,
-                      gate_channels, c, p, tiles, dp, (T*)gx, (T*)gf, (T*)gg, sums};
+                      gate_channels, c, p, sh.cluster, sh.share, tiles, dp, (T*)gx, (T*)gf, (T*)gg,
+                      nullptr};
       void (*k)(BwdArgs<T>) = vec.ok ? residual_norm_bwd_kernel<kTaped, true, T>
                                      : residual_norm_bwd_kernel<kTaped, false, T>;
-      int smem = 5 * c * (int)sizeof(float);
+      int smem = 5 * sh.share * (int)sizeof(float);
       if (sh.mode >= 0)
         smem = by_mode(sh.mode, [&](auto m) {
           using S = BwdSlot<decltype(m)::value, kTaped, T>;
           k = residual_norm_bwd_staged_kernel<decltype(m)::value, kTaped, T>;
-          return (S::kSlots * (S::kBytes + S::kExps) + S::kB) * sh.warps * 32;
+          return S::kBytes * sh.warps + tail_bytes<4>(sh.share, sh.warps);
         });
-      ZJAI_TRY(cuda_check(cudaFuncSetAttribute((const void*)k,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                          me));
-      k<<<blocks, sh.warps * 32, smem, ctx->stream>>>(a);
-      return cuda_check(cudaGetLastError(), me);
+      ZJAI_TRY(cuda_check(blocks_of(sh, k, smem, tiles, ctx->sms, &blocks), me));
+      sums = static_cast<float*>(ctx->arena.alloc((size_t)blocks * 5 * c * sizeof(float)));
+      if (!sums) return fail(ZJAI_LIMIT_EXCEEDED, "device arena exhausted (parameter sums)");
+      a.sums = sums;
+      return cuda_check(launch(sh, k, smem, blocks, ctx->stream, a), me);
     };
     ZJAI_TRY(by_dtype(dtype, [&](auto t) -> int {
-      return taped ? launch(t, std::true_type()) : launch(t, std::false_type());
+      return taped ? run(t, std::true_type()) : run(t, std::false_type());
     }));
     residual_sums_kernel<<<dim3((c + 31) / 32, 5), 256, 0, ctx->stream>>>(sums, blocks, c, so);
     ctx->launches += 2;
