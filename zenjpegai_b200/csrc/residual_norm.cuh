@@ -329,10 +329,10 @@ __device__ __forceinline__ void stage_copy_some(char* dst, const void* src, int 
                "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void stage_copy_two(char* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+__device__ __forceinline__ void stage_copy_two(char* dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(
                    (uint32_t)__cvta_generic_to_shared(dst)),
-               "l"(src)
+               "l"(src), "r"(on ? 8 : 0)
                : "memory");
 }
 __device__ __forceinline__ void stage_commit() {
@@ -418,9 +418,10 @@ struct Region {
           stage_copy_some(to + j * kBytes + lane * 16 + i * 4, map + row.e(j) + i,
                           row.on(j) && nv > i ? 4 : 0);
     } else {
-      // the 8 bytes from the ones that hold the map's first element on. For what is behind the tensor
-      // (rows that do not exist) its last ones are copied: nothing of them is used.
-      const uint32_t sub = (uint32_t)reinterpret_cast<uintptr_t>(map) & 7u;
+      // the 8 bytes from the ones that hold the map's first element on; what would begin behind the
+      // tensor is replaced by its last ones, of which nothing is used; zeros for rows that do not
+      // exist
+      const uint32_t sub = (uint32_t)reinterpret_cast<uintptr_t>(map) & 7u, on = row.warp_rows();
       const char* from = reinterpret_cast<const char*>(map) - sub;
       const uint32_t last =
           (uint32_t)min((long long)(reinterpret_cast<const char*>(end) - 1 - from), 0xffffffffLL);
@@ -429,7 +430,7 @@ struct Region {
       const uint32_t step = (uint32_t)row.p * kSize;
       uint32_t o = row.warp_e() * kSize + sub;
       auto chunk = [&](uint32_t at, int r, int k) {
-        stage_copy_two(to + r * kRowBytes + k * 8, from + (min(at, last) & ~7u));
+        stage_copy_two(to + r * kRowBytes + k * 8, from + (min(at, last) & ~7u), on >> r & 1);
       };
       if (lane < 4 * kStagedRows) chunk(o + lane * step + 8u * kLanes, lane, kLanes);
       o += lane / kLanes * step + 8u * (lane % kLanes);
