@@ -19,9 +19,9 @@
 // (the CTAs of a tile work on neighbouring chunks at a time: rows are far apart in memory, and with
 // ranges of their own they kept opening DRAM pages for 128 bytes):
 //  - the operands come to shared memory some chunks ahead: by TMA where all rows start on 16 bytes
-//    (kVec; bf16 d_out, which needs no conversion, straight into the operand), else by cp.async,
-//    each thread copying what it will itself convert (rows of odd length start anywhere, which a
-//    TMA box cannot);
+//    (kVec; bf16 d_out, which needs no conversion, straight into the operand), else by cp.async:
+//    rows of odd length start anywhere, which a TMA box cannot, so a warp copies the aligned 16
+//    bytes that hold the rows it will itself convert, and shifts them into place as it reads them;
 //  - 16 converter warps, in groups that take turns, turn a chunk into bf16 in the 128-byte-swizzled
 //    K-major layout that the tensor core reads (16-byte piece j of row r at j ^ (r & 7)), and drain
 //    the accumulators, half a window after they are complete;
@@ -50,9 +50,7 @@ constexpr int kBufCols = 256;              // TMEM columns of an accumulator set
 // Per element type and alignment: bf16 terms of a d_out element; groups of converter warps, which
 // take every kGroups-th chunk (a chunk has a fixed cost of waits and hand-offs per warp, about as
 // long as its conversion by 16 warps: with one group the kernel took 1.3 to 1.5 times as long);
-// stages of converted operands and chunks copied ahead of them; chunks between drains. cp.async:
-// 32-bit words a thread copies of 8 positions of d_out (the words that hold them: one more where
-// they start anywhere) and of 16 codes.
+// stages of converted operands and chunks copied ahead of them; chunks between drains.
 template <bool kVec, class T>
 struct Form;
 template <>
@@ -73,10 +71,10 @@ struct Form<true, __nv_bfloat16> {  // kRaw: the codes alone
 template <class T>
 struct Form<false, T> {
   static constexpr int kTerms = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;
-  static constexpr int kGroups = 1, kStages = kTerms == 1 ? 3 : 2, kAhead = kTerms == 3 ? 2 : 3;
+  static constexpr int kGroups = 1, kStages = kTerms == 1 ? 3 : 2, kAhead = kTerms == 3 ? 2 : 4;
   static constexpr int kPerWindow = 4;
-  static constexpr int kWordsD = sizeof(T) == 4 ? 8 : 5, kWordsX = 5;
-  static constexpr int kRaw = (2 * kWordsD + kWordsX) * 4 * kWorkThreads;
+  static constexpr int kPitchD = kChunk * (int)sizeof(T) + 16, kPitchX = kChunk + 16;  // of a row
+  static constexpr int kRaw = kM * kPitchD + kN * kPitchX;
 };
 template <bool kVec, class T>
 constexpr bool direct() {  // d_out is copied into the operand, the ones row gives db
@@ -135,9 +133,9 @@ __device__ __forceinline__ uint32_t ld_shared4(uint32_t at) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
-// asynchronous copy to shared memory: the first `bytes` from src, zeros after them
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+// 16 bytes from src, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() {
@@ -148,70 +146,43 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kNewer) : "memory");
 }
 
-// The five aligned words that hold the `valid` (0 to 16) bytes at q, word j to dst + j kWorkThreads
-// words; q may start anywhere. Words without a valid byte are zero. Nothing outside the tensor
-// [lo, hi) is read: a word that sticks out behind is copied as far as it goes, and the one that may
-// stick out before (the tensor's first) is put together from its bytes.
-__device__ __forceinline__ void copy_words5(uint32_t dst, const uint8_t* q, int valid,
-                                            const uint8_t* lo, const uint8_t* hi) {
-  const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3);
-  const uint8_t* a = q - off;
+// Rows that start anywhere: a chunk's kBytes of kRows rows, `first` and those behind it, of a map
+// whose chunk starts at `at` in row 0, rows `row_bytes` apart, to rows of kBytes + 16 in shared
+// memory, by the aligned 16 bytes that hold them: of memory outside the map none but the rest of an
+// aligned 16 bytes with a byte of it is touched (what would begin behind the map is replaced by its
+// last). Rows from `rows` on do not exist: zeros. (Copies of the map's last bytes in their place, from
+// every block, took the kernel from 37 to 67 us at 64 x 64 channels in bf16.)
+template <int kRows, int kBytes>
+__device__ __forceinline__ void copy_rows(uint32_t to, const char* at, long long row_bytes, int first,
+                                          int rows, const char* last) {
+  constexpr int kLanes = kBytes / 16, kAtOnce = 32 / kLanes;
+  const int lane = threadIdx.x & 31;
+  auto piece = [&](int r, int j) {
+    const uintptr_t q = (reinterpret_cast<uintptr_t>(at + r * row_bytes) & ~(uintptr_t)15) + 16 * j;
+    copy16(to + r * (kBytes + 16) + 16 * j,
+           reinterpret_cast<const void*>(min(q, reinterpret_cast<uintptr_t>(last))), r < rows);
+  };
 #pragma unroll
-  for (int j = 0; j < 5; ++j) {
-    const uint8_t* at = a + 4 * j;
-    const uint32_t to = dst + j * 4 * kWorkThreads;
-    const bool want = 4 * j - off < valid;
-    if (j == 0 && want && at < lo) {
-      uint32_t w = 0u;
-      for (int i = 0; i < 4; ++i)
-        if (at + i >= lo && at + i < hi) w |= (uint32_t)__ldg(at + i) << (8 * i);
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(w) : "memory");
-    } else {
-      const long long left = hi - at;
-      copy4(to, want ? at : lo + ((4 - (reinterpret_cast<uintptr_t>(lo) & 3)) & 3),
-            want ? (left < 4 ? (int)left : 4) : 0);
-    }
-  }
+  for (int r = 0; r < kRows; r += kAtOnce) piece(first + r + lane / kLanes, lane % kLanes);
+  if (lane < kRows) piece(first + lane, kLanes);
 }
-// the 16 bytes in place, those from `valid` on zero
-__device__ __forceinline__ void place_words5(uint32_t src, const uint8_t* q, int valid,
-                                             uint32_t* v) {
-  const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(q) & 3) * 8;
-  uint32_t w[5];
+// Words of 4 kWords bytes from the byte `from` of shared memory on.
+template <int kWords>
+__device__ __forceinline__ void ld_shifted(uint32_t from, uint32_t* w) {
+  const uint32_t at = from & ~3u, sh = (from & 3u) * 8u;
+  uint32_t v[kWords + 1];
 #pragma unroll
-  for (int j = 0; j < 5; ++j) w[j] = ld_shared4(src + j * 4 * kWorkThreads);
+  for (int i = 0; i <= kWords; ++i) v[i] = ld_shared4(at + 4 * i);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = __funnelshift_r(w[j], w[j + 1], sh);
-    const int left = valid - 4 * j;
-    if (left < 4) v[j] = left <= 0 ? 0u : v[j] & (0xffffffffu >> (32 - 8 * left));
-  }
+  for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], sh);
 }
-
-// One thread's piece of a chunk of d_out whose rows start anywhere, 8 positions of a row: the copy
-// to `raw` (the thread's place in a slot), and the words from there (8 f32, or 8 halves in 4).
-template <class T>
-__device__ __forceinline__ void copy_piece(uint32_t raw, const T* row, int at, int p, bool ok,
-                                           const T* lo, const T* hi) {
-  const int valid = ok ? max(0, min(8, p - at)) : 0;
-  if constexpr (sizeof(T) == 4) {
+// bytes from `valid` on zero
+template <int kWords>
+__device__ __forceinline__ void clip_words(uint32_t* w, int valid) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      copy4(raw + i * 4 * kWorkThreads, i < valid ? row + at + i : lo, i < valid ? 4 : 0);
-  } else {
-    copy_words5(raw, reinterpret_cast<const uint8_t*>(row + at), 2 * valid,
-                reinterpret_cast<const uint8_t*>(lo), reinterpret_cast<const uint8_t*>(hi));
-  }
-}
-template <class T>
-__device__ __forceinline__ void get_piece(uint32_t raw, const T* row, int at, int p, bool ok,
-                                          uint32_t* w) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = ld_shared4(raw + i * 4 * kWorkThreads);
-  } else {
-    place_words5(raw, reinterpret_cast<const uint8_t*>(row + at),
-                 ok ? 2 * max(0, min(8, p - at)) : 0, w);
+  for (int i = 0; i < kWords; ++i) {
+    const int left = valid - 4 * i;
+    if (left < 4) w[i] = left <= 0 ? 0u : w[i] & (0xffffffffu >> (32 - 8 * left));
   }
 }
 
@@ -258,6 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // a slot is always read by the same group: another one's parity test would take the phase before
   // the last for the one it waits for
   static_assert(kAhead % kGroups == 0, "slots change groups");
+  // and with fewer stages than groups, of a stage
+  static_assert(kStages >= kGroups, "a group may be two phases behind");
   constexpr int kGroupWarps = kWorkers / kGroups, kGroupThreads = kWorkThreads / kGroups;
   constexpr int kStageBytes = stage_bytes<kVec, T>();
   constexpr bool kDirect = direct<kVec, T>();
@@ -412,28 +385,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x_rows = min(a.nb, a.c - i0);
     auto swizzled = [](uint32_t base, int r, int j) { return base + r * 128 + ((j ^ (r & 7)) << 4); };
 
-    // cp.async: the chunk being copied, and the one being converted
-    const T* d_lo = static_cast<const T*>(a.dout);
-    const T* d_hi = d_lo + a.d_elems;
-    const uint8_t* x_lo = reinterpret_cast<const uint8_t*>(a.codes);
-    const uint8_t* x_hi = x_lo + a.x_elems;
-    const long long d64 = 64LL * a.p;
-    Chunk next(split, a.splits, a.chunks_img), cur = next;
-    auto row_d = [&](const Chunk& q) { return d_lo + ((long long)q.img * a.oc + o0 + dr) * a.p; };
-    auto row_x = [&](const Chunk& q) { return x_lo + ((long long)q.img * a.c + i0 + xr) * a.p; };
-    int copied = 0;
+    // cp.async: the group's chunk being copied, and the one being converted
+    const char* d_lo = static_cast<const char*>(a.dout);
+    const char* x_lo = reinterpret_cast<const char*>(a.codes);
+    const long long d_row = (long long)a.p * (int)sizeof(T);
+    auto last_of = [](const char* hi) {  // the aligned 16 bytes with the byte before hi
+      return reinterpret_cast<const char*>((reinterpret_cast<uintptr_t>(hi) - 1) & ~(uintptr_t)15);
+    };
+    const char *d_last = last_of(d_lo + a.d_elems * (int)sizeof(T)), *x_last = last_of(x_lo + a.x_elems);
+    Chunk next(split + group * a.splits, kGroups * a.splits, a.chunks_img), cur = next;
+    auto at_d = [&](const Chunk& q) {
+      return d_lo + (((long long)q.img * a.oc + o0) * a.p + q.in * kChunk) * (int)sizeof(T);
+    };
+    auto at_x = [&](const Chunk& q) {
+      return x_lo + ((long long)q.img * a.c + i0) * a.p + q.in * kChunk;
+    };
+    int copied = group;
     auto copy_chunk = [&]() {
       if constexpr (!kVec) {
         if (copied < count) {
-          const uint32_t raw = raw_base + copied % kAhead * kRaw + tid * 4;
+          const uint32_t raw = raw_base + copied % kAhead * kRaw;
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            copy_piece<T>(raw + u * F::kWordsD * 4 * kWorkThreads, row_d(next) + u * d64,
-                          next.in * kChunk + dj * 8, a.p, o0 + u * 64 + dr < a.oc, d_lo, d_hi);
-          const int at = next.in * kChunk + xj * 16;
-          copy_words5(raw + 2 * F::kWordsD * 4 * kWorkThreads, row_x(next) + at,
-                      xr < x_rows ? max(0, min(16, a.p - at)) : 0, x_lo, x_hi);
-          ++copied;
+          for (int u = 0; u < kUnitsD; ++u)
+            copy_rows<4, kChunk * (int)sizeof(T)>(raw, at_d(next), d_row,
+                                                  u * kRowsD + (tid >> 5) * 4, a.oc - o0, d_last);
+#pragma unroll
+          for (int u = 0; u < kUnitsX; ++u)
+            copy_rows<8, kChunk>(raw + kM * F::kPitchD, at_x(next), a.p,
+                                 u * kRowsX + (tid >> 5) * 8, x_rows, x_last);
+          copied += kGroups;
           next.next();
         }
         copy_commit();
@@ -494,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float btot[kUnitsD] = {};
 
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) copy_chunk();
+    for (int j = 0; j < kAhead / kGroups; ++j) copy_chunk();
     load_exps(group < count);
     bool ok = true;
     for (int k = group, turn = 0; k < count && ok; k += kGroups, ++turn) {
@@ -528,14 +508,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(raw_empty + 8 * sl);
       } else {
-        copy_wait<kAhead - 1>();
-        const int at = cur.in * kChunk + xj * 16;
-        place_words5(raw + tid * 4 + 2 * F::kWordsD * 4 * kWorkThreads, row_x(cur) + at,
-                     xr < x_rows ? max(0, min(16, a.p - at)) : 0, wx[0]);
+        copy_wait<kAhead / kGroups - 1>();
+        __syncwarp();
+        const uint32_t d_sub = (uint32_t)reinterpret_cast<uintptr_t>(at_d(cur));
+        const uint32_t x_sub = (uint32_t)reinterpret_cast<uintptr_t>(at_x(cur));
 #pragma unroll
-        for (int i = 0; i < kParts; ++i)
-          get_piece<T>(raw + tid * 4 + i * F::kWordsD * 4 * kWorkThreads, row_d(cur) + i * d64,
-                       cur.in * kChunk + dj * 8, a.p, o0 + i * 64 + dr < a.oc, wd[i]);
+        for (int u = 0; u < kUnitsX; ++u) {
+          const int r = u * kRowsX + xr;
+          ld_shifted<4>(raw + kM * F::kPitchD + r * F::kPitchX + ((x_sub + r * (uint32_t)a.p) & 15u) +
+                            xj * 16,
+                        wx[u]);
+        }
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const int r = i * kRowsD + dr;
+          const uint32_t from = raw + r * F::kPitchD + ((d_sub + r * (uint32_t)d_row) & 15u) +
+                                dj * 8 * (int)sizeof(T);
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) wd[i][q] = ld_shared4(from + 4 * q);
+          } else {
+            ld_shifted<4>(from, wd[i]);
+          }
+        }
+        __syncwarp();
+        copy_chunk();
+        if (cur.in * kChunk + kChunk > a.p) {  // a row's last chunk
+          const int left = a.p - cur.in * kChunk;
+#pragma unroll
+          for (int u = 0; u < kUnitsX; ++u) clip_words<4>(wx[u], left - xj * 16);
+#pragma unroll
+          for (int i = 0; i < kParts; ++i)
+            clip_words<2 * (int)sizeof(T)>(wd[i], (left - dj * 8) * (int)sizeof(T));
+        }
+        cur.next();
       }
       if (k >= kStages) {
         ok = mbar_wait_sleep(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
@@ -598,8 +604,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!kVec) cur.next();
-      copy_chunk();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(full + 8 * st);
