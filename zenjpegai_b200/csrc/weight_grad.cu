@@ -48,14 +48,16 @@ constexpr int kOnes = 16 * kChunk * 2;     // and of the 16 rows with the ones
 constexpr int kBufCols = 256;              // TMEM columns of an accumulator set
 
 // Per element type and alignment: bf16 terms of a d_out element; groups of converter warps, which
-// take every kGroups-th chunk (a chunk has a fixed cost of waits and hand-offs per warp, about as
-// long as its conversion by 16 warps: with one group the kernel took 1.3 to 1.5 times as long);
-// stages of converted operands and chunks copied ahead of them; chunks between drains.
+// take every kGroups-th chunk; stages of converted operands and chunks copied ahead of them; chunks
+// between drains. A chunk has a fixed cost of waits and hand-offs per warp, which groups hide where
+// there are chunks enough in shared memory (28 x 128 x 128^2: f16 to 384 channels 163 us with two
+// groups, 171 with one; bf16 to 1024 242 us with four, a tenth more with one); f32's few and large
+// ones are done with sooner by all warps at once (to 384: 204 us with one group, 230 with two).
 template <bool kVec, class T>
 struct Form;
 template <>
 struct Form<true, float> {
-  static constexpr int kTerms = 3, kGroups = 2, kStages = 2, kAhead = 2, kPerWindow = 4;
+  static constexpr int kTerms = 3, kGroups = 1, kStages = 2, kAhead = 2, kPerWindow = 4;
   static constexpr int kRaw = 2 * kBlock + kBlock / 2;
 };
 template <>
