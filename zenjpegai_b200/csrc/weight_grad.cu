@@ -188,6 +188,13 @@ __device__ __forceinline__ void clip_words(uint32_t* w, int valid) {
   }
 }
 
+// Before a slot is given to the next copy: the registers of each vector that was read from it have
+// their values, in all lanes. (Arriving at the slot's barrier does not say so: the next chunk's copy
+// was seen to land before reads issued ahead of the arrival.) `seen` combines a register of each.
+__device__ __forceinline__ void wait_read(uint32_t seen) {
+  if (__all_sync(0xffffffffu, seen == 0x9e3779b9u)) __nanosleep(1);  // any use will do
+}
+
 // 4 codes -> 4 bf16 values code 2^e: the low 7 bits and the sign bit of a code, each as the low
 // mantissa bits of 128 (bf16 0x4300), give code = (128 + low7) - (128 + 128 sign); the subtraction
 // and the scaling are exact.
@@ -490,6 +497,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       // read all of it, so that the slot is free for the next copy while this one is converted
       constexpr int kParts = kDirect ? 0 : kUnitsD * (kHalves ? 2 : 1);  // f32: part i of half i & 1
       uint32_t wx[kUnitsX][4], wd[kParts ? kParts : 1][2 * sizeof(T)];
+      auto read_all = [&]() {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int u = 0; u < kUnitsX; ++u) seen += wx[u][0] ^ wx[u][3];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+          for (int q = 0; q < 2 * (int)sizeof(T); q += kVec ? 4 : 1) seen += wd[i][q];
+        if constexpr (!kVec)
+#pragma unroll
+          for (int u = 0; u < kUnitsX; ++u) seen += wx[u][1] ^ wx[u][2];
+        wait_read(seen);
+      };
       if constexpr (kVec) {
         ok = mbar_wait_sleep(raw_full + 8 * sl, (k / kAhead) & 1, abort, a.err, DEV_TIMEOUT_FULL,
                              a.limit);
@@ -507,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ld_shared16(swizzled(raw, i * kRowsD + dr, dj), wd[i]);
           }
         }
+        read_all();
         __syncwarp();
         if (lane == 0) mbar_arrive(raw_empty + 8 * sl);
       } else {
@@ -533,6 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ld_shifted<4>(from, wd[i]);
           }
         }
+        read_all();
         __syncwarp();
         copy_chunk();
         if (cur.in * kChunk + kChunk > a.p) {  // a row's last chunk
