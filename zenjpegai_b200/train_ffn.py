@@ -16,14 +16,16 @@ import argparse
 
 import torch
 
-from . import Engine
+from . import STREAM_LEGACY, Engine
 
 
 class GatedFFN:
     """`depth` halves on maps [dim, h, w]: parameters as float32 CUDA tensors in `params`, a list
-    of dicts; `forward` keeps the tapes that `backward` reads."""
+    of dicts; `forward` keeps the tapes that `backward` reads. The engine works on torch's current
+    stream from here on: its convolutions and torch's own kernels take turns."""
 
     def __init__(self, engine, dim, hidden, depth, seed=0, device="cuda"):
+        engine.set_stream(torch.cuda.current_stream().cuda_stream or STREAM_LEGACY)
         g = torch.Generator().manual_seed(seed)
 
         def normal(*shape, std):
@@ -97,7 +99,7 @@ def main():
     ap.add_argument("--size", type=int, default=128)
     ap.add_argument("--depth", type=int, default=2)
     ap.add_argument("--steps", type=int, default=20)
-    ap.add_argument("--rate", type=float, default=0.2)
+    ap.add_argument("--rate", type=float, default=20.0)
     a = ap.parse_args()
     engine = Engine(0, arena_bytes=1 << 30)
     torch.manual_seed(1)
