@@ -16,11 +16,14 @@
 // three times the instructions, and issue slots bounded the kernels, not HBM). A block takes up to
 // 256 channels, four rows a thread, and a cluster of up to eight blocks up to 2048, reading the
 // partial sums of each other's shared memory. Everything is read once, copied to shared memory a
-// tile ahead (the staged kernels). More channels are read again for each pass. A position's sums go over the warps' shared-memory partials, gathered by four
-// lanes each. Statistics: a mean and sum of squared
-// deviations per warp, joined by their exact update formula (sums of squares would cancel).
+// tile ahead (the staged kernels). More channels are read again for each pass. A position's sums go
+// over the warps' shared-memory partials, gathered by four lanes each. Statistics: a mean and sum of
+// squared deviations per warp, joined by their exact update formula (sums of squares would cancel).
 // The products in a - mean a and b - mean b are the ones that were summed (not fused): with one
-// channel they cancel to zero. Both kernels are bound by HBM at large sizes.
+// channel they cancel to zero.
+// Measured at 28 x 128 x 128^2 in f32 with a full gate: forward with four tapes 296 us of kernel,
+// 5.2 TB/s, and backward from tapes 435 us, 3.1 TB/s: the sixteen warps an SM that the registers
+// leave issue every other cycle, each waiting on its own latencies between the exchanges.
 #pragma once
 #include <algorithm>
 #include <type_traits>

@@ -28,6 +28,9 @@
 //  - one thread issues the MMAs of a chunk, alternating between two accumulator sets in TMEM;
 //  - db comes from the converters' registers, or, where d_out does not pass through them, from a
 //    row of ones below the input's rows in the operand: one more column of the product.
+// At 28 x 128 x 128^2: f32 to 384 channels 204 us (3.7 TB/s; its copies alone take 154), bf16 to 1024
+// 242 us (4.1 TB/s; 198): what is left is a chunk's way through conversion while its places in shared
+// memory are taken.
 // Shares of one tile are summed in order by a second kernel (no atomics). Every wait is bounded.
 #include <algorithm>
 #include <type_traits>
