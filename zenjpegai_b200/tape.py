@@ -22,7 +22,7 @@ STREAM_LEGACY = 1  # CUDA's handle of the legacy default stream, for `Engine.set
 
 _NUMPY_CODE = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
 _F32, _I8 = np.dtype(np.float32), np.dtype(np.int8)
-_torch, _torch_code, _current_stream = None, {}, None
+_torch, _torch_code, _current_stream, _Tensor = None, {}, None, ()
 
 
 def _bad(msg):
@@ -31,17 +31,17 @@ def _bad(msg):
 
 def _is_torch(a):
     """Whether a is a torch tensor; torch is imported when the first one comes."""
-    global _torch, _torch_code, _current_stream
+    global _torch, _torch_code, _current_stream, _Tensor
     if _torch is None:
         if isinstance(a, np.ndarray) or not type(a).__module__.startswith("torch"):
             return False
         import torch
-        _torch = torch
+        _torch, _Tensor = torch, torch.Tensor
         _torch_code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         # the handle of torch's current stream; the raw form makes no Stream object (3 us a call)
         _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda device: torch.cuda.current_stream(device).cuda_stream)
-    return isinstance(a, _torch.Tensor)
+    return isinstance(a, _Tensor)
 
 
 class Tape:
@@ -63,13 +63,13 @@ class _Call:
     """The buffers of one call: the side they lie on (that of `like`), their checks, their pointers
     and new ones like them, and the stream order."""
 
-    __slots__ = ("engine", "cuda", "f32", "i8")
+    __slots__ = ("engine", "device", "cuda", "f32", "i8", "like")
 
     def __init__(self, engine, like):
-        self.engine = engine
-        self.cuda = _is_torch(like)
+        self.engine, self.like = engine, like
+        self.cuda = isinstance(like, _Tensor) or _is_torch(like)
         if self.cuda:
-            self.f32, self.i8 = _torch.float32, _torch.int8
+            self.f32, self.i8, self.device = _torch.float32, _torch.int8, engine.device
             if like.get_device() != engine.device:
                 raise _bad("torch tensors must be CUDA tensors of the engine's GPU")
         elif isinstance(like, np.ndarray):
@@ -87,7 +87,11 @@ class _Call:
     def ptr(self, a, what, shape, dtype):
         """Pointer of an array that must have this shape and type and lie with the others."""
         if self.cuda:
-            if not isinstance(a, _torch.Tensor) or a.get_device() != self.engine.device:
+            # most of a small call's time is spent here: what is wrong is looked at afterwards
+            if (isinstance(a, _Tensor) and a.dtype is dtype and a.shape == shape
+                    and a.is_contiguous() and a.get_device() == self.device):
+                return a.data_ptr()
+            if not isinstance(a, _Tensor) or a.get_device() != self.device:
                 raise _bad("%s must be a tensor of the same GPU" % what)
             contiguous = a.is_contiguous()
         else:
@@ -96,7 +100,7 @@ class _Call:
             contiguous = a.flags.c_contiguous
         if a.dtype != dtype:
             raise _bad("%s has type %s, expected %s" % (what, a.dtype, dtype))
-        if a.shape != shape:
+        if tuple(a.shape) != tuple(shape):
             raise _bad("%s has shape %s, expected %s" % (what, tuple(a.shape), tuple(shape)))
         if not contiguous:
             raise _bad("%s must be contiguous" % what)
@@ -109,13 +113,17 @@ class _Call:
         """zjai_tape of a Tape of a map of this shape."""
         if not isinstance(t, Tape):
             raise _bad("%s must be a Tape" % what)
-        return _lib.TapeC(self.ptr(t.codes, what + ".codes", shape, self.i8),
-                          self.ptr(t.exps, what + ".exps", _exps_shape(shape), self.i8))
+        return _lib.TapeC(self.ptr(t.codes, what, shape, self.i8),
+                          self.ptr(t.exps, what + "'s exponents", _exps_shape(shape), self.i8))
 
     def empty(self, shape, dtype):
         if self.cuda:
-            return _torch.empty(shape, dtype=dtype, device=self.engine.device)
+            return self.like.new_empty(shape, dtype=dtype)
         return np.empty(shape, dtype)
+
+    def empty_like(self):
+        """A map like the one that the call began with."""
+        return _torch.empty_like(self.like) if self.cuda else np.empty_like(self.like)
 
     def at(self, a):
         """Pointer of an array of `empty`."""
@@ -221,8 +229,8 @@ def gated_residual_norm(engine, x, f, post=None, gate=None, scale=None, pre=None
         gshape = _gate_shape(gate, shape)
         pg, gc = call.ptr(gate, "gate", gshape, dt), gshape[-3]
     prm = _params(call, c, post, scale, pre)
-    y = call.empty(shape, dt)
-    z = call.empty(shape, dt) if pre is not None else None
+    y = call.empty_like()
+    z = call.empty_like() if pre is not None else None
     tapes, tc = {}, None
     for name in tape:
         if name not in ("f", "gate", "y", "z"):
@@ -249,37 +257,42 @@ def gated_residual_norm_backward(engine, dy, dz=None, f=None, y=None, post=None,
         raise _bad("dz goes with pre")
     pdz = call.ptr(dz, "dz", shape, dt) if pre is not None else None
     prm = _params(call, c, post, scale, pre)
-    kept = {}
-    if post is not None or scale is not None or gate is not None:
-        kept["f"] = f
-    if pre is not None:
-        kept["y"] = y
-    gshape = None
-    if gate is not None:
-        kept["gate"], gshape = gate, _gate_shape(gate, shape)
-    taped = any(isinstance(v, Tape) for v in kept.values())
-    ptr, tc = {"f": None, "y": None, "gate": None}, _lib.ResidualTapes() if taped else None
-    for name, v in kept.items():
-        if v is None:
+    gated = gate is not None
+    need_f = gated or post is not None or scale is not None
+    need_y = pre is not None
+    gshape = _gate_shape(gate, shape) if gated else None
+    taped = ((need_f and isinstance(f, Tape)) or (need_y and isinstance(y, Tape))
+             or (gated and isinstance(gate, Tape)))
+    for name, v, on in (("f", f, need_f), ("y", y, need_y)):
+        if on and v is None:
             raise _bad("%s is missing" % name)
-        want = gshape if name == "gate" else shape
-        if taped:  # all of them
-            setattr(tc, name, call.tape(v, name, want))
-        else:
-            ptr[name] = call.ptr(v, name, want, dt)
-    out = {"x": call.empty(shape, dt), "f": call.empty(shape, dt)}
-    if gate is not None:
-        out["gate"] = call.empty(gshape, dt)
-    names = ((["post_weight", "post_bias"] if post is not None else [])
-             + (["scale"] if scale is not None else [])
-             + (["pre_weight", "pre_bias"] if pre is not None else []))
-    if names:  # rows of one array
-        out.update(zip(names, call.empty((len(names), c), call.f32)))
-    gr = _lib.ResidualGrads()
-    for k, v in out.items():
-        setattr(gr, k, call.at(v))
-    call(_lib.lib().zjai_gated_residual_norm_backward, pdy, pdz, ptr["f"], ptr["gate"],
-         gshape[-3] if gshape else 0, ptr["y"], ctypes.byref(tc) if taped else None, code, n, c, h,
+    pf = pg = py = tc = None
+    if taped:  # all of them
+        none = _lib.TapeC()
+        tc = _lib.ResidualTapes(call.tape(f, "f", shape) if need_f else none,
+                                call.tape(gate, "gate", gshape) if gated else none,
+                                call.tape(y, "y", shape) if need_y else none)
+    else:
+        pf = call.ptr(f, "f", shape, dt) if need_f else None
+        pg = call.ptr(gate, "gate", gshape, dt) if gated else None
+        py = call.ptr(y, "y", shape, dt) if need_y else None
+    dx, df = call.empty_like(), call.empty_like()
+    out, pgate = {"x": dx, "f": df}, None
+    if gated:
+        out["gate"] = call.empty_like() if gshape == shape else call.empty(gshape, dt)
+        pgate = call.at(out["gate"])
+    rows, at = None, [None] * 5
+    count = 2 * (post is not None) + (scale is not None) + 2 * need_y
+    if count:  # rows of one array
+        rows = call.empty((count, c), call.f32)
+        first, rows = call.at(rows), iter(rows.unbind() if call.cuda else rows)
+        for i, (name, on) in enumerate((("post_weight", post), ("post_bias", post), ("scale", scale),
+                                        ("pre_weight", pre), ("pre_bias", pre))):
+            if on is not None:
+                out[name], at[i], first = next(rows), first, first + 4 * c
+    gr = _lib.ResidualGrads(call.at(dx), call.at(df), pgate, *at)
+    call(_lib.lib().zjai_gated_residual_norm_backward, pdy, pdz, pf, pg,
+         gshape[-3] if gated else 0, py, ctypes.byref(tc) if taped else None, code, n, c, h,
          w, ctypes.byref(prm), ctypes.byref(gr))
     return out
 
