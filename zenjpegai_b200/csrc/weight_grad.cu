@@ -709,14 +709,14 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const float* __restrict_
 }
 
 // Ranges per tile: the fewest rounds of CTAs over the SMs times the chunks of a range, with a few
-// chunks' time for what a CTA does once (start, write its partial tile).
+// chunks' time for what a CTA does once (start, write its partial tile) and for the second launch.
 int choose_splits(long long tiles, long long chunks, int sms) {
   long long best = 1;
   double cost = 1e300;
   const long long most = std::min<long long>({chunks, std::max<long long>(1, 4LL * sms / tiles), 1024});
   for (long long s = 1; s <= most; ++s) {
     const double rounds = (double)((tiles * s + sms - 1) / sms);
-    const double t = rounds * ((double)((chunks + s - 1) / s) + 8.0) + (s > 1 ? 2.0 : 0.0);
+    const double t = rounds * ((double)((chunks + s - 1) / s) + 8.0) + (s > 1 ? 6.0 : 0.0);
     if (t < cost) cost = t, best = s;
   }
   return (int)best;

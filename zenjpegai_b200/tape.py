@@ -63,10 +63,10 @@ class _Call:
     """The buffers of one call: the side they lie on (that of `like`), their checks, their pointers
     and new ones like them, and the stream order."""
 
-    __slots__ = ("engine", "device", "cuda", "f32", "i8", "like")
+    __slots__ = ("engine", "device", "cuda", "f32", "i8", "like", "shape", "groups")
 
     def __init__(self, engine, like):
-        self.engine, self.like = engine, like
+        self.engine, self.like, self.shape, self.groups = engine, like, None, None
         self.cuda = isinstance(like, _Tensor) or _is_torch(like)
         if self.cuda:
             self.f32, self.i8, self.device = _torch.float32, _torch.int8, engine.device
@@ -114,23 +114,33 @@ class _Call:
         if not isinstance(t, Tape):
             raise _bad("%s must be a Tape" % what)
         return _lib.TapeC(self.ptr(t.codes, what, shape, self.i8),
-                          self.ptr(t.exps, what + "'s exponents", _exps_shape(shape), self.i8))
+                          self.ptr(t.exps, what, self.exps_shape(shape), self.i8))
+
+    def exps_shape(self, shape):
+        if shape == self.shape:
+            return self.groups
+        groups = -(-(shape[-2] * shape[-1]) // GROUP)
+        self.shape, self.groups = shape, tuple(shape[:-2]) + (groups,)
+        return self.groups
 
     def empty(self, shape, dtype):
         if self.cuda:
             return self.like.new_empty(shape, dtype=dtype)
         return np.empty(shape, dtype)
 
-    def empty_like(self):
-        """A map like the one that the call began with."""
-        return _torch.empty_like(self.like) if self.cuda else np.empty_like(self.like)
+    def empty_like(self, dtype=None):
+        """A map like the one that the call began with (of an element type)."""
+        empty = _torch.empty_like if self.cuda else np.empty_like
+        return empty(self.like, dtype=dtype)
 
     def at(self, a):
         """Pointer of an array of `empty`."""
         return a.data_ptr() if self.cuda else a.ctypes.data
 
-    def new_tape(self, shape):
-        t = Tape(self.empty(shape, self.i8), self.empty(_exps_shape(shape), self.i8))
+    def new_tape(self, shape, like=False):
+        """A tape of a map of this shape (like: that of the map that the call began with)."""
+        codes = self.empty_like(self.i8) if like else self.empty(shape, self.i8)
+        t = Tape(codes, self.empty(self.exps_shape(shape), self.i8))
         return t, _lib.TapeC(self.at(t.codes), self.at(t.exps))
 
     def __call__(self, f, *args):
@@ -149,10 +159,6 @@ class _Call:
         check(L.zjai_ctx_release_stream(h, cur))
 
 
-def _exps_shape(shape):
-    return tuple(shape[:-2]) + (-(-(shape[-2] * shape[-1]) // GROUP),)
-
-
 def _dims(shape, what):
     """(n, c, h, w) of a map's shape."""
     if len(shape) == 4:
@@ -169,7 +175,7 @@ def tape_pack(engine, x):
     n, c, h, w = _dims(shape, "x")
     px = call.ptr(x, "x", shape, x.dtype)
     code = call.code(x, "x")
-    t, tc = call.new_tape(tuple(shape))
+    t, tc = call.new_tape(tuple(shape), True)
     call(_lib.lib().zjai_tape_pack, px, code, n, c, h, w, ctypes.byref(tc))
     return t
 
@@ -182,7 +188,7 @@ def tape_unpack(engine, tape, dtype=None):
     shape = tape.shape
     n, c, h, w = _dims(shape, "tape")
     tc = call.tape(tape, "tape", shape)
-    x = call.empty(shape, dtype or call.f32)
+    x = call.empty_like(dtype or call.f32)  # (the codes' shape)
     call(_lib.lib().zjai_tape_unpack, ctypes.byref(tc), n, c, h, w, call.at(x),
          call.code(x, "the unpacked map"))
     return x
@@ -238,7 +244,8 @@ def gated_residual_norm(engine, x, f, post=None, gate=None, scale=None, pre=None
         if (name == "gate" and gate is None) or (name == "z" and pre is None):
             continue
         tc = tc or _lib.ResidualTapes()
-        tapes[name], one = call.new_tape(gshape if name == "gate" else shape)
+        gates = name == "gate"
+        tapes[name], one = call.new_tape(gshape if gates else shape, not gates or gshape == shape)
         setattr(tc, name, one)
     call(_lib.lib().zjai_gated_residual_norm, px, pf, pg, gc, code, n, c, h, w, ctypes.byref(prm),
          call.at(y), call.at(z) if z is not None else None, ctypes.byref(tc) if tc else None)
