@@ -322,8 +322,8 @@ struct Tiles {
 //     before or behind the tensor no more than an aligned 8 bytes' rest is touched, never a whole
 //     one), neighbouring ones by neighbouring lanes, are shifted into place when read, and go through
 //     shared memory to whole rows. (For f32 that takes more instructions than it saves sectors:
-//     backward, 8 x 128 x 127 x 129 taped, 248 us so and 223 us one by one; bf16 190 us so and
-//     220 us one by one.)
+//     backward, 8 x 128 x 127 x 129 taped, 248 us so and 223 one by one, 200 with the L1 cache that one
+//     slot leaves; bf16 190 us so and 220 one by one.)
 enum { kWholeTiles, kAligned, kAnywhere };
 // the first `bytes` (1 to 4) of an aligned word, zeros behind them
 __device__ __forceinline__ void stage_copy_some(char* dst, const void* src, int bytes) {

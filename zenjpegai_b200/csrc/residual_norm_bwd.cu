@@ -50,10 +50,11 @@ struct BwdSlot {
   static constexpr int kMaps = kStagedRows * (2 * Grad::kBytes + 3 * Kept::kBytes);
   static constexpr int kExps = kTaped ? 3 * 4 * kStagedRows * 4 : 0;
   static constexpr int kB = sizeof(T) == 4 ? 0 : kStagedRows * 32 * (int)sizeof(float4);
-  // two slots where 227 KB hold them
+  // two slots where 227 KB hold them; one for rows that start anywhere, whose copies want the rest as
+  // L1 cache (8 x 128 x 127 x 129 taped, two and one: f32 227 and 200 us, bf16 189 and 181 us)
   static constexpr int kRest = tail_bytes<4>(kBlockC, kMaxWarps) + 9 * 32 * (int)sizeof(float);
   static constexpr int kSlots =
-      (2 * (kMaps + kExps) + kB) * kMaxWarps + kRest <= 227 * 1024 ? 2 : 1;
+      kMode != kAnywhere && (2 * (kMaps + kExps) + kB) * kMaxWarps + kRest <= 227 * 1024 ? 2 : 1;
   static constexpr int kBytes = kSlots * (kMaps + kExps) + kB;
 };
 template <int kMode, bool kTaped, class T>
