@@ -15,7 +15,13 @@ struct FwdArgs {
   zjai_residual_tapes tp;
 };
 
-// Rows held, the next tile copied ahead into the other of two slots.
+// Rows held, the next tile copied ahead into the other of two slots; with one, as soon as the current
+// one has been read: rows that start anywhere, whose copies want the rest as L1 cache (8 x 128 x 127 x
+// 129, two and one: f32 146 and 114 us, bf16 98 and 94 us).
+template <int kMode>
+constexpr int fwd_slots() {
+  return kMode == kAnywhere ? 1 : 2;
+}
 template <int kMode, class T>
 constexpr int fwd_slot_bytes() {  // per warp: f, x and the gate's logits
   return 3 * kStagedRows * Region<kMode, T>::kBytes;
@@ -36,10 +42,11 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   const float inv_c = 1.f / (float)a.c;
   const bool post = a.prm.post_weight, pre = a.prm.pre_weight, per_row = a.gate_c > 1;
   const StagedRows<kMode> row(c, a.p, groups);
-  char* mine = slots + wp * 2 * fwd_slot_bytes<kMode, T>();
+  constexpr int kSlots = fwd_slots<kMode>();
+  char* mine = slots + wp * kSlots * fwd_slot_bytes<kMode, T>();
   Params<kRows> prm = {nullptr, a.share};
   Exchange<2> ex = {nullptr, totals};
-  take_tail(slots + warps * 2 * fwd_slot_bytes<kMode, T>(), a.share, &prm.v, &ex);
+  take_tail(slots + warps * kSlots * fwd_slot_bytes<kMode, T>(), a.share, &prm.v, &ex);
   auto place = [&](int slot, int k, int j) {
     return mine + ((slot * 3 + k) * kRows + j) * R::kBytes;
   };
@@ -56,11 +63,12 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   Tiles tile(a.tiles, groups, cl.size), ahead = tile;
   if (ahead.on()) copy(ahead, 0);
   stage_commit();
-  for (int slot = 0; tile.on(); tile.next(), slot ^= 1) {
+  for (int slot = 0; tile.on(); tile.next(), slot ^= kSlots - 1) {
     ahead.next();
-    if (!kVec) __syncwarp();  // the other slot has been read by all lanes
-    if (ahead.on()) copy(ahead, slot ^ 1);
-    stage_commit();
+    if (kSlots == 2) {
+      if (ahead.on()) copy(ahead, slot ^ 1);
+      stage_commit();
+    }
     const int at = tile.g * kTapeGroup + (lane & 7) * 4;
     const int nv = kWhole ? 4 : a.p - at;
     const long long e0 = ((long long)tile.img * a.c + ch0) * a.p + tile.g * kTapeGroup;
@@ -70,12 +78,10 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
       gate1 = load4<kVec>(a.gate + (long long)tile.img * a.p, at, a.p);
       sigmoid4(gate1, &sg1, &unused);
     }
-    stage_wait<1>();
-    if (!kVec) __syncwarp();  // and the current one copied by all
-    // a row's f has been read before anything of it is stored: its place is free
-    auto scratch = [&](int j) { return reinterpret_cast<float*>(place(slot, 0, j)); };
+    stage_wait<kSlots - 1>();
+    if (!kVec) __syncwarp();  // what other lanes copied
     auto hold = [&](const zjai_tape& t, int j, F4 v) {
-      staged_hold<kMode>(t.codes + e0, t.exps + x0, v, row, j, nv, scratch(j));
+      staged_hold<kMode>(t.codes + e0, t.exps + x0, v, row, j, nv, ex.at(0, wp));
     };
     F4 nm = all(0.f), r = all(1.f);  // of f, then of y: the negated mean and 1 / sigma
     auto exchange = [&](auto v) {
@@ -107,8 +113,13 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
         if (a.tp.gate.codes) hold(a.tp.gate, j, g);
       }
       y[j] = fma4(s * prm.get(a.prm, kScale, row.ch(j)), u, get(a.x, 1, j));
-      staged_store<kMode>(a.y + e0, y[j], row, j, nv, scratch(j));
+      staged_store<kMode>(a.y + e0, y[j], row, j, nv, ex.at(0, wp));
       if (a.tp.y.codes) hold(a.tp.y, j, kWhole ? y[j] : clip4<kVec>(y[j], at, a.p));
+    }
+    if (kSlots == 1) {
+      __syncwarp();  // read, before another lane copies over it
+      if (ahead.on()) copy(ahead, 0);
+      stage_commit();
     }
     if (!pre) continue;
     exchange([&](int j) { return y[j]; });
@@ -116,7 +127,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     for (int j = 0; j < kRows; ++j) {
       const F4 z =
           fma4((y[j] + nm) * r, prm.get(a.prm, kPreW, row.ch(j)), prm.get(a.prm, kPreB, row.ch(j)));
-      staged_store<kMode>(a.z + e0, z, row, j, nv, scratch(j));
+      staged_store<kMode>(a.z + e0, z, row, j, nv, ex.at(0, wp));
       if (a.tp.z.codes) hold(a.tp.z, j, kWhole ? z : clip4<kVec>(z, at, a.p));
     }
   }
@@ -256,7 +267,7 @@ int zjai_gated_residual_norm(zjai_ctx* ctx, const void* x, const void* f, const 
         smem = by_mode(sh.mode, [&](auto m) {
           constexpr int kMode = decltype(m)::value;
           k = residual_norm_staged_kernel<kMode, T>;
-          return 2 * fwd_slot_bytes<kMode, T>() * sh.warps +
+          return fwd_slots<kMode>() * fwd_slot_bytes<kMode, T>() * sh.warps +
                  tail_bytes<2>(sh.share, sh.warps);
         });
       int count = 0;
