@@ -98,6 +98,10 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
   auto exp_at = [&](int slot, int k, int r) {
     return mine + S::kSlots * S::kMaps + ((slot * 3 + k) * kWarpRows + r) * 4;
   };
+  // how far behind an aligned word a tape's exponents begin (kVec: they begin with one)
+  auto exp_sub = [](const zjai_tape& tp) {
+    return kVec ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(tp.exps) & 3u;
+  };
   // b of a row, until df: where dy was, or (f16, bf16) in a place of its own
   auto b_at = [&](int slot, int j) {
     return reinterpret_cast<float4*>(sizeof(T) == 4 ? grad_at(slot, 0, j)
@@ -114,10 +118,14 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     auto keep_exps = [&](const zjai_tape& tp, int k) {
       const int ch = wp * kWarpRows + lane;
       if (lane >= kWarpRows || (!kWhole && ch >= c)) return;
-      const uint32_t at = ((uint32_t)(x & 3) + (uint32_t)ch * (uint32_t)groups) & ~3u;
-      const int8_t* src = tp.exps + (x & ~3LL) + at;
+      // counted from the aligned word that holds the tape's first exponent: of memory before or
+      // behind the tape no more than the rest of a word with one of its bytes is touched
+      const uint32_t sub = exp_sub(tp);
+      const long long first = (x + sub) & ~3LL;
+      const uint32_t at = ((uint32_t)((x + sub) & 3) + (uint32_t)ch * (uint32_t)groups) & ~3u;
+      const int8_t* src = tp.exps - sub + first + at;
       // whole tiles: a multiple of four exponents in all
-      const int bytes = kWhole ? 4 : (int)min(4LL, x_all - (x & ~3LL) - at);
+      const int bytes = kWhole ? 4 : (int)min(4LL, x_all + sub - first - at);
       stage_copy_some(exp_at(slot, k, lane), src, bytes);
     };
     if (kTaped) {
@@ -158,7 +166,7 @@ __global__ void __launch_bounds__(kThreadsMost, 1)
     auto kept = [&](const T* map, const zjai_tape& tp, int k, int j) {
       if constexpr (kTaped) {
         const uint32_t w = *reinterpret_cast<const uint32_t*>(exp_at(slot, k, j * 4 + (lane >> 3)));
-        const int e = (int)(int8_t)(w >> ((x0 + row.x(j)) & 3) * 8);
+        const int e = (int)(int8_t)(w >> ((x0 + row.x(j) + exp_sub(tp)) & 3) * 8);
         return taped4(S::Kept::words(kept_at(slot, k, j), tp.codes + e0, row, j, nv).x, e);
       } else {
         return S::Kept::get(kept_at(slot, k, j), map + e0, row, j, nv);
