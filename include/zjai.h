@@ -88,7 +88,10 @@ int zjai_ctx_create(int device, size_t arena_bytes, zjai_ctx **out);
 int zjai_ctx_destroy(zjai_ctx *ctx);
 
 /* Use the caller's CUDA stream (a cudaStream_t) instead of the context's own; NULL restores
- * the context's stream. */
+ * the context's stream. The stream must stay valid until another one is set or the context is
+ * destroyed. Calls share the context's arena, so the new stream first waits for what the last one
+ * holds; not while one of the two is capturing: what was captured is the caller's to order against
+ * the context's other work. */
 int zjai_ctx_set_stream(zjai_ctx *ctx, void *cuda_stream);
 
 /* Wait for all work enqueued on the context's stream, then report a kernel status word

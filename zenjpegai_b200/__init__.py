@@ -97,7 +97,8 @@ class Engine:
 
     def set_stream(self, cuda_stream_ptr):
         """Work on the caller's CUDA stream (its handle as an int; STREAM_LEGACY for torch's default
-        stream); 0 or None restores the context's own."""
+        stream); 0 or None restores the context's own. The new stream first waits for the engine's
+        work on the last one, which must still exist."""
         check(_lib.lib().zjai_ctx_set_stream(self.handle, ctypes.c_void_p(cuda_stream_ptr)))
         self.stream = cuda_stream_ptr or None
 

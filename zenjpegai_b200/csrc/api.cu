@@ -194,7 +194,23 @@ int zjai_ctx_destroy(zjai_ctx* ctx) {
 
 int zjai_ctx_set_stream(zjai_ctx* ctx, void* s) {
   ZJAI_TRY(ctx_enter(ctx));
-  ctx->stream = s ? static_cast<cudaStream_t>(s) : ctx->own;
+  cudaStream_t next = s ? static_cast<cudaStream_t>(s) : ctx->own;
+  if (next == ctx->stream) return ZJAI_OK;
+  // Calls on either stream take their scratch from the same arena: the next one's wait for what the
+  // last one holds. Not while either is capturing: a graph's work runs when the graph does, and
+  // neither stream can wait for the other (the query also fails for the legacy stream beside a
+  // capture).
+  cudaStreamCaptureStatus last_status, next_status;
+  const bool known = cudaStreamIsCapturing(ctx->stream, &last_status) == cudaSuccess &&
+                     cudaStreamIsCapturing(next, &next_status) == cudaSuccess;
+  if (!known) {
+    cudaGetLastError();
+  } else if (last_status == cudaStreamCaptureStatusNone &&
+             next_status == cudaStreamCaptureStatusNone) {
+    ZJAI_TRY(cuda_check(cudaEventRecord(ctx->ev_caller, ctx->stream), "stream order"));
+    ZJAI_TRY(cuda_check(cudaStreamWaitEvent(next, ctx->ev_caller, 0), "stream order"));
+  }
+  ctx->stream = next;
   return ZJAI_OK;
 }
 
