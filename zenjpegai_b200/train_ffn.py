@@ -13,19 +13,31 @@ Usage: python -m zenjpegai_b200.train_ffn [--dim C] [--hidden C] [--size S] [--d
 """
 
 import argparse
+import contextlib
 
 import torch
 
 from . import STREAM_LEGACY, Engine
 
 
+@contextlib.contextmanager
+def _on_current_stream(engine):
+    """The engine on torch's current stream, where its layers and torch's own kernels take turns; then
+    on the one that it was set to before."""
+    before = engine.stream
+    engine.set_stream(torch.cuda.current_stream(engine.device).cuda_stream or STREAM_LEGACY)
+    try:
+        yield
+    finally:
+        engine.set_stream(before)
+
+
 class GatedFFN:
     """`depth` halves on maps [dim, h, w]: parameters as float32 CUDA tensors in `params`, a list
-    of dicts; `forward` keeps the tapes that `backward` reads. The engine works on torch's current
-    stream from here on: its convolutions and torch's own kernels take turns."""
+    of dicts; `forward` keeps the tapes that `backward` reads. Each pass works on the stream that is
+    torch's current one as it is called, and leaves the engine's stream as it was."""
 
     def __init__(self, engine, dim, hidden, depth, seed=0, device="cuda"):
-        engine.set_stream(torch.cuda.current_stream().cuda_stream or STREAM_LEGACY)
         g = torch.Generator().manual_seed(seed)
 
         def normal(*shape, std):
@@ -52,6 +64,10 @@ class GatedFFN:
 
     def forward(self, x, gate=None):
         """x [dim, h, w] and the gate's logits, [1, h, w] or like x: the last half's (y, z)."""
+        with _on_current_stream(self.engine):
+            return self._forward(x, gate)
+
+    def _forward(self, x, gate):
         e, z = self.engine, x
         self.tapes = []
         for p, w_dw in zip(self.params, self.w_dw):
@@ -68,6 +84,10 @@ class GatedFFN:
     def backward(self, dy, dz):
         """From the gradients of the last half's y and z: those of x and of the gate (None without
         one), and of each half's parameters."""
+        with _on_current_stream(self.engine):
+            return self._backward(dy, dz)
+
+    def _backward(self, dy, dz):
         e, grads, dgate = self.engine, [], None
         for p, w_dw, t in zip(self.params[::-1], self.w_dw[::-1], self.tapes[::-1]):
             h, w = dy.shape[1:]
