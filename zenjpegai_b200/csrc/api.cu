@@ -92,8 +92,11 @@ int stage_out_finish(Ctx* ctx, float* host, const float* dev, size_t n, int mem)
 }
 
 // Host copy of a caller array that the host must read (weights, biases, LN parameters):
-// device arrays are copied down, host arrays are used in place.
-int fetch_host(const float* p, size_t n, int mem, std::vector<float>* buf, const float** out) {
+// device arrays are copied down, host arrays are used in place. The copy is ordered after the
+// context's stream (a caller's, perhaps, that does not synchronise with the legacy stream) and, as a
+// copy on that, after the legacy stream.
+int fetch_host(Ctx* ctx, const float* p, size_t n, int mem, std::vector<float>* buf,
+               const float** out) {
   if (!p) {
     *out = nullptr;
     return ZJAI_OK;
@@ -103,6 +106,7 @@ int fetch_host(const float* p, size_t n, int mem, std::vector<float>* buf, const
     return ZJAI_OK;
   }
   buf->resize(n);
+  ZJAI_TRY(cuda_check(cudaStreamSynchronize(ctx->stream), "stream sync"));
   ZJAI_TRY(cuda_check(cudaMemcpy(buf->data(), p, n * sizeof(float), cudaMemcpyDeviceToHost),
                       "parameter D2H"));
   *out = buf->data();
@@ -344,8 +348,8 @@ int zjai_conv2d(zjai_ctx* ctx, const float* x, int c, int h, int w, const float*
   std::vector<float> wbuf, bbuf;
   const float *hw, *hb;
   if (groups <= 0 || c % groups) return fail(ZJAI_INVALID_ARGUMENT, "conv2d: groups");
-  ZJAI_TRY(fetch_host(weight, (size_t)oc * (c / groups) * kh * kw, mem, &wbuf, &hw));
-  ZJAI_TRY(fetch_host(bias, (size_t)oc, mem, &bbuf, &hb));
+  ZJAI_TRY(fetch_host(ctx, weight, (size_t)oc * (c / groups) * kh * kw, mem, &wbuf, &hw));
+  ZJAI_TRY(fetch_host(ctx, bias, (size_t)oc, mem, &bbuf, &hb));
   ConvLayer L;
   ZJAI_TRY(pack_conv(ctx, &L, hw, hb, c, oc, kh, kw, stride, pad_h, pad_w, groups, extra, 1));
   LayerGuard guard(&L);
@@ -379,8 +383,8 @@ int zjai_conv_transpose2d(zjai_ctx* ctx, const float* x, int c, int h, int w,
   ArenaScope scope(ctx);
   std::vector<float> wbuf, bbuf;
   const float *hw, *hb;
-  ZJAI_TRY(fetch_host(weight, (size_t)c * oc * k * k, mem, &wbuf, &hw));
-  ZJAI_TRY(fetch_host(bias, (size_t)oc, mem, &bbuf, &hb));
+  ZJAI_TRY(fetch_host(ctx, weight, (size_t)c * oc * k * k, mem, &wbuf, &hw));
+  ZJAI_TRY(fetch_host(ctx, bias, (size_t)oc, mem, &bbuf, &hb));
   ConvLayer L;
   ZJAI_TRY(pack_convT(ctx, &L, hw, hb, c, oc, k, pad, out_pad, 1));
   LayerGuard guard(&L);

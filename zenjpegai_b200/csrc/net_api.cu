@@ -980,9 +980,9 @@ int zjai_transformer_ffn(zjai_ctx* ctx, const float* x, int c, int h, int w, int
   ArenaScope scope(ctx);
   std::vector<float> bi, bd, bo;
   const float *hi, *hd, *ho;
-  ZJAI_TRY(fetch_host(w_in, (size_t)2 * hidden * c, mem, &bi, &hi));
-  ZJAI_TRY(fetch_host(w_dw, (size_t)2 * hidden * 9, mem, &bd, &hd));
-  ZJAI_TRY(fetch_host(w_out, (size_t)c * hidden, mem, &bo, &ho));
+  ZJAI_TRY(fetch_host(ctx, w_in, (size_t)2 * hidden * c, mem, &bi, &hi));
+  ZJAI_TRY(fetch_host(ctx, w_dw, (size_t)2 * hidden * 9, mem, &bd, &hd));
+  ZJAI_TRY(fetch_host(ctx, w_out, (size_t)c * hidden, mem, &bo, &ho));
   FfnLayer F;
   struct Guard {
     FfnLayer* f;

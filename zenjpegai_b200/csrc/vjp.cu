@@ -478,7 +478,7 @@ int zjai_conv2d_backward(zjai_ctx* ctx, const float* dout, int oc, int oh, int o
   const int icg = c / groups;
   std::vector<float> wbuf;
   const float* hw;
-  ZJAI_TRY(fetch_host(weight, (size_t)oc * icg * kh * kw, mem, &wbuf, &hw));
+  ZJAI_TRY(fetch_host(ctx, weight, (size_t)oc * icg * kh * kw, mem, &wbuf, &hw));
   const float* dd;
   ZJAI_TRY(stage_in(ctx, dout, (size_t)oc * oh * ow, mem, &dd));
   float* ddin;
@@ -512,7 +512,7 @@ int zjai_conv_transpose2d_backward(zjai_ctx* ctx, const float* dout, int oc, int
   ArenaScope scope(ctx);
   std::vector<float> wbuf;
   const float* hw;
-  ZJAI_TRY(fetch_host(weight, (size_t)c * oc * k * k, mem, &wbuf, &hw));
+  ZJAI_TRY(fetch_host(ctx, weight, (size_t)c * oc * k * k, mem, &wbuf, &hw));
   const float* dd;
   ZJAI_TRY(stage_in(ctx, dout, (size_t)oc * oh * ow, mem, &dd));
   float* ddin;
@@ -536,8 +536,8 @@ int zjai_residual_block_backward(zjai_ctx* ctx, const float* dout, const float* 
   const size_t n = (size_t)c * h * w, nw = (size_t)c * c * 9;
   std::vector<float> b1, b2;
   const float *h1, *h2;
-  ZJAI_TRY(fetch_host(w1, nw, mem, &b1, &h1));
-  ZJAI_TRY(fetch_host(w2, nw, mem, &b2, &h2));
+  ZJAI_TRY(fetch_host(ctx, w1, nw, mem, &b1, &h1));
+  ZJAI_TRY(fetch_host(ctx, w2, nw, mem, &b2, &h2));
   const float *dd, *dp;
   ZJAI_TRY(stage_in(ctx, dout, n, mem, &dd));
   ZJAI_TRY(stage_in(ctx, conv1_out, n, mem, &dp));
@@ -573,7 +573,7 @@ int zjai_cab_backward(zjai_ctx* ctx, const float* dout, int c, int h, int w,
   const size_t n = (size_t)c * h * w, nm = (size_t)c * mh * mw, nw = (size_t)c * c * 9;
   std::vector<float> wb[10];
   const float* hw[10];
-  for (int i = 0; i < 10; ++i) ZJAI_TRY(fetch_host(wp[i], nw, mem, &wb[i], &hw[i]));
+  for (int i = 0; i < 10; ++i) ZJAI_TRY(fetch_host(ctx, wp[i], nw, mem, &wb[i], &hw[i]));
   const float *dd, *dt[6];
   ZJAI_TRY(stage_in(ctx, dout, n, mem, &dd));
   for (int i = 0; i < 6; ++i) ZJAI_TRY(stage_in(ctx, tp[i], i < 4 ? n : nm, mem, &dt[i]));
@@ -706,7 +706,7 @@ int zjai_transformer_block_backward(zjai_ctx* ctx, const float* dout, int dim, i
   const size_t wn[9] = {(size_t)dim, (size_t)3 * dim * dim, (size_t)3 * dim * 9, (size_t)heads,
                         (size_t)dim * dim, (size_t)dim, (size_t)2 * hidden * dim,
                         (size_t)2 * hidden * 9, (size_t)dim * hidden};
-  for (int i : {1, 2, 4, 6, 7, 8}) ZJAI_TRY(fetch_host(wp[i], wn[i], mem, &wb[i], &hw[i]));
+  for (int i : {1, 2, 4, 6, 7, 8}) ZJAI_TRY(fetch_host(ctx, wp[i], wn[i], mem, &wb[i], &hw[i]));
   const float *dd, *dt[5], *dprep_norm, *dtemp, *dffn_norm;
   ZJAI_TRY(stage_in(ctx, dout, (size_t)dim * n, mem, &dd));
   for (int i = 0; i < 5; ++i) ZJAI_TRY(stage_in(ctx, tp[i], tn[i], mem, &dt[i]));
