@@ -98,8 +98,8 @@ int zjai_ctx_set_stream(zjai_ctx *ctx, void *cuda_stream);
  * (ZJAI_DEVICE_TIMEOUT) if a bounded wait gave up. */
 int zjai_ctx_sync(zjai_ctx *ctx);
 
-/* Limit of the convolution kernel's pipeline waits (a stage, a halo or an accumulator that
- * does not arrive), in SM clock cycles; 0 restores the default of 4e9 cycles (about 2 s at
+/* Limit of the pipeline waits of the convolution kernel and of the 1x1 weight gradient's (a stage, a
+ * halo or an accumulator that does not arrive), in SM clock cycles; 0 restores the default of 4e9 cycles (about 2 s at
  * the boost clock). A wait that runs out makes the kernel record its status word, drain the
  * copies and MMAs it has in flight and end; the next synchronising call on the context then
  * returns ZJAI_DEVICE_TIMEOUT, clears the status word, and the context stays usable. No

@@ -129,15 +129,17 @@ __device__ __forceinline__ bool mbar_wait_idle(uint32_t bar, uint32_t parity, vo
   }
 }
 
-// mbar_wait whose polls sleep in the barrier unit (up to 20 us each) while the phase is
-// incomplete: for many threads waiting on one barrier at once.
+// mbar_wait whose polls sleep in the barrier unit while the phase is incomplete: for many threads
+// waiting on one barrier at once. A poll sleeps up to 20 us; under a limit below that (40000 cycles)
+// none does, so that the limit holds.
 __device__ __forceinline__ bool mbar_wait_sleep(uint32_t bar, uint32_t parity,
                                                 volatile int* abort, int* err, int code,
                                                 long long limit = kWaitCycles) {
   if (mbar_test(bar, parity)) return true;
   const long long t0 = clock64();
+  const bool sleeps = limit >= 40000;
   for (;;) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    if (sleeps ? mbar_try_wait_sleep(bar, parity, 20000u) : mbar_test(bar, parity)) return true;
     if (*abort) return false;
     if (clock64() - t0 > limit) {
       atomicCAS(err, 0, code);

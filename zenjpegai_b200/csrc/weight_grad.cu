@@ -31,7 +31,9 @@
 // At 28 x 128 x 128^2: f32 to 384 channels 204 us (3.7 TB/s; its copies alone take 154), bf16 to 1024
 // 242 us (4.1 TB/s; 198): what is left is a chunk's way through conversion while its places in shared
 // memory are taken.
-// Shares of one tile are summed in order by a second kernel (no atomics). Every wait is bounded.
+// Shares of one tile are summed in order by a second kernel (no atomics). Every wait is bounded
+// (zjai_ctx_set_wait_limit); a role whose time is up has the others give up too, and the CTA ends once
+// its copies and MMAs in flight have.
 #include <algorithm>
 #include <type_traits>
 
@@ -194,8 +196,13 @@ __device__ __forceinline__ void clip_words(uint32_t* w, int valid) {
 // Before a slot is given to the next copy: the registers of each vector that was read from it have
 // their values, in all lanes. (Arriving at the slot's barrier does not say so: the next chunk's copy
 // was seen to land before reads issued ahead of the arrival.) `seen` combines a register of each.
-__device__ __forceinline__ void wait_read(uint32_t seen) {
-  if (__all_sync(0xffffffffu, seen == 0x9e3779b9u)) __nanosleep(1);  // any use will do
+// One answer for the whole warp: whether `ok` holds in all lanes.
+__device__ __forceinline__ bool wait_read(uint32_t seen, bool ok) {
+  if (!__all_sync(0xffffffffu, ok && seen != 0x9e3779b9u)) {
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    __nanosleep(1);  // any use of `seen` will do
+  }
+  return true;
 }
 
 // 4 codes -> 4 bf16 values code 2^e: the low 7 bits and the sign bit of a code, each as the low
@@ -445,6 +452,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       ahead.next();
     };
 
+    // A warp's wait, with one answer for all its lanes: a warp whose time is up leaves as a whole, and
+    // no lane of it is left alone in a vote, a warp barrier or a TMEM load. (The wait for a copied
+    // chunk gets its answer from wait_read's vote.)
+    auto wait = [&](uint32_t bar, int phase, int code) {
+      return __all_sync(0xffffffffu,
+                        mbar_wait_sleep(bar, phase & 1, abort, a.err, code, a.limit)) != 0;
+    };
+
     // accumulator rows 32 (warp % 4) + lane, columns 32 (warp / 4) ..
     float acc[32], acc_db = 0.f;
 #pragma unroll
@@ -453,11 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int drained = 0;
     auto drain_window = [&]() {
       const int buf = drained & 1;
-      if (!mbar_wait_sleep(acc_full + 8 * buf, (drained >> 1) & 1, abort, a.err,
-                           DEV_TIMEOUT_ACC_FULL, a.limit))
-        return false;
+      if (!wait(acc_full + 8 * buf, drained >> 1, DEV_TIMEOUT_ACC_FULL)) return false;
       tc_fence_after();
-      __syncwarp();
       const uint32_t base = tmem + ((uint32_t)(warp & 3) * 32u << 16) + buf * kBufCols;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -500,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // read all of it, so that the slot is free for the next copy while this one is converted
       constexpr int kParts = kDirect ? 0 : kUnitsD * (kHalves ? 2 : 1);  // f32: part i of half i & 1
       uint32_t wx[kUnitsX][4], wd[kParts ? kParts : 1][2 * sizeof(T)];
-      auto read_all = [&]() {
+      auto read_all = [&](bool copied_in) {
         uint32_t seen = 0;
 #pragma unroll
         for (int u = 0; u < kUnitsX; ++u) seen += wx[u][0] ^ wx[u][3];
@@ -511,12 +523,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (!kVec)
 #pragma unroll
           for (int u = 0; u < kUnitsX; ++u) seen += wx[u][1] ^ wx[u][2];
-        wait_read(seen);
+        return wait_read(seen, copied_in);
       };
       if constexpr (kVec) {
-        ok = mbar_wait_sleep(raw_full + 8 * sl, (k / kAhead) & 1, abort, a.err, DEV_TIMEOUT_FULL,
-                             a.limit);
-        if (!ok) break;
+        const bool here = mbar_wait_sleep(raw_full + 8 * sl, (k / kAhead) & 1, abort, a.err,
+                                          DEV_TIMEOUT_FULL, a.limit);
 #pragma unroll
         for (int u = 0; u < kUnitsX; ++u)
           ld_shared16(raw + kRaw - kBlock / 2 + (u * kRowsX + xr) * 64 + xj * 16, wx[u]);
@@ -530,7 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             ld_shared16(swizzled(raw, i * kRowsD + dr, dj), wd[i]);
           }
         }
-        read_all();
+        ok = read_all(here);
+        if (!ok) break;
         __syncwarp();
         if (lane == 0) mbar_arrive(raw_empty + 8 * sl);
       } else {
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ld_shifted<4>(from, wd[i]);
           }
         }
-        read_all();
+        read_all(true);
         __syncwarp();
         copy_chunk();
         if (cur.in * kChunk + kChunk > a.p) {  // a row's last chunk
@@ -571,8 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         cur.next();
       }
       if (k >= kStages) {
-        ok = mbar_wait_sleep(empty + 8 * st, (k / kStages - 1) & 1, abort, a.err, DEV_TIMEOUT_EMPTY,
-                             a.limit);
+        ok = wait(empty + 8 * st, k / kStages - 1, DEV_TIMEOUT_EMPTY);
         if (!ok) break;
       }
 #pragma unroll
