@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(kDsThreads + 32, 1)
       float2 v[4][2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) load_col(src, j, v[j]);
+      fence_proxy_async_smem();  // the reads are ahead of the copy that the arrival allows
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
       if (++stage == kDsStages) {
