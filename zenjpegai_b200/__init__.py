@@ -333,8 +333,9 @@ class Engine:
     # ---- training operators: 8-bit tapes and what reads them (tape.py) --------------------
     def tape_pack(self, x):
         """Hold a map in 8 bits: x [(n,) c, h, w] -> Tape, one power-of-two scale per group of 32
-        positions of a channel row (error at most half a step; a step is 2^-6 of the group's
-        largest magnitude rounded down to a power of two)."""
+        positions of a channel row. A step is 2^-6 of the group's largest magnitude rounded down to
+        a power of two; the error is at most half a step, a whole one above 127 steps, where codes
+        end."""
         return _tape.tape_pack(self, x)
 
     def tape_unpack(self, tape, dtype=None):

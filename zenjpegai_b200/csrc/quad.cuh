@@ -132,8 +132,7 @@ __device__ __forceinline__ uint32_t amax4(F4 v) {
 // largest 1 / 128 of magnitudes can round to 128, and a marked group has no codes: a warp that has
 // neither (one of 30 or so has) saves the clamps.
 __device__ __forceinline__ uint32_t codes4(F4 v, uint32_t m) {
-  const int e = max((int)(m >> 23) - 133, -126);
-  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  const float inv = tape_inv_scale(max((int)(m >> 23) - 133, -126));
   F4 c = fma4(v, all(inv), all(12582912.f));  // see tape_code_bits
   if (__any_sync(0xffffffffu, (m & 0x7fffffu) >= 0x7f0000u || m >= 0x7f800000u)) {
     const float none = m >= 0x7f800000u ? 0.f : inv;

@@ -21,9 +21,11 @@
 // squared deviations per warp, joined by their exact update formula (sums of squares would cancel).
 // The products in a - mean a and b - mean b are the ones that were summed (not fused): with one
 // channel they cancel to zero.
-// Measured at 28 x 128 x 128^2 in f32 with a full gate: forward with four tapes 296 us of kernel,
-// 5.2 TB/s, and backward from tapes 435 us, 3.1 TB/s: the sixteen warps an SM that the registers
-// leave issue every other cycle, each waiting on its own latencies between the exchanges.
+// Measured at 28 x 128 x 128^2 with a full gate, kernels alone: f32 forward with four tapes 285 us,
+// 5.0 TB/s, and backward from tapes 428 us, 3.2 TB/s: the sixteen warps an SM that the registers
+// leave issue every other cycle, each waiting on its own latencies between the exchanges. So bf16,
+// with half of the bytes and the same instructions, is hardly faster: forward without tapes 173 us
+// (f32 195), backward 383 us.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -43,7 +45,11 @@ constexpr int kMaxCluster = 8;
 
 // sigmoid(g) and sigmoid(g) (1 - sigmoid(g)), an even function of g: with a = exp(-|g|) and
 // r = 1 / (1 + a), sigmoid is r or a r and the product a r^2, nothing by cancellation and both finite
-// for every g but NaN.
+// for every g but NaN. __expf's documented error is 2 + floor(1.16 |g|) units in the last place: where
+// it grows, at large |g|, what carries it (sigmoid's small side, the slope) is as small as exp(-|g|)
+// itself: at |g| = 20 some 25 units, 3e-6 of values of 2e-9. expf took 2 to 6 % longer (28 x 128 x
+// 128^2, full gate, a call: f32 forward with tapes read back 402 and 412 us, backward 437 and 449; bf16
+// forward 171 and 182, backward 384 and 402). __fdividef's two units are as many as the sums' own.
 __device__ __forceinline__ void sigmoid2(float g, float* s, float* slope) {
   const float a = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + a), ar = a * r;
   *s = g >= 0.f ? r : ar;
@@ -109,11 +115,12 @@ struct Cluster {
 };
 
 // The block's partial sums per warp and position, and their totals: written by the warps, cl.sync(),
-// joined, cl.sync() (no block sums them any more). Then a warp may use its own rows as it likes, 128 B
-// each.
+// joined, cl.sync() (no block sums them any more). Then a warp may use its own as scratch.
+constexpr int kScratchBytes = 256;  // of a warp, from at(0, warp) on: 128 halves
 template <int kVals>
 struct Exchange {
   static constexpr int kPitch = kVals * 32 + 8;  // per warp; the lanes of a join meet no bank twice
+  static_assert(kScratchBytes <= kPitch * (int)sizeof(float), "scratch reaches the next warp's sums");
   float *part, *totals;
   __device__ __forceinline__ float* at(int val, int w) const { return part + w * kPitch + val * 32; }
   __device__ __forceinline__ float* total(int val) const { return totals + val * 32; }
@@ -502,6 +509,7 @@ __device__ __forceinline__ void store_if(T* to, T v, uint32_t on) {
 template <class T, class F>
 __device__ __forceinline__ void scatter(T* map, F&& put, const StagedRows<kAnywhere>& row, int j, int nv,
                                         float* scratch) {
+  static_assert(4 * 32 * sizeof(T) <= kScratchBytes, "four rows of halves or codes");
   const int lane = threadIdx.x & 31;
   const uint32_t in = row.in_tile(nv);
   T* s = reinterpret_cast<T*>(scratch);
@@ -512,7 +520,8 @@ __device__ __forceinline__ void scatter(T* map, F&& put, const StagedRows<kAnywh
 #pragma unroll
   for (int r = 0; r < 4; ++r, to += row.p) store_if(to, s[r * 32 + lane], in & 1u << (4 * j + r));
 }
-// four positions of the rows of step j to a map (scratch: 512 B of the warp, for kAnywhere)
+// four positions of the rows of step j to a map (scratch: kScratchBytes of the warp, for halves of
+// kAnywhere)
 template <int kMode, class T>
 __device__ __forceinline__ void staged_store(T* map, F4 v, const StagedRows<kMode>& row, int j, int nv,
                                              float* scratch) {

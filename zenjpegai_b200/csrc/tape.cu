@@ -1,7 +1,7 @@
 // 8-bit activation tapes (zjai_tape_pack, zjai_tape_unpack): the format is in tape.cuh. Both
 // directions are one pass over the map, bound by HBM: per element the map's 4 or 2 bytes plus
-// 1 + 1/32 for the tape. 28 x 1024 x 128^2 f16, packed and unpacked: 429 us, 6.6 TB/s, the speed of a
-// plain copy.
+// 1 + 1/32 for the tape. 28 x 1024 x 128^2 f16, packed and unpacked: 429 to 439 us, 6.5 TB/s and more,
+// the speed of a plain copy.
 //
 // Groups lie one behind the other in memory. Where all are whole (rows of a multiple of 32
 // positions) a thread has eight neighbouring positions (four lanes a group) and several such pieces
@@ -9,7 +9,8 @@
 // anywhere. Packing, a block copies its run of groups to shared memory by aligned 16 bytes, works on
 // it with eight lanes a group, and stores the codes by 16 bytes again. Unpacking, a lane has four
 // neighbouring elements, whatever groups they are of. (With eight lanes a group at global memory
-// both together took 51 us on f32, 8 x 128 x 127 x 129, and 52 us on f16; now 46 and 43.)
+// both calls together took 51 us on f32, 8 x 128 x 127 x 129, and 52 us on f16; now 46 and 43, of which
+// the kernels take 24 and 18 in either type: instructions bound them, not the bytes' 26 and 16 us.)
 #include <algorithm>
 
 #include "quad.cuh"
@@ -92,7 +93,8 @@ __global__ void __launch_bounds__(256) tape_unpack_flat_kernel(const int8_t* __r
   }
 }
 
-// n / d for n < 2^31, by a multiplication
+// n / d for n < 2^31, by a multiplication (Granlund and Montgomery, "Division by invariant integers
+// using multiplication", 1994: the quotient's multiplier has 33 bits, its top one added as n)
 struct Div {
   uint32_t magic, shift, d;
   explicit Div(uint32_t d_) : shift(0), d(d_) {

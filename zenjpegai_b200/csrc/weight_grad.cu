@@ -28,9 +28,11 @@
 //  - one thread issues the MMAs of a chunk, alternating between two accumulator sets in TMEM;
 //  - db comes from the converters' registers, or, where d_out does not pass through them, from a
 //    row of ones below the input's rows in the operand: one more column of the product.
-// At 28 x 128 x 128^2: f32 to 384 channels 204 us (3.7 TB/s; its copies alone take 154), bf16 to 1024
-// 242 us (4.1 TB/s; 198): what is left is a chunk's way through conversion while its places in shared
-// memory are taken.
+// At 28 x 128 x 128^2, the kernel alone: f32 to 384 channels 210 us (3.6 TB/s; its copies alone take
+// 154), f16 164 us, bf16 to 1024 241 us (4.1 TB/s; 198): what is left is a chunk's way through
+// conversion while its places in shared memory are taken. The sums of the shares take 12 to 14 us
+// more (f32 224 us a call, bf16 258). Call after call for seconds f32 settles at 245 us and bf16 at 290:
+// the card is at its 1000 W limit then, and the SMs at 1.6 GHz of 1.965.
 // Shares of one tile are summed in order by a second kernel (no atomics). Every wait is bounded
 // (zjai_ctx_set_wait_limit); a role whose time is up has the others give up too, and the CTA ends once
 // its copies and MMAs in flight have.
@@ -55,9 +57,10 @@ constexpr int kBufCols = 256;              // TMEM columns of an accumulator set
 // Per element type and alignment: bf16 terms of a d_out element; groups of converter warps, which
 // take every kGroups-th chunk; stages of converted operands and chunks copied ahead of them; chunks
 // between drains. A chunk has a fixed cost of waits and hand-offs per warp, which groups hide where
-// there are chunks enough in shared memory (28 x 128 x 128^2: f16 to 384 channels 163 us with two
-// groups, 171 with one; bf16 to 1024 242 us with four, a tenth more with one); f32's few and large
-// ones are done with sooner by all warps at once (to 384: 204 us with one group, 230 with two).
+// there are chunks enough in shared memory (28 x 128 x 128^2, the kernel alone: f16 to 384 channels
+// 163 us with two groups, 171 with one; bf16 to 1024 242 us with four, a tenth more with one); f32's
+// few and large ones are done with sooner by all warps at once (to 384: a ninth sooner than by two
+// groups).
 template <bool kVec, class T>
 struct Form;
 template <>
